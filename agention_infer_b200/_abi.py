@@ -73,6 +73,14 @@ SIGNATURES = {
     "agn_kv_write_f32": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i64]),
     "agn_kv_read_f32": (_i32, [_vp, _i32, _vp, _vp, _i64, _i64, _vp, _vp]),
     "agn_kv_bytes_per_token": (_i64, [_i32, _i64]),
+    "agn_attention_kv_workspace_bytes": (_i64, [_i64, _i32, _i32, _i32, _i64, _i32]),
+    "agn_attention_kv_f32": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _i64, _i64, _f32, _vp, _sz]),
+    "agn_attention_kv_f16": (_i32, [_vp, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _i64, _i64, _f32, _vp, _sz]),
+    "agn_gated_delta_rule_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "agn_gated_delta_rule_f32": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i64, _i64,
+                                        _i64, _f32, _f32, _vp, _sz]),
+    "agn_rms_norm_silu_gate_f32": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32]),
+    "agn_rms_norm_silu_gate_f32_out16": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32]),
     "agn_router_top2_f32": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp]),
     "agn_gather_rows_by_expert_f32": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
     "agn_silu_mul_f16": (_i32, [_vp, _vp, _vp, _vp, _i64]),

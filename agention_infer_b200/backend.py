@@ -55,6 +55,12 @@ def _ptr(obj) -> Optional[int]:
     return int(obj.data_ptr())  # DeviceBuffer or torch CUDA tensor
 
 
+def _nbytes(obj) -> int:
+    if obj is None:
+        return 0
+    return obj.nbytes if isinstance(obj, DeviceBuffer) else obj.numel() * obj.element_size()  # DeviceBuffer or torch tensor
+
+
 class CudaBackend:
     """One GPU, one stream.  Replaces `create_backend(BackendPreference::Cuda)`
     (src/ops/backend_select.rs:60-108), whose Cuda arm silently falls back to CPU."""
@@ -346,6 +352,70 @@ class CudaBackend:
         self._check(self._lib.agn_kv_read_f32(self._ctx, kv_dtype, _ptr(k_cache), _ptr(v_cache), n_pos, head_dim_kv,
                                               _ptr(k_out), _ptr(v_out)))
         return k_out, v_out
+
+    # ------------------------------------------------------------ token mixers
+    def attention_kv_workspace_bytes(self, T: int, n_q_heads: int, n_kv_heads: int, head_dim: int, max_seq_len: int,
+                                     has_pos: bool) -> int:
+        """Device bytes `launch_attention_kv` needs beside its buffers for a call of these sizes."""
+        return int(self._lib.agn_attention_kv_workspace_bytes(T, n_q_heads, n_kv_heads, head_dim, max_seq_len, int(has_pos)))
+
+    def launch_attention_kv(self, q, k_cache, v_cache, kv_dtype: int, T: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
+                            max_seq_len: int, pos=None, pos_start: int = 0, seq=None, n_seqs: int = 1,
+                            scale: Optional[float] = None, act_dtype: int = AGN_F32, out=None, workspace=None):
+        """`launch_attention` (resident.rs:551-565) for T rows over the cache `kv_write` filled: row t sees slots 0..pos[t] of
+        sequence seq[t] (device int32 arrays), or, without `pos`, slots 0..pos_start + t of the one sequence.  q, out:
+        [T, n_q_heads, head_dim] f32 or f16 (`act_dtype`); scale None: 1 / sqrt(head_dim).  `workspace` (a buffer of
+        `attention_kv_workspace_bytes`) is allocated per call if it is not given."""
+        if act_dtype not in (AGN_F32, AGN_F16):
+            raise ValueError(f"activations are f32 or f16, not dtype {act_dtype}")
+        if out is None:
+            out = self.empty((4 if act_dtype == AGN_F32 else 2) * T * n_q_heads * head_dim)
+        if workspace is None:
+            need = self.attention_kv_workspace_bytes(T, n_q_heads, n_kv_heads, head_dim, max_seq_len, pos is not None)
+            workspace = self.empty(need) if need else None
+        fn = self._lib.agn_attention_kv_f32 if act_dtype == AGN_F32 else self._lib.agn_attention_kv_f16
+        self._check(fn(self._ctx, _ptr(q), _ptr(out), kv_dtype, _ptr(k_cache), _ptr(v_cache), T, n_q_heads, n_kv_heads, head_dim,
+                       _ptr(pos), pos_start, _ptr(seq), n_seqs, max_seq_len, head_dim ** -0.5 if scale is None else scale,
+                       _ptr(workspace), _nbytes(workspace)))
+        return out
+
+    def gated_delta_rule_workspace_bytes(self, T: int, n_seqs: int, n_k_heads: int, n_v_heads: int, head_k: int, head_v: int) -> int:
+        """Device bytes `launch_gated_delta_rule` needs beside its buffers for a call of these sizes."""
+        return int(self._lib.agn_gated_delta_rule_workspace_bytes(T, n_seqs, n_k_heads, n_v_heads, head_k, head_v))
+
+    def launch_gated_delta_rule(self, q, k, v, g, beta, state, T: int, n_seqs: int, n_k_heads: int, n_v_heads: int, head_k: int,
+                                head_v: int, cu_seqlens=None, scale: Optional[float] = None, l2norm_eps: float = 1e-6,
+                                q_stride: Optional[int] = None, k_stride: Optional[int] = None, v_stride: Optional[int] = None,
+                                state_out=None, out=None, workspace=None) -> Tuple:
+        """The recurrence of a GatedDeltaNet layer (cpu_path.rs:397-688) over the rows of n_seqs sequences (cu_seqlens: device int32
+        offsets; None: equal lengths).  state [n_seqs, n_v_heads, head_k, head_v] or None for zeros; returns (out, state_out)."""
+        if out is None:
+            out = self.empty(4 * max(T, 1) * n_v_heads * head_v)
+        if state_out is None:
+            state_out = self.empty(4 * n_seqs * n_v_heads * head_k * head_v)
+        if workspace is None:
+            need = self.gated_delta_rule_workspace_bytes(T, n_seqs, n_k_heads, n_v_heads, head_k, head_v)
+            workspace = self.empty(need) if need else None
+        self._check(self._lib.agn_gated_delta_rule_f32(
+            self._ctx, _ptr(q), _ptr(k), _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(state_out), _ptr(out), T, n_seqs,
+            _ptr(cu_seqlens), n_k_heads, n_v_heads, head_k, head_v, n_k_heads * head_k if q_stride is None else q_stride,
+            n_k_heads * head_k if k_stride is None else k_stride, n_v_heads * head_v if v_stride is None else v_stride,
+            head_k ** -0.5 if scale is None else scale, l2norm_eps, _ptr(workspace), _nbytes(workspace)))
+        return out, state_out
+
+    def launch_rms_norm_silu_gate(self, x, gate, w, rows: int, n: int, eps: float, out=None):
+        """The gated norm behind a recurrent mixer: rms_norm(x, w) * silu(gate) over rows of one head each."""
+        if out is None:
+            out = self.empty(4 * rows * n)
+        self._check(self._lib.agn_rms_norm_silu_gate_f32(self._ctx, _ptr(x), _ptr(gate), _ptr(w), _ptr(out), rows, n, eps))
+        return out
+
+    def launch_rms_norm_silu_gate_out16(self, x, gate, w, rows: int, n: int, eps: float, out_dtype: int, out=None):
+        """The same with the result stored as f16 / bf16 (the operand of a half-precision output projection)."""
+        if out is None:
+            out = self.empty(2 * rows * n)
+        self._check(self._lib.agn_rms_norm_silu_gate_f32_out16(self._ctx, _ptr(x), _ptr(gate), _ptr(w), _ptr(out), rows, n, eps, out_dtype))
+        return out
 
     def router_top2(self, logits, T: int, n_experts: int, idx=None, w=None):
         """MoE router: softmax + top-2 per token (docs/08-moe-routing.md:27-33). Returns (idx [T,2] i32, w [T,2] f32)."""

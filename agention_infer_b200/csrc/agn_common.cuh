@@ -17,6 +17,8 @@
 #define AGN_FLAG_TIMEOUT 2u      // a bounded staging wait gave up
 #define AGN_FLAG_OOB_EXPERT 4u   // gather_rows_by_expert: expert index outside [0, n_experts)
 #define AGN_FLAG_OOB_SLOT 8u     // kv_write / fused cache write: position outside [0, max_seq_len)
+#define AGN_FLAG_OOB_ATTN 16u    // attention_kv: position outside [-1, max_seq_len) or sequence outside [0, n_seqs)
+#define AGN_FLAG_BAD_SEQLENS 32u // gated_delta_rule: sequence offsets outside [0, T] or out of order
 
 // Polls of an mbarrier before a staging wait gives up (a few hundred ms at most); the option
 // "mbar_spin_limit" overrides it per context.

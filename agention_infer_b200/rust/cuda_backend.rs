@@ -368,6 +368,64 @@ impl CudaBackend {
         })
     }
 
+    /// `launch_attention` (src/ops/wgpu_backend/resident.rs:551-565) over one layer's cache: token `i` of `t` sees slots
+    /// `0..=pos_start + i`.  `workspace` holds `attention_workspace_bytes(..)` bytes (`None` if that is 0).
+    #[allow(clippy::too_many_arguments)]
+    pub fn launch_attention_kv(&self, q: &DevBuf, kv_dtype: i32, k_cache: &DevBuf, v_cache: &DevBuf, t: usize, n_q_heads: usize,
+                               n_kv_heads: usize, head_dim: usize, pos_start: usize, max_seq_len: usize, scale: f32,
+                               workspace: Option<&DevBuf>) -> Result<DevBuf> {
+        let out = self.empty(4 * t * n_q_heads * head_dim)?;
+        self.check(unsafe {
+            agn_attention_kv_f32(self.ctx, q.ptr as *const f32, out.ptr as *mut f32, kv_dtype, k_cache.ptr as *const c_void,
+                                 v_cache.ptr as *const c_void, t as i64, n_q_heads as i32, n_kv_heads as i32, head_dim as i32,
+                                 std::ptr::null(), pos_start as i32, std::ptr::null(), 1, max_seq_len as i64, scale,
+                                 workspace.map_or(std::ptr::null_mut(), |b| b.ptr), workspace.map_or(0, |b| b.bytes))
+        })?;
+        Ok(out)
+    }
+
+    /// Bytes of workspace `launch_attention_kv` needs for a call of these sizes.
+    pub fn attention_workspace_bytes(t: usize, n_q_heads: usize, n_kv_heads: usize, head_dim: usize, max_seq_len: usize) -> usize {
+        unsafe {
+            agn_attention_kv_workspace_bytes(t as i64, n_q_heads as i32, n_kv_heads as i32, head_dim as i32, max_seq_len as i64, 0) as usize
+        }
+    }
+
+    /// The gated delta rule of a linear-attention layer (cpu_path.rs:397-688) over `t` rows of one sequence, q and k normalised;
+    /// `state` `[n_v_heads, head_k, head_v]` is advanced in place.
+    #[allow(clippy::too_many_arguments)]
+    pub fn launch_gated_delta_rule(&self, q: &DevBuf, k: &DevBuf, v: &DevBuf, g: &DevBuf, beta: &DevBuf, state: &DevBuf, t: usize,
+                                   n_k_heads: usize, n_v_heads: usize, head_k: usize, head_v: usize, scale: f32, eps: f32,
+                                   workspace: Option<&DevBuf>) -> Result<DevBuf> {
+        let out = self.empty(4 * t * n_v_heads * head_v)?;
+        self.check(unsafe {
+            agn_gated_delta_rule_f32(self.ctx, q.ptr as *const f32, k.ptr as *const f32, v.ptr as *const f32, g.ptr as *const f32,
+                                     beta.ptr as *const f32, state.ptr as *const f32, state.ptr as *mut f32, out.ptr as *mut f32,
+                                     t as i64, 1, std::ptr::null(), n_k_heads as i32, n_v_heads as i32, head_k as i32,
+                                     head_v as i32, (n_k_heads * head_k) as i64, (n_k_heads * head_k) as i64,
+                                     (n_v_heads * head_v) as i64, scale, eps,
+                                     workspace.map_or(std::ptr::null_mut(), |b| b.ptr), workspace.map_or(0, |b| b.bytes))
+        })?;
+        Ok(out)
+    }
+
+    /// Bytes of workspace `launch_gated_delta_rule` needs for a call of these sizes.
+    pub fn gated_delta_rule_workspace_bytes(t: usize, n_k_heads: usize, n_v_heads: usize, head_k: usize, head_v: usize) -> usize {
+        unsafe {
+            agn_gated_delta_rule_workspace_bytes(t as i64, 1, n_k_heads as i32, n_v_heads as i32, head_k as i32, head_v as i32) as usize
+        }
+    }
+
+    /// The gated norm behind it: `rms_norm(x, w) * silu(gate)` over `rows` rows of `n` values.
+    pub fn launch_rms_norm_silu_gate(&self, x: &DevBuf, gate: &DevBuf, w: &DevBuf, rows: usize, n: usize, eps: f32) -> Result<DevBuf> {
+        let out = self.empty(4 * rows * n)?;
+        self.check(unsafe {
+            agn_rms_norm_silu_gate_f32(self.ctx, x.ptr as *const f32, gate.ptr as *const f32, w.ptr as *const f32,
+                                       out.ptr as *mut f32, rows as i64, n as i64, eps)
+        })?;
+        Ok(out)
+    }
+
     /// Router logits `[t, n_experts]` -> the two largest per token (ties to the lower index) and
     /// their softmax probabilities, not renormalised (docs/08-moe-routing.md:27-33).
     pub fn router_top2(&self, logits: &DevBuf, t: usize, n_experts: usize) -> Result<(DevBuf, DevBuf)> {

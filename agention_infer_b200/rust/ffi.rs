@@ -96,6 +96,13 @@ extern "C" {
     pub fn agn_qk_norm_rope_kv_write_f32(ctx: *mut AgnCtx, q: *mut f32, k: *mut f32, v: *const f32, wq: *const f32, wk: *const f32, T: i64, n_q_heads: i32, n_kv_heads: i32, head_dim: i32, eps: f32, n_rot: i32, pos: *const i32, pos_start: i32, theta: f32, freq_scale: f32, layout: i32, kv_dtype: i32, k_cache: *mut c_void, v_cache: *mut c_void, max_seq_len: i64) -> i32;
     pub fn agn_kv_read_f32(ctx: *mut AgnCtx, kv_dtype: i32, k_cache: *const c_void, v_cache: *const c_void, n_pos: i64, head_dim_kv: i64, k_out: *mut f32, v_out: *mut f32) -> i32;
     pub fn agn_kv_bytes_per_token(kv_dtype: i32, head_dim_kv: i64) -> i64;
+    pub fn agn_attention_kv_workspace_bytes(T: i64, n_q_heads: i32, n_kv_heads: i32, head_dim: i32, max_seq_len: i64, has_pos: i32) -> i64;
+    pub fn agn_attention_kv_f32(ctx: *mut AgnCtx, q: *const f32, out: *mut f32, kv_dtype: i32, k_cache: *const c_void, v_cache: *const c_void, T: i64, n_q_heads: i32, n_kv_heads: i32, head_dim: i32, pos: *const i32, pos_start: i32, seq: *const i32, n_seqs: i64, max_seq_len: i64, scale: f32, workspace: *mut c_void, workspace_bytes: usize) -> i32;
+    pub fn agn_attention_kv_f16(ctx: *mut AgnCtx, q: *const c_void, out: *mut c_void, kv_dtype: i32, k_cache: *const c_void, v_cache: *const c_void, T: i64, n_q_heads: i32, n_kv_heads: i32, head_dim: i32, pos: *const i32, pos_start: i32, seq: *const i32, n_seqs: i64, max_seq_len: i64, scale: f32, workspace: *mut c_void, workspace_bytes: usize) -> i32;
+    pub fn agn_gated_delta_rule_workspace_bytes(T: i64, n_seqs: i64, n_k_heads: i32, n_v_heads: i32, head_k: i32, head_v: i32) -> i64;
+    pub fn agn_gated_delta_rule_f32(ctx: *mut AgnCtx, q: *const f32, k: *const f32, v: *const f32, g: *const f32, beta: *const f32, state_in: *const f32, state_out: *mut f32, out: *mut f32, T: i64, n_seqs: i64, cu_seqlens: *const i32, n_k_heads: i32, n_v_heads: i32, head_k: i32, head_v: i32, q_stride: i64, k_stride: i64, v_stride: i64, scale: f32, l2norm_eps: f32, workspace: *mut c_void, workspace_bytes: usize) -> i32;
+    pub fn agn_rms_norm_silu_gate_f32(ctx: *mut AgnCtx, x: *const f32, gate: *const f32, w: *const f32, out: *mut f32, rows: i64, n: i64, eps: f32) -> i32;
+    pub fn agn_rms_norm_silu_gate_f32_out16(ctx: *mut AgnCtx, x: *const f32, gate: *const f32, w: *const f32, out: *mut c_void, rows: i64, n: i64, eps: f32, out_dtype: i32) -> i32;
     pub fn agn_router_top2_f32(ctx: *mut AgnCtx, logits: *const f32, T: i64, n_experts: i32, idx: *mut i32, w: *mut f32) -> i32;
     pub fn agn_gather_rows_by_expert_f32(ctx: *mut AgnCtx, x: *const f32, idx: *const i32, T: i64, H: i64, n_experts: i32, out: *mut f32, offsets: *mut i32, src_token: *mut i32, src_slot: *mut i32) -> i32;
     pub fn agn_silu_mul_f16(ctx: *mut AgnCtx, gate: *const c_void, up: *const c_void, out: *mut c_void, n: i64) -> i32;

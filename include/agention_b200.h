@@ -337,6 +337,70 @@ AGN_API int32_t agn_kv_read_f32(agn_ctx *ctx, int32_t kv_dtype, const void *k_ca
 /* `KvDtype::bytes_per_token` (src/model/mod.rs:550-556); 0 for an unknown dtype. */
 AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
 
+/* ------------------------------------------------------------------ token mixers */
+
+/* Attention of T query rows over the KV cache that agn_kv_write_f32 / agn_qk_norm_rope_kv_write_f32 fill:
+ * `launch_attention` (src/ops/wgpu_backend/resident.rs:551-565; `attention_scores`, `attention_softmax`,
+ * `attention_output` and their `_q8_0` forms, src/ops/kernels_wgpu.rs:749-980), CPU `attention_into`
+ * (src/model/llama/cpu_path.rs:160-192), without the scores in memory:
+ *   out[t,h] = sum_j softmax_j(scale * q[t,h] . K[s,j,h/G]) V[s,j,h/G],  j = 0 .. p,  G = n_q_heads / n_kv_heads
+ * q, out: [T, n_q_heads, head_dim], f32 or f16 (the accumulation and the softmax are f32 in both); caches: n_seqs
+ * sequences of [max_seq_len, agn_kv_bytes_per_token(kv_dtype, n_kv_heads * head_dim)] bytes, one after the other;
+ * kv_dtype AGN_F16, AGN_Q8_0 or AGN_KV_Q8_0_WORDS.  Two forms:
+ *   pos != NULL: row t is the token of position p = pos[t] (device int32) of sequence s = seq[t] (device int32; NULL:
+ *     sequence 0) — the decode step of many conversations.  p = -1 sees nothing: its row is 0.  A position outside
+ *     [-1, max_seq_len) or a sequence outside [0, n_seqs) gives a row of zeros and makes the next agn_sync return AGN_EOOB_ID.
+ *   pos == NULL: the rows are the positions pos_start + t of the one sequence the caches hold — a prompt, or a
+ *     piece of one, whose own keys are already in the cache (seq must be NULL, pos_start + T <= max_seq_len).
+ * What the cache holds in slots that a row does not see, infinities and NaN included, does not change that row.
+ * head_dim: a multiple of 32 up to 256; scale > 0 and finite; q and out 16-byte aligned and not the same buffer.
+ * workspace: at least agn_attention_kv_workspace_bytes(...) bytes of device memory, 16-byte aligned, whose contents
+ * need not be kept between calls; calls that can overlap on the GPU need a workspace each.  NULL if that is 0.
+ * The function takes the call's own sizes (has_pos: pos != NULL), needs no context and returns 0 for sizes the op refuses. */
+AGN_API int64_t agn_attention_kv_workspace_bytes(int64_t T, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                                 int64_t max_seq_len, int32_t has_pos);
+AGN_API int32_t agn_attention_kv_f32(agn_ctx *ctx, const float *q, float *out, int32_t kv_dtype, const void *k_cache,
+                                     const void *v_cache, int64_t T, int32_t n_q_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, const int32_t *pos, int32_t pos_start, const int32_t *seq,
+                                     int64_t n_seqs, int64_t max_seq_len, float scale, void *workspace,
+                                     size_t workspace_bytes);
+AGN_API int32_t agn_attention_kv_f16(agn_ctx *ctx, const void *q, void *out, int32_t kv_dtype, const void *k_cache,
+                                     const void *v_cache, int64_t T, int32_t n_q_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, const int32_t *pos, int32_t pos_start, const int32_t *seq,
+                                     int64_t n_seqs, int64_t max_seq_len, float scale, void *workspace,
+                                     size_t workspace_bytes);
+
+/* The gated delta rule of the linear-attention layers (GatedDeltaNet, src/model/llama/cpu_path.rs:397-688, kernels
+ * src/ops/kernels_wgpu.rs:331-559) over the rows of n_seqs sequences.  Per value head h, with a state S [head_k, head_v]:
+ *   S_t = a_t S_(t-1) + k_t d_t^T,  d_t = beta_t (v_t - a_t S_(t-1)^T k_t),  o_t = S_t^T q_t,  a_t = exp(g_t)
+ * q, k: rows of [n_k_heads, head_k], value head h uses head h / (n_v_heads / n_k_heads); v: rows of [n_v_heads, head_v];
+ * q_stride, k_stride, v_stride: floats from row to row (so the three can be parts of one projection's row), multiples
+ * of 4; g, beta: [T, n_v_heads]; out: [T, n_v_heads, head_v], none of q, k, v; all f32.  l2norm_eps >= 0: q and k are
+ * multiplied by 1 / sqrt(sum of squares + l2norm_eps) first; < 0: taken as they are.  q is also multiplied by `scale`.  The decay is
+ * meant to be one: g <= 0.
+ * state_in [n_seqs, n_v_heads, head_k, head_v] (NULL: zeros) -> state_out, which may be the same buffer.
+ * cu_seqlens: device int32 [n_seqs + 1], sequence s is the rows cu_seqlens[s] .. cu_seqlens[s+1] (none: its state is copied);
+ * NULL: T / n_seqs rows each.  Rows behind the last sequence are left as they are.  Offsets outside [0, T] or out of order are cut
+ * and make the next agn_sync return AGN_EOOB_ID.
+ * head_k 64 or 128, head_v a multiple of 32 up to 256.  workspace as in agn_attention_kv_f32. */
+AGN_API int64_t agn_gated_delta_rule_workspace_bytes(int64_t T, int64_t n_seqs, int32_t n_k_heads, int32_t n_v_heads,
+                                                     int32_t head_k, int32_t head_v);
+AGN_API int32_t agn_gated_delta_rule_f32(agn_ctx *ctx, const float *q, const float *k, const float *v, const float *g,
+                                         const float *beta, const float *state_in, float *state_out, float *out,
+                                         int64_t T, int64_t n_seqs, const int32_t *cu_seqlens, int32_t n_k_heads,
+                                         int32_t n_v_heads, int32_t head_k, int32_t head_v, int64_t q_stride,
+                                         int64_t k_stride, int64_t v_stride, float scale, float l2norm_eps,
+                                         void *workspace, size_t workspace_bytes);
+
+/* The norm behind that mixer with its gate (gated norms, src/ops/kernels_wgpu.rs:175-214), over rows of one head each:
+ *   out[r,i] = (w[i] * x[r,i]) / sqrt(sum_i x[r,i]^2 / n + eps) * gate[r,i] / (1 + exp(-gate[r,i]))
+ * n: 1 .. 1024, any alignment of float (16-byte aligned rows are faster); out may be x or gate.  The _out16 form stores
+ * the f32 result rounded to f16 / bf16 (out_dtype), into a buffer of its own. */
+AGN_API int32_t agn_rms_norm_silu_gate_f32(agn_ctx *ctx, const float *x, const float *gate, const float *w, float *out,
+                                           int64_t rows, int64_t n, float eps);
+AGN_API int32_t agn_rms_norm_silu_gate_f32_out16(agn_ctx *ctx, const float *x, const float *gate, const float *w,
+                                                 void *out, int64_t rows, int64_t n, float eps, int32_t out_dtype);
+
 /* MoE router: softmax over the n_experts logits of each token and top-2 selection.  The
  * reference has no MoE forward pass; the semantics follow its design notes
  * (docs/08-moe-routing.md:27-33): weights are the softmax probabilities of the two picks,

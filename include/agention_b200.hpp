@@ -262,6 +262,35 @@ class CudaBackend {
         check(agn_kv_read_f32(ctx_, kv_dtype, k_cache, v_cache, n_pos, head_dim_kv, k_out, v_out));
     }
 
+    // ---- token mixers: attention over that cache (resident.rs:551-565), the gated delta rule and its gated norm
+    void launch_attention_kv(const float *q, float *out, int kv_dtype, const void *k_cache, const void *v_cache, int64_t T, int n_q,
+                             int n_kv, int head_dim, const int32_t *pos, int pos_start, const int32_t *seq, int64_t n_seqs,
+                             int64_t max_seq_len, float scale, void *workspace, size_t workspace_bytes) {
+        check(agn_attention_kv_f32(ctx_, q, out, kv_dtype, k_cache, v_cache, T, n_q, n_kv, head_dim, pos, pos_start, seq, n_seqs,
+                                   max_seq_len, scale, workspace, workspace_bytes));
+    }
+    void launch_attention_kv_f16(const void *q, void *out, int kv_dtype, const void *k_cache, const void *v_cache, int64_t T, int n_q,
+                                 int n_kv, int head_dim, const int32_t *pos, int pos_start, const int32_t *seq, int64_t n_seqs,
+                                 int64_t max_seq_len, float scale, void *workspace, size_t workspace_bytes) {
+        check(agn_attention_kv_f16(ctx_, q, out, kv_dtype, k_cache, v_cache, T, n_q, n_kv, head_dim, pos, pos_start, seq, n_seqs,
+                                   max_seq_len, scale, workspace, workspace_bytes));
+    }
+    void launch_gated_delta_rule(const float *q, const float *k, const float *v, const float *g, const float *beta,
+                                 const float *state_in, float *state_out, float *out, int64_t T, int64_t n_seqs,
+                                 const int32_t *cu_seqlens, int n_k, int n_v, int head_k, int head_v, int64_t q_stride,
+                                 int64_t k_stride, int64_t v_stride, float scale, float l2norm_eps, void *workspace,
+                                 size_t workspace_bytes) {
+        check(agn_gated_delta_rule_f32(ctx_, q, k, v, g, beta, state_in, state_out, out, T, n_seqs, cu_seqlens, n_k, n_v, head_k,
+                                       head_v, q_stride, k_stride, v_stride, scale, l2norm_eps, workspace, workspace_bytes));
+    }
+    void launch_rms_norm_silu_gate(const float *x, const float *gate, const float *w, float *out, int64_t rows, int64_t n, float eps) {
+        check(agn_rms_norm_silu_gate_f32(ctx_, x, gate, w, out, rows, n, eps));
+    }
+    void launch_rms_norm_silu_gate_out16(const float *x, const float *gate, const float *w, void *out, int64_t rows, int64_t n,
+                                         float eps, int out_dtype) {
+        check(agn_rms_norm_silu_gate_f32_out16(ctx_, x, gate, w, out, rows, n, eps, out_dtype));
+    }
+
     // ---- host slices, as the CPU path takes them (src/model/llama/cpu_path.rs:67,975-978)
     void rms_norm_into(const float *x_host, const float *w_dev, float *out_host, int64_t T, int64_t H, float eps) {
         check(agn_host_rms_norm_f32(ctx_, x_host, w_dev, out_host, T, H, eps));
