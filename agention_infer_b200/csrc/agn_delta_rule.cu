@@ -137,6 +137,594 @@ template <int DK> __global__ void __launch_bounds__(128) delta_recurrent_kernel(
     for (int i = 0; i < R; i++) *reinterpret_cast<float4 *>(a.state_out + soff + (int64_t)16 * i * a.dv) = S[i];
 }
 
+// ---- Chunked form, for prompts -----------------------------------------------------------------------------------------
+//
+// Inside a chunk of C = 64 rows, with c_i = a_1 ... a_i and r_ij = a_(j+1) ... a_i (products, so a decay of 0 needs no care):
+//   A_ij = beta_i r_ij k_i.k_j (i > j),   N = (I + A)^-1 diag(beta),   P_ij = r_ij q_i.k_j (i >= j)
+//   D = N (V - diag(c) K S),   O = diag(c) Q S + P D,   S' = c_C S + K^T diag(r_Cj) D
+// delta_prepare_kernel computes N, P, c, r_C and the normalised q and k of every chunk side by side; delta_chunk_kernel carries 32
+// columns of one head's state from chunk to chunk (the columns are independent: 128 CTAs for one sequence of 32 heads of 128).
+//
+// Bound by the matrix units: 1.05 M multiply-adds per chunk and 32 columns, three times over.  f32 operands are split into two f16
+// parts each, x = hi + lo (22 bits), and hi hi + hi lo + lo hi is summed in f32 by m16n8k16 (twice the rate of tf32's three
+// products; two tf32 parts would not need the scaling below).  f16's range is met by powers of two: |k|, |q| <= 1 and the
+// entries of N and P have known bounds; states and values are scaled by a power of two taken from their largest magnitude in front of
+// every chunk.  Those bounds hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that breaks them is
+// computed row by row in f32 instead.
+constexpr int CH = 64, CHUNK_THREADS = 256;
+constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals
+
+struct ChunkArgs {
+    DeltaArgs d;
+    __half *kq;    // [slots][n_k][k hi, k lo, q hi, q lo][64][head_k], times KQ_UP
+    __half *np;    // [slots][n_v][N hi, N lo, P hi, P lo][64][64], times NP_UP
+    float *decay;  // [slots][n_v][128]: c_i, then r_Cj
+    int *odd;      // [slots][n_v]: the chunk breaks the bounds
+};
+
+// A sequence's chunks have slots of their own: sequence s from slot b_s / 64 + s on.
+__device__ __forceinline__ int64_t delta_slot(int64_t begin, int64_t s) { return begin / CH + s; }
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
+}
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(agn_smem_u32(dst)), "l"(src) : "memory");
+}
+
+// One CTA per (chunk slot, key head); the value heads of the key head share its two products.
+template <int DK> struct PrepSmem {
+    static constexpr int ROW = DK + 8;  // f16 elements: 16 bytes off a multiple of 128, so that eight rows of a fragment do not collide
+    union {
+        __half op[4][CH * ROW];  // k hi, k lo, q hi, q lo
+        struct {
+            float kk[CH][CH + 1], qk[CH][CH + 1], r[CH][CH + 1], A[CH][CH + 1], N[CH][CH + 1], Y[3][16][17];
+        } t;
+    };
+    float a[CH], beta[CH], c[CH];
+    int odd_kq, odd;
+};
+
+template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare_kernel(ChunkArgs x) {
+    agn_pdl_prologue();
+    extern __shared__ __align__(128) unsigned char raw[];
+    PrepSmem<DK> &sm = *reinterpret_cast<PrepSmem<DK> *>(raw);
+    constexpr int ROW = PrepSmem<DK>::ROW;
+    const DeltaArgs &d = x.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hk = blockIdx.y;
+    const int64_t slot = blockIdx.x;
+    // the sequence: the last one that begins at or before this slot
+    int64_t lo = 0, hi = d.n_seqs - 1, b, e;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) / 2;
+        delta_rows(d, mid, &b, &e);
+        if (delta_slot(b, mid) <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    delta_rows(d, lo, &b, &e);
+    const int64_t first = b + (slot - delta_slot(b, lo)) * CH;
+    if (first < b || first >= e) return;
+    const int rows = (int)(e - first < CH ? e - first : CH);
+    if (tid == 0) sm.odd_kq = 0;
+    __syncthreads();
+
+    // q and k, a warp per row
+    constexpr int V = DK / 32;
+    for (int i = warp; i < CH; i += 8) {
+        float v[2][V], ss[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const float *src = w == 0 ? d.k + (first + i) * d.k_stride + hk * DK : d.q + (first + i) * d.q_stride + hk * DK;
+#pragma unroll
+            for (int j = 0; j < V / 2; j++) {
+                const float2 y = i < rows ? *reinterpret_cast<const float2 *>(src + 2 * (lane + 32 * j)) : make_float2(0.0f, 0.0f);
+                v[w][2 * j] = y.x;
+                v[w][2 * j + 1] = y.y;
+                ss[w] = __fmaf_rn(y.x, y.x, __fmaf_rn(y.y, y.y, ss[w]));
+            }
+            ss[w] = agn_warp_sum(ss[w]);
+            const float f = d.eps >= 0.0f ? rsqrtf(ss[w] + d.eps) : 1.0f;
+            // the normalised row's norm is at most 1 unless a sum of squares overflowed or was not a number
+            if (lane == 0 && !(d.eps >= 0.0f ? ss[w] < INFINITY && (ss[w] + d.eps > 0.0f || i >= rows) : ss[w] < 1.01f)) sm.odd_kq = 1;
+            __half *g = x.kq + (((slot * d.n_k + hk) * 4 + 2 * w) * CH + i) * DK;
+#pragma unroll
+            for (int j = 0; j < V / 2; j++) {
+                uint32_t h2, l2;
+                const float u = i < rows ? f * KQ_UP : 0.0f;
+                split2(v[w][2 * j] * u, v[w][2 * j + 1] * u, h2, l2);
+                const int at = 2 * (lane + 32 * j);
+                *reinterpret_cast<uint32_t *>(&sm.op[2 * w][i * ROW + at]) = h2;
+                *reinterpret_cast<uint32_t *>(&sm.op[2 * w + 1][i * ROW + at]) = l2;
+                *reinterpret_cast<uint32_t *>(g + at) = h2;
+                *reinterpret_cast<uint32_t *>(g + (int64_t)CH * DK + at) = l2;
+            }
+        }
+    }
+    __syncthreads();
+
+    // k k^T (warps 0-3) and q k^T (warps 4-7), 16 rows per warp, up to the diagonal
+    const int wm = warp & 3, which = warp >> 2, g = lane >> 2, t4 = lane & 3;
+    float acc[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+    for (int ks = 0; ks < DK / 16; ks++) {
+        uint32_t ah[4], al[4];
+        const int arow = (wm * 16 + (lane & 15)) * ROW + ks * 16 + (lane >> 4) * 8;
+        ldsm4(ah, &sm.op[2 * which][arow]);
+        ldsm4(al, &sm.op[2 * which + 1][arow]);
+#pragma unroll
+        for (int n = 0; n < 8; n += 2) {
+            if (n > 2 * wm + 1) break;
+            // k as the second operand: its rows are the columns of the product; two tiles of eight
+            uint32_t bh[4], bl[4];
+            const int brow = (n * 8 + (lane & 7) + (lane >> 4) * 8) * ROW + ks * 16 + ((lane >> 3) & 1) * 8;
+            ldsm4(bh, &sm.op[0][brow]);
+            ldsm4(bl, &sm.op[1][brow]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                mma16(acc[n + h], ah, bh[2 * h], bh[2 * h + 1]);
+                mma16(acc[n + h], ah, bl[2 * h], bl[2 * h + 1]);
+                mma16(acc[n + h], al, bh[2 * h], bh[2 * h + 1]);
+            }
+        }
+    }
+    __syncthreads();  // the operands are done with: the tables take their place
+    {
+        float(*to)[CH + 1] = which ? sm.t.qk : sm.t.kk;
+        constexpr float DOWN = 1.0f / (KQ_UP * KQ_UP);
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            to[wm * 16 + g][n * 8 + 2 * t4] = acc[n][0] * DOWN;
+            to[wm * 16 + g][n * 8 + 2 * t4 + 1] = acc[n][1] * DOWN;
+            to[wm * 16 + g + 8][n * 8 + 2 * t4] = acc[n][2] * DOWN;
+            to[wm * 16 + g + 8][n * 8 + 2 * t4 + 1] = acc[n][3] * DOWN;
+        }
+    }
+
+    const int ratio = d.n_v / d.n_k;
+    for (int hv = hk * ratio; hv < (hk + 1) * ratio; hv++) {
+        if (tid == 0) sm.odd = 0;
+        __syncthreads();
+        if (tid < CH) {
+            const int64_t at = (first + tid) * d.n_v + hv;
+            const float a = tid < rows ? expf(d.g[at]) : 1.0f, be = tid < rows ? d.beta[at] : 0.0f;
+            sm.a[tid] = a;
+            sm.beta[tid] = be;
+            if (!(a <= 1.0f) || !(be >= 0.0f && be <= 2.0f)) sm.odd = 1;
+        }
+        __syncthreads();
+        if (tid < CH) {
+            float r = 1.0f;
+            for (int i = 0; i < CH; i++) {
+                if (i > tid) r *= sm.a[i];
+                sm.t.r[i][tid] = i >= tid ? r : 0.0f;
+            }
+        } else if (tid == CH) {
+            float c = 1.0f;
+            for (int i = 0; i < CH; i++) sm.c[i] = c *= sm.a[i];
+        }
+        __syncthreads();
+        __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * CH;
+        for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
+            const int row = i >> 5, col = 2 * (i & 31);
+            const float r0 = sm.t.r[row][col], r1 = sm.t.r[row][col + 1], be = sm.beta[row];
+            sm.t.A[row][col] = row > col ? be * r0 * sm.t.kk[row][col] : 0.0f;
+            sm.t.A[row][col + 1] = row > col + 1 ? be * r1 * sm.t.kk[row][col + 1] : 0.0f;
+            sm.t.N[row][col] = sm.t.N[row][col + 1] = 0.0f;
+            uint32_t h2, l2;
+            split2(row >= col ? r0 * sm.t.qk[row][col] * NP_UP : 0.0f, row >= col + 1 ? r1 * sm.t.qk[row][col + 1] * NP_UP : 0.0f, h2, l2);
+            *reinterpret_cast<uint32_t *>(np + 2 * CH * CH + row * CH + col) = h2;
+            *reinterpret_cast<uint32_t *>(np + 3 * CH * CH + row * CH + col) = l2;
+        }
+        __syncthreads();
+        // (I + A)^-1: the four 16 x 16 blocks of the diagonal by substitution, a column per thread
+        if (tid < CH) {
+            const int o = tid & ~15, col = tid & 15;
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float s = i == col ? 1.0f : 0.0f;
+#pragma unroll
+                for (int l = 0; l < 16; l++)
+                    if (l < i) s = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s);
+                y[i] = s;
+                sm.t.N[o + i][o + col] = s;
+            }
+        }
+        __syncthreads();
+        // the blocks below it, distance by distance: N_ij = -N_ii sum_l A_il N_lj
+        const int br = tid >> 4, bc = tid & 15;
+        for (int dist = 1; dist < 4; dist++) {
+            for (int j = 0; j + dist < 4; j++) {
+                const int i = j + dist;
+                float s = 0.0f;
+                for (int l = 16 * j; l < 16 * i; l++) s = __fmaf_rn(sm.t.A[16 * i + br][l], sm.t.N[l][16 * j + bc], s);
+                sm.t.Y[j][br][bc] = s;
+            }
+            __syncthreads();
+            for (int j = 0; j + dist < 4; j++) {
+                const int i = j + dist;
+                float s = 0.0f;
+#pragma unroll
+                for (int l = 0; l < 16; l++) s = __fmaf_rn(-sm.t.N[16 * i + br][16 * i + l], sm.t.Y[j][l][bc], s);
+                sm.t.N[16 * i + br][16 * j + bc] = s;
+            }
+            __syncthreads();
+        }
+        for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
+            const int row = i >> 5, col = 2 * (i & 31);
+            uint32_t h2, l2;
+            split2(sm.t.N[row][col] * sm.beta[col] * NP_UP, sm.t.N[row][col + 1] * sm.beta[col + 1] * NP_UP, h2, l2);
+            *reinterpret_cast<uint32_t *>(np + row * CH + col) = h2;
+            *reinterpret_cast<uint32_t *>(np + CH * CH + row * CH + col) = l2;
+        }
+        if (tid < CH) {
+            x.decay[(slot * d.n_v + hv) * 2 * CH + tid] = sm.c[tid];
+            x.decay[(slot * d.n_v + hv) * 2 * CH + CH + tid] = sm.t.r[CH - 1][tid];
+        }
+        if (tid == 0) x.odd[slot * d.n_v + hv] = sm.odd | sm.odd_kq;
+        __syncthreads();
+    }
+}
+
+template <int DK> struct ChunkSmem {
+    static constexpr int KROW = DK + 8, NROW = CH + 8, SROW = 40, VROW = 40;  // elements; rows whose fragments do not collide
+    __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
+    __half s[2][DK * SROW], xx[2][CH * SROW], dd[2][CH * SROW], dr[2][CH * SROW];  // B operands: S, V - c K S, D, r D (hi, lo)
+    float v[2][CH * VROW], decay[2][2 * CH];
+    uint32_t most[8];
+};
+
+// Rows of an odd chunk one by one in f32: the 32 columns of the state are in shared memory as [DK][33] floats.
+template <int DK> __device__ __noinline__ void delta_rows_by_one(const DeltaArgs &d, float *S, float *tmp, int64_t first, int rows, int hk, int hv, int c0) {
+    const int tid = threadIdx.x, col = tid & 31, part = tid >> 5;
+    constexpr int PER = DK / 8;
+    for (int i = 0; i < rows; i++) {
+        const int64_t t = first + i;
+        const float *kr = d.k + t * d.k_stride + hk * DK, *qr = d.q + t * d.q_stride + hk * DK;
+        float qq = 0.0f, kk = 0.0f, qk = 0.0f;
+        for (int j = col; j < DK; j += 32) {
+            qq = __fmaf_rn(qr[j], qr[j], qq);
+            kk = __fmaf_rn(kr[j], kr[j], kk);
+            qk = __fmaf_rn(qr[j], kr[j], qk);
+        }
+        const float fq = d.scale * (d.eps >= 0.0f ? rsqrtf(agn_warp_sum(qq) + d.eps) : 1.0f), fk = d.eps >= 0.0f ? rsqrtf(agn_warp_sum(kk) + d.eps) : 1.0f;
+        qk = agn_warp_sum(qk) * fq * fk;
+        float dk = 0.0f, dq = 0.0f;
+        for (int j = part * PER; j < (part + 1) * PER; j++) {
+            dk = __fmaf_rn(kr[j] * fk, S[j * 33 + col], dk);
+            dq = __fmaf_rn(qr[j] * fq, S[j * 33 + col], dq);
+        }
+        tmp[part * 64 + col] = dk;
+        tmp[part * 64 + 32 + col] = dq;
+        __syncthreads();
+        dk = dq = 0.0f;
+        for (int w = 0; w < 8; w++) {
+            dk += tmp[w * 64 + col];
+            dq += tmp[w * 64 + 32 + col];
+        }
+        const float al = expf(d.g[t * d.n_v + hv]), be = d.beta[t * d.n_v + hv];
+        const float dl = be * __fmaf_rn(-al, dk, d.v[t * d.v_stride + hv * d.dv + c0 + col]);
+        if (part == 0) d.out[(t * d.n_v + hv) * d.dv + c0 + col] = __fmaf_rn(qk, dl, al * dq);
+        for (int j = part * PER; j < (part + 1) * PER; j++) S[j * 33 + col] = __fmaf_rn(kr[j] * fk, dl, al * S[j * 33 + col]);
+        __syncthreads();
+    }
+}
+
+template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_kernel(ChunkArgs x) {
+    agn_pdl_prologue();
+    extern __shared__ __align__(128) unsigned char raw[];
+    using SM = ChunkSmem<DK>;
+    SM &sm = *reinterpret_cast<SM *>(raw);
+    constexpr int KROW = SM::KROW, NROW = SM::NROW, SROW = SM::SROW, VROW = SM::VROW;
+    constexpr int MT = DK / 16, NU = MT / 2;  // the state's 16 x 8 tiles: MT x 4, NU to a warp
+    const DeltaArgs &d = x.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int c0 = blockIdx.x * 32, hv = blockIdx.y, hk = hv / (d.n_v / d.n_k);
+    const int64_t s = blockIdx.z;
+    int64_t b, e;
+    delta_rows(d, s, &b, &e);
+    const int64_t slot0 = delta_slot(b, s), chunks = (e - b + CH - 1) / CH;
+    const int mt = warp % MT, n0 = warp / MT * NU;  // this warp's tiles of the state: rows 16 mt .., columns 8 (n0 + n) ..
+
+    float S[NU][4];
+    const int64_t soff = ((s * d.n_v + hv) * DK + 16 * mt + g) * d.dv + c0 + 2 * t4;
+#pragma unroll
+    for (int n = 0; n < NU; n++) {
+        float2 u = make_float2(0.0f, 0.0f), w = u;
+        if (d.state_in) {
+            u = *reinterpret_cast<const float2 *>(d.state_in + soff + 8 * (n0 + n));
+            w = *reinterpret_cast<const float2 *>(d.state_in + soff + 8 * (n0 + n) + (int64_t)8 * d.dv);
+        }
+        S[n][0] = u.x; S[n][1] = u.y; S[n][2] = w.x; S[n][3] = w.y;
+    }
+
+    auto load_kq = [&](int64_t c, int w, __half *dst0, __half *dst1) {  // k (w = 0) or q (w = 2) of chunk c, both parts
+        const __half *src = x.kq + ((slot0 + c) * d.n_k + hk) * 4 * CH * DK + (int64_t)w * CH * DK;
+        constexpr int CPR = DK / 8;
+        for (int i = tid; i < 2 * CH * CPR; i += CHUNK_THREADS) {
+            const int part = i / (CH * CPR), row = i / CPR % CH, at = i % CPR * 8;
+            cp16((part ? dst1 : dst0) + row * KROW + at, src + (int64_t)i * 8);
+        }
+    };
+    auto load_np = [&](int64_t c, int w, __half *dst0, __half *dst1) {
+        const __half *src = x.np + ((slot0 + c) * d.n_v + hv) * 4 * CH * CH + (int64_t)w * CH * CH;
+        for (int i = tid; i < 2 * CH * 8; i += CHUNK_THREADS) {
+            const int part = i / (CH * 8), row = i / 8 % CH, at = i % 8 * 8;
+            cp16((part ? dst1 : dst0) + row * NROW + at, src + (int64_t)i * 8);
+        }
+    };
+    auto load_v = [&](int64_t c) {
+        const int64_t first = b + c * CH;
+        float *dst = sm.v[c & 1];
+        for (int i = tid; i < CH * 8; i += CHUNK_THREADS) {
+            const int row = i >> 3, at = (i & 7) * 4;
+            if (first + row < e) cp16(dst + row * VROW + at, d.v + (first + row) * d.v_stride + (int64_t)hv * d.dv + c0 + at);
+            else *reinterpret_cast<float4 *>(dst + row * VROW + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        if (tid < 32) cp16(sm.decay[c & 1] + tid * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + tid * 4);
+    };
+    auto fetched = [] { asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory"); };
+
+    if (chunks > 0) {
+        load_v(0);
+        load_kq(0, 0, sm.k[0][0], sm.k[0][1]);
+        load_kq(0, 2, sm.q[0], sm.q[1]);
+        load_np(0, 0, sm.n[0], sm.n[1]);
+        load_np(0, 2, sm.p[0], sm.p[1]);
+    }
+    for (int64_t c = 0; c < chunks; c++) {
+        const int64_t first = b + c * CH;
+        const int rows = (int)(e - first < CH ? e - first : CH);
+        fetched();
+        __syncthreads();
+        // ---- the largest magnitude of state and values, as bits: NaN above infinity above the numbers
+        uint32_t most = 0;
+        const float *v = sm.v[c & 1];
+        for (int i = tid; i < CH * 32; i += CHUNK_THREADS) most = max(most, __float_as_uint(v[(i >> 5) * VROW + (i & 31)]) & 0x7fffffffu);
+#pragma unroll
+        for (int n = 0; n < NU; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(S[n][i]) & 0x7fffffffu);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) sm.most[warp] = most;
+        const int odd = x.odd[(slot0 + c) * d.n_v + hv];
+        __syncthreads();
+        for (int w = 0; w < 8; w++) most = max(most, sm.most[w]);
+        const bool more = c + 1 < chunks;
+        if (odd || most >= 0x7f800000u) {
+            float *Sf = reinterpret_cast<float *>(sm.q), *tmp = reinterpret_cast<float *>(sm.n);  // q, N are not needed
+#pragma unroll
+            for (int n = 0; n < NU; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) Sf[(16 * mt + g + (i >> 1) * 8) * 33 + 8 * (n0 + n) + 2 * t4 + (i & 1)] = S[n][i];
+            __syncthreads();
+            delta_rows_by_one<DK>(d, Sf, tmp, first, rows, hk, hv, c0);
+#pragma unroll
+            for (int n = 0; n < NU; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[n][i] = Sf[(16 * mt + g + (i >> 1) * 8) * 33 + 8 * (n0 + n) + 2 * t4 + (i & 1)];
+            __syncthreads();
+            if (more) {
+                load_v(c + 1);
+                load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
+                load_kq(c + 1, 2, sm.q[0], sm.q[1]);
+                load_np(c + 1, 0, sm.n[0], sm.n[1]);
+                load_np(c + 1, 2, sm.p[0], sm.p[1]);
+            }
+            continue;
+        }
+        // up = 2^(5 - exponent): the largest becomes 2^5 .. 2^6, V - c K S at most 2^10, D at most 2^15
+        const int ex = max((int)(most >> 23), 24);
+        const float up = __uint_as_float((uint32_t)(259 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 5) << 23);
+#pragma unroll
+        for (int n = 0; n < NU; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint32_t h2, l2;
+                split2(S[n][2 * i] * up, S[n][2 * i + 1] * up, h2, l2);
+                const int at = (16 * mt + g + 8 * i) * SROW + 8 * (n0 + n) + 2 * t4;
+                *reinterpret_cast<uint32_t *>(&sm.s[0][at]) = h2;
+                *reinterpret_cast<uint32_t *>(&sm.s[1][at]) = l2;
+            }
+        __syncthreads();
+
+        // ---- K S and Q S: 16 rows and 16 columns per warp
+        const int wm = warp & 3, wn = (warp >> 2) * 16;
+        const __half *kh = sm.k[c & 1][0], *kl = sm.k[c & 1][1];
+        float ks[2][4] = {}, qs[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; kk++) {
+            uint32_t a0[4], a1[4], q0[4], q1[4], bh[4], bl[4];
+            const int arow = (wm * 16 + (lane & 15)) * KROW + kk * 16 + (lane >> 4) * 8;
+            const int brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
+            ldsm4(a0, kh + arow);
+            ldsm4(a1, kl + arow);
+            ldsm4(q0, sm.q[0] + arow);
+            ldsm4(q1, sm.q[1] + arow);
+            ldsm4t(bh, sm.s[0] + brow);
+            ldsm4t(bl, sm.s[1] + brow);
+#pragma unroll
+            for (int n = 0; n < 2; n++) { mma16(ks[n], a0, bh[2 * n], bh[2 * n + 1]); mma16(qs[n], q0, bh[2 * n], bh[2 * n + 1]); }
+#pragma unroll
+            for (int n = 0; n < 2; n++) { mma16(ks[n], a0, bl[2 * n], bl[2 * n + 1]); mma16(qs[n], q0, bl[2 * n], bl[2 * n + 1]); }
+#pragma unroll
+            for (int n = 0; n < 2; n++) { mma16(ks[n], a1, bh[2 * n], bh[2 * n + 1]); mma16(qs[n], q1, bh[2 * n], bh[2 * n + 1]); }
+        }
+        const int r0 = wm * 16 + g;
+        const float *dec = sm.decay[c & 1];
+        const float cg[2] = {dec[r0] * (1.0f / KQ_UP), dec[r0 + 8] * (1.0f / KQ_UP)};
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int col = wn + 8 * n + 2 * t4;
+                const float2 vv = *reinterpret_cast<const float2 *>(v + (r0 + 8 * i) * VROW + col);
+                uint32_t h2, l2;
+                split2(__fmaf_rn(-cg[i], ks[n][2 * i], vv.x * up), __fmaf_rn(-cg[i], ks[n][2 * i + 1], vv.y * up), h2, l2);
+                *reinterpret_cast<uint32_t *>(&sm.xx[0][(r0 + 8 * i) * SROW + col]) = h2;
+                *reinterpret_cast<uint32_t *>(&sm.xx[1][(r0 + 8 * i) * SROW + col]) = l2;
+                qs[n][2 * i] *= cg[i];
+                qs[n][2 * i + 1] *= cg[i];
+            }
+        __syncthreads();
+        if (more) {  // q has been read, the other buffers of k and v were last chunk's
+            load_v(c + 1);
+            load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
+            load_kq(c + 1, 2, sm.q[0], sm.q[1]);
+        }
+
+        // ---- D = N X: a lower triangle, so up to the warp's own rows
+        float dd[2][4] = {}, po[2][4] = {};
+        for (int kk = 0; kk <= wm; kk++) {
+            uint32_t a0[4], a1[4], bh[4], bl[4];
+            const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
+            ldsm4(a0, sm.n[0] + arow);
+            ldsm4(a1, sm.n[1] + arow);
+            ldsm4t(bh, sm.xx[0] + brow);
+            ldsm4t(bl, sm.xx[1] + brow);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                mma16(dd[n], a0, bh[2 * n], bh[2 * n + 1]);
+                mma16(dd[n], a0, bl[2 * n], bl[2 * n + 1]);
+                mma16(dd[n], a1, bh[2 * n], bh[2 * n + 1]);
+            }
+        }
+        const float rc[2] = {dec[CH + r0], dec[CH + r0 + 8]};
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int at = (r0 + 8 * i) * SROW + wn + 8 * n + 2 * t4;
+                const float u = dd[n][2 * i] * (1.0f / NP_UP), w = dd[n][2 * i + 1] * (1.0f / NP_UP);
+                uint32_t h2, l2;
+                split2(u, w, h2, l2);
+                *reinterpret_cast<uint32_t *>(&sm.dd[0][at]) = h2;
+                *reinterpret_cast<uint32_t *>(&sm.dd[1][at]) = l2;
+                split2(u * rc[i], w * rc[i], h2, l2);
+                *reinterpret_cast<uint32_t *>(&sm.dr[0][at]) = h2;
+                *reinterpret_cast<uint32_t *>(&sm.dr[1][at]) = l2;
+            }
+        __syncthreads();
+        if (more) load_np(c + 1, 0, sm.n[0], sm.n[1]);
+
+        // ---- S' = c_C S + K^T (r D)
+        float up_s[NU][4];
+#pragma unroll
+        for (int n = 0; n < NU; n++) up_s[n][0] = up_s[n][1] = up_s[n][2] = up_s[n][3] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < CH / 16; kk++) {
+            uint32_t a0[4], a1[4];
+            const int arow = (kk * 16 + (lane & 7) + (lane >> 4) * 8) * KROW + mt * 16 + ((lane >> 3) & 1) * 8;
+            ldsm4t(a0, kh + arow);
+            ldsm4t(a1, kl + arow);
+#pragma unroll
+            for (int n = 0; n < NU; n += 2) {
+                uint32_t bh[4], bl[4];
+                const int brow = (kk * 16 + (lane & 15)) * SROW + 8 * (n0 + n) + (lane >> 4) * 8;
+                ldsm4t(bh, sm.dr[0] + brow);
+                ldsm4t(bl, sm.dr[1] + brow);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mma16(up_s[n + h], a0, bh[2 * h], bh[2 * h + 1]);
+                    mma16(up_s[n + h], a0, bl[2 * h], bl[2 * h + 1]);
+                    mma16(up_s[n + h], a1, bh[2 * h], bh[2 * h + 1]);
+                }
+            }
+        }
+        const float cc = dec[CH - 1], f = down * (1.0f / KQ_UP);
+#pragma unroll
+        for (int n = 0; n < NU; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[n][i] = __fmaf_rn(up_s[n][i], f, cc * S[n][i]);
+
+        // ---- O = c Q S + P D
+        for (int kk = 0; kk <= wm; kk++) {
+            uint32_t a0[4], a1[4], bh[4], bl[4];
+            const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
+            ldsm4(a0, sm.p[0] + arow);
+            ldsm4(a1, sm.p[1] + arow);
+            ldsm4t(bh, sm.dd[0] + brow);
+            ldsm4t(bl, sm.dd[1] + brow);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                mma16(po[n], a0, bh[2 * n], bh[2 * n + 1]);
+                mma16(po[n], a0, bl[2 * n], bl[2 * n + 1]);
+                mma16(po[n], a1, bh[2 * n], bh[2 * n + 1]);
+            }
+        }
+        const float fo = d.scale * down;
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (r0 + 8 * i < rows) {
+                    float2 y;
+                    y.x = __fmaf_rn(po[n][2 * i], 1.0f / NP_UP, qs[n][2 * i]) * fo;
+                    y.y = __fmaf_rn(po[n][2 * i + 1], 1.0f / NP_UP, qs[n][2 * i + 1]) * fo;
+                    *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) = y;
+                }
+        __syncthreads();  // P and D have been read
+        if (more) load_np(c + 1, 2, sm.p[0], sm.p[1]);
+    }
+#pragma unroll
+    for (int n = 0; n < NU; n++) {
+        *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n)) = make_float2(S[n][0], S[n][1]);
+        *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n) + (int64_t)8 * d.dv) = make_float2(S[n][2], S[n][3]);
+    }
+}
+
+// The chunked form pays from about this many rows a sequence on.
+constexpr int CHUNK_MIN_ROWS = 48;
+bool delta_chunked(int64_t T, int64_t n_seqs) { return T >= CHUNK_MIN_ROWS * n_seqs; }
+
+struct ChunkLayout {
+    int64_t slots, kq, np, decay, odd, bytes;  // byte offsets
+};
+ChunkLayout chunk_layout(int64_t T, int64_t n_seqs, int n_k, int n_v, int dk) {
+    ChunkLayout l;
+    l.slots = T / CH + n_seqs;
+    l.kq = 0;
+    l.np = l.kq + l.slots * n_k * 4 * CH * dk * 2;
+    l.decay = l.np + l.slots * n_v * 4 * CH * CH * 2;
+    l.odd = l.decay + l.slots * n_v * 2 * CH * 4;
+    l.bytes = (l.odd + l.slots * n_v * 4 + 15) / 16 * 16;
+    return l;
+}
+
+template <int DK> int32_t launch_chunked(agn_ctx *ctx, const DeltaArgs &d, void *workspace, int n_seqs) {
+    const ChunkLayout l = chunk_layout(d.T, d.n_seqs, d.n_k, d.n_v, DK);
+    ChunkArgs x;
+    unsigned char *w = static_cast<unsigned char *>(workspace);
+    x.d = d;
+    x.kq = reinterpret_cast<__half *>(w + l.kq);
+    x.np = reinterpret_cast<__half *>(w + l.np);
+    x.decay = reinterpret_cast<float *>(w + l.decay);
+    x.odd = reinterpret_cast<int *>(w + l.odd);
+    if (agn_ring_ctas_per_sm(ctx, delta_prepare_kernel<DK>, CHUNK_THREADS, sizeof(PrepSmem<DK>)) < 1 ||
+        agn_ring_ctas_per_sm(ctx, delta_chunk_kernel<DK>, CHUNK_THREADS, sizeof(ChunkSmem<DK>)) < 1)
+        return agn_fail(ctx, AGN_ECUDA, "gated_delta_rule: the chunk kernels do not fit the device's shared memory");
+    agn_launch(ctx, delta_prepare_kernel<DK>, dim3((unsigned)l.slots, (unsigned)d.n_k), dim3(CHUNK_THREADS), sizeof(PrepSmem<DK>), x);
+    AGN_LAUNCHED(ctx, "gated_delta_chunk");
+    agn_launch(ctx, delta_chunk_kernel<DK>, dim3((unsigned)(d.dv / 32), (unsigned)d.n_v, (unsigned)n_seqs), dim3(CHUNK_THREADS), sizeof(ChunkSmem<DK>), x);
+    AGN_LAUNCHED(ctx, "gated_delta_chunk");
+    return AGN_OK;
+}
+
 bool delta_shape_ok(int64_t T, int64_t n_seqs, int n_k, int n_v, int dk, int dv) {
     return T >= 0 && T <= 0x7fffffffLL && n_seqs > 0 && n_seqs <= 65535 && n_k > 0 && n_v > 0 && n_v % n_k == 0 && n_v <= 65535 && (dk == 64 || dk == 128) &&
            dv > 0 && dv % 32 == 0 && dv <= 256;
@@ -146,8 +734,8 @@ bool delta_shape_ok(int64_t T, int64_t n_seqs, int n_k, int n_v, int dk, int dv)
 
 extern "C" int64_t agn_gated_delta_rule_workspace_bytes(int64_t T, int64_t n_seqs, int32_t n_k_heads, int32_t n_v_heads, int32_t head_k,
                                                         int32_t head_v) {
-    if (!delta_shape_ok(T, n_seqs, n_k_heads, n_v_heads, head_k, head_v)) return 0;
-    return 0;
+    if (!delta_shape_ok(T, n_seqs, n_k_heads, n_v_heads, head_k, head_v) || !delta_chunked(T, n_seqs)) return 0;
+    return chunk_layout(T, n_seqs, n_k_heads, n_v_heads, head_k).bytes;
 }
 
 extern "C" int32_t agn_gated_delta_rule_f32(agn_ctx *ctx, const float *q, const float *k, const float *v, const float *g, const float *beta,
@@ -174,11 +762,16 @@ extern "C" int32_t agn_gated_delta_rule_f32(agn_ctx *ctx, const float *q, const 
     a.q = q; a.k = k; a.v = v; a.g = g; a.beta = beta; a.state_in = state_in; a.state_out = state_out; a.out = out; a.cu = cu_seqlens;
     a.T = T; a.n_seqs = n_seqs; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
     a.n_k = n_k_heads; a.n_v = n_v_heads; a.dv = head_v; a.scale = scale; a.eps = l2norm_eps; a.flags = ctx->d_flags;
+    if (cu_seqlens) ctx->flags_dirty = true;
+    if (delta_chunked(T, n_seqs)) {
+        const int64_t need = chunk_layout(T, n_seqs, n_k_heads, n_v_heads, head_k).bytes;
+        if (!workspace || (int64_t)workspace_bytes < need || !agn_aligned16(workspace))
+            return agn_fail(ctx, AGN_EINVAL, "gated_delta_rule: needs %lld bytes of 16-byte aligned workspace", (long long)need);
+        return head_k == 64 ? launch_chunked<64>(ctx, a, workspace, (int)n_seqs) : launch_chunked<128>(ctx, a, workspace, (int)n_seqs);
+    }
     const dim3 grid((unsigned)(head_v / 32), (unsigned)n_v_heads, (unsigned)n_seqs);
     if (head_k == 64) agn_launch(ctx, delta_recurrent_kernel<64>, grid, dim3(128), 0, a);
     else agn_launch(ctx, delta_recurrent_kernel<128>, grid, dim3(128), 0, a);
-    if (cu_seqlens) ctx->flags_dirty = true;
     AGN_LAUNCHED(ctx, "gated_delta_recurrent");
-    (void)workspace; (void)workspace_bytes;
     return AGN_OK;
 }
