@@ -7,20 +7,9 @@
 // src/model/llama/cpu_path.rs:160-192).  G = n_q_heads / n_kv_heads query heads share a KV head.
 #include <math.h>
 
-#include "agn_common.cuh"
+#include "agn_attention.cuh"
 
 namespace {
-
-struct AttnArgs {
-    const void *q;
-    void *out;
-    const unsigned char *k_cache, *v_cache;
-    const int32_t *pos, *seq;
-    int64_t T, n_seqs, max_seq;
-    int n_q, n_kv, hd, pos_start, bytes_per_token;
-    float scale;
-    uint32_t *flags;
-};
 
 // Visible slots of row t and the first byte of its sequence's cache; 0 slots for an empty row or one outside the cache.
 __device__ __forceinline__ int attn_row(const AttnArgs &a, int64_t t, int64_t *seq_off) {
@@ -35,17 +24,6 @@ __device__ __forceinline__ int attn_row(const AttnArgs &a, int64_t t, int64_t *s
     return (int)(p + 1);
 }
 
-constexpr int KV_F16 = 0, KV_Q8 = 1, KV_WORDS = 2;
-template <int KV> struct KvFormat;  // a block of 32 values of one head: BYTES, with the values DATA bytes behind its start
-template <> struct KvFormat<KV_F16> { static constexpr int BYTES = 64, DATA = 0; };
-template <> struct KvFormat<KV_Q8> { static constexpr int BYTES = 34, DATA = 2; };
-template <> struct KvFormat<KV_WORDS> { static constexpr int BYTES = 36, DATA = 4; };
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -100,11 +78,6 @@ __device__ __forceinline__ void load8_at(const unsigned char *p, bool odd, uint3
         y = reinterpret_cast<const uint32_t *>(p)[1];
     }
 }
-template <int KV> __device__ __forceinline__ float block_scale(const unsigned char *blk) {
-    if (KV == KV_WORDS) return *reinterpret_cast<const float *>(blk);
-    return __half2float(*reinterpret_cast<const __half *>(blk));
-}
-
 // ---- Decode: rows of any position and sequence ----------------------------------------------------------------------
 //
 // Bound by HBM: a slot's 2 * bytes_per_token bytes are read once for all query heads.  What a CTA works on is a run of tiles of
@@ -672,7 +645,8 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     const int ca = kv_dtype == AGN_KV_Q8_0_WORDS ? 4 : 2;
     if (!agn_aligned(k_cache, ca) || !agn_aligned(v_cache, ca))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: caches must be %d-byte aligned", ca);
-    const int64_t need = attn_workspace(rows, n_q, hd);
+    const bool prompt = !pos && sizeof(T) == 2 && agn_attention_prompt_fits(rows, n_q, n_kv, hd);
+    const int64_t need = prompt ? agn_attention_prompt_workspace(pos_start + rows, n_kv, hd) : attn_workspace(rows, n_q, hd);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !agn_aligned16(workspace)))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     AGN_CUDA(ctx, cudaSetDevice(ctx->device));
@@ -680,6 +654,8 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     a.q = q; a.out = out; a.k_cache = static_cast<const unsigned char *>(k_cache); a.v_cache = static_cast<const unsigned char *>(v_cache);
     a.pos = pos; a.seq = seq; a.T = rows; a.n_seqs = n_seqs; a.max_seq = max_seq; a.n_q = n_q; a.n_kv = n_kv; a.hd = hd; a.pos_start = pos_start;
     a.bytes_per_token = (int)agn_kv_bytes_per_token(kv_dtype, (int64_t)n_kv * hd); a.scale = scale; a.flags = ctx->d_flags;
+    ctx->flags_dirty = true;
+    if (prompt) return agn_attention_prompt_f16(ctx, a, kv_dtype, workspace);
     const int block_bytes = kv_dtype == AGN_F16 ? 64 : kv_dtype == AGN_Q8_0 ? 34 : 36;
     const DecodePlan p = decode_plan(rows, n_q, n_kv, hd, max_seq, block_bytes, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);
     DecodeArgs d;
@@ -692,7 +668,6 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     d.granule = (int)(bits & (0 - bits));
     DecodePlan use = p;
     if (d.granule < 4) { d.stages = use.stages = 1; use.smem = (size_t)2 * p.tt * p.row_stride + 16; }
-    ctx->flags_dirty = true;
     if (kv_dtype == AGN_F16) return launch_decode_kv<T, KV_F16>(ctx, use, d);
     if (kv_dtype == AGN_Q8_0) return launch_decode_kv<T, KV_Q8>(ctx, use, d);
     return launch_decode_kv<T, KV_WORDS>(ctx, use, d);
@@ -703,8 +678,10 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
 extern "C" int64_t agn_attention_kv_workspace_bytes(int64_t T, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t max_seq_len,
                                                     int32_t has_pos) {
     if (!attn_shape_ok(T, n_q_heads, n_kv_heads, head_dim, max_seq_len)) return 0;
-    (void)has_pos;
-    return attn_workspace(T, n_q_heads, head_dim);
+    const int64_t decode = attn_workspace(T, n_q_heads, head_dim);
+    if (has_pos || !agn_attention_prompt_fits(T, n_q_heads, n_kv_heads, head_dim)) return decode;
+    const int64_t prompt = agn_attention_prompt_workspace(max_seq_len, n_kv_heads, head_dim);
+    return prompt > decode ? prompt : decode;
 }
 
 extern "C" int32_t agn_attention_kv_f32(agn_ctx *ctx, const float *q, float *out, int32_t kv_dtype, const void *k_cache, const void *v_cache,

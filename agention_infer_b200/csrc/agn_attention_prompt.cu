@@ -1,0 +1,431 @@
+// Attention of a prompt's rows (consecutive positions of one sequence, f16) over the KV cache, on the 5th-generation tensor cores.
+//
+// Bound by the tensor cores (4 * head_dim flop per row, head and slot) and, equally, by the exponentials (16 a clock and SM
+// against 128 x 128 products of 128 in 1024 clocks).  Two kernels:
+//
+//   attn_unpack_kernel writes the sequence's K and V as f16 tiles of 128 slots of one head, each the very bytes that the matrix
+//   instruction wants in shared memory (rows of 128 bytes, 16-byte pieces exchanged by row: the 128-byte swizzle), so that a tile is
+//   one bulk copy and no CTA dequantises what another one needs too (every tile is read by T * G / 256 CTAs).
+//
+//   attn_prompt_kernel: a CTA takes 256 query rows of one KV head - row r is (token r / G, head r % G of the group), so a tile
+//   serves the whole group - as two tiles of 128, so that the tensor cores work on one tile while the softmax of the other
+//   runs.  Warps 0-3 and 4-7: softmax of the two tiles, a row per thread; warp 8 fetches tiles; warp 9 issues the products.
+//   TMEM: S0, S1, O0, O1 (128 columns each); the weights overwrite their scores as f16 and are the A operand of the second
+//   product from there.  The output is rescaled only when a row's maximum has grown by more than 2^8 (weights stay below f16's
+//   range; sums and accumulators are f32).
+#include <math.h>
+
+#include "agn_attention.cuh"
+
+namespace {
+
+constexpr int TILE = 128, PROMPT_THREADS = 320, STAGES = 2;
+
+struct PromptArgs {
+    AttnArgs a;
+    __half *k, *v;   // [n_kv][tiles] images of TILE x hd
+    int *odd;        // [0]: any value that is not finite; then per (KV head, dim) the first slot of +inf, -inf, NaN
+    int64_t tiles, rows;  // tiles of the sequence; rows T * G of a KV head
+    int spin;
+};
+
+// One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a row does
+// not see must not meet them in the product.
+template <int KV> __global__ void __launch_bounds__(256) attn_unpack_kernel(PromptArgs p) {
+    agn_pdl_prologue();
+    const AttnArgs &a = p.a;
+    const int64_t tile = blockIdx.x;
+    const int head = blockIdx.y, hd = a.hd, chunks = hd / 8, n_odd = a.n_kv * hd;
+    const bool is_v = blockIdx.z;
+    const int end = a.pos_start + (int)a.T;
+    const unsigned char *src = is_v ? a.v_cache : a.k_cache;
+    unsigned char *dst = reinterpret_cast<unsigned char *>(is_v ? p.v : p.k) + (head * p.tiles + tile) * TILE * hd * 2;
+    for (int i = threadIdx.x; i < TILE * chunks; i += blockDim.x) {
+        const int r = i / chunks, c = i % chunks;
+        const int64_t slot = tile * TILE + r;
+        float v[8];
+        if (slot < end) {
+            const unsigned char *row = src + slot * a.bytes_per_token;
+            const int d = head * hd + c * 8;
+            if (KV == KV_F16) {
+                const uint16_t *w = reinterpret_cast<const uint16_t *>(row) + d;
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = __half2float(__ushort_as_half(w[k]));
+            } else {
+                const unsigned char *blk = row + (d >> 5) * KvFormat<KV>::BYTES;
+                const float s = block_scale<KV>(blk);
+                const uint16_t *w = reinterpret_cast<const uint16_t *>(blk + KvFormat<KV>::DATA + (d & 31));
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t u = KV == KV_Q8 ? w[k] ^ 0x8080u : w[k];
+                    v[2 * k] = (float)((int)(u & 0xff) - 128) * s;
+                    v[2 * k + 1] = (float)((int)(u >> 8) - 128) * s;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = 0.0f;
+        }
+        if (is_v) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = __half2float(__float2half_rn(v[k]));
+                if ((__float_as_uint(f) & 0x7f800000u) == 0x7f800000u) {
+                    p.odd[0] = 1;
+                    const int kind = f != f ? 2 : f > 0.0f ? 0 : 1;
+                    atomicMin(&p.odd[4 + kind * n_odd + head * hd + c * 8 + k], (int)slot);
+                    v[k] = 0.0f;
+                }
+            }
+        }
+        __half2 h[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        *reinterpret_cast<uint4 *>(dst + (c >> 3) * TILE * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4 *>(h);
+    }
+}
+
+__global__ void __launch_bounds__(256) attn_odd_reset_kernel(int *odd, int n) {
+    agn_pdl_prologue();
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) odd[i] = i < 4 ? 0 : 0x7fffffff;
+}
+
+// ---- tensor-core instructions
+// Operand in shared memory: rows of 128 bytes, swizzled in groups of eight rows (1024 bytes).  lead: bytes to the next 64 elements of the
+// row dimension where that is the contiguous one.
+__device__ __forceinline__ uint64_t smem_operand(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lead >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// f16 x f16 -> f32, M = 128; b_rows_contiguous: the second operand's N is its contiguous dimension
+__device__ __forceinline__ constexpr uint32_t mma_shape(int n, bool b_rows_contiguous) {
+    return 1u << 4 | (b_rows_contiguous ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
+                 "r"(shape), "r"((int)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
+                 "r"(shape), "r"((int)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(agn_smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(agn_smem_u32(bar)) : "memory");
+}
+#define TMEM_R4(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define TMEM_W4(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3])
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+                 "%28,%29,%30,%31}, [%32];"
+                 : TMEM_R4(r, 0), TMEM_R4(r, 4), TMEM_R4(r, 8), TMEM_R4(r, 12), TMEM_R4(r, 16), TMEM_R4(r, 20), TMEM_R4(r, 24), TMEM_R4(r, 28)
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+                 "%28,%29,%30,%31};" ::TMEM_W4(r, 0), TMEM_W4(r, 4), TMEM_W4(r, 8), TMEM_W4(r, 12), TMEM_W4(r, 16), TMEM_W4(r, 20), TMEM_W4(r, 24), TMEM_W4(r, 28),
+                 "r"(at)
+                 : "memory");
+}
+// The registers go through the wait, so that nothing that uses them is scheduled in front of it.
+#define TMEM_RW4(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3])
+__device__ __forceinline__ void tmem_loaded(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : TMEM_RW4(r, 0), TMEM_RW4(r, 4), TMEM_RW4(r, 8), TMEM_RW4(r, 12), TMEM_RW4(r, 16), TMEM_RW4(r, 20), TMEM_RW4(r, 24), TMEM_RW4(r, 28)::"memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int HD> struct PromptSmem {
+    unsigned char q[2][TILE * HD * 2], k[STAGES][TILE * HD * 2], v[STAGES][TILE * HD * 2];
+    uint64_t q_full, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], s_full[2], p_full[2], o_full[2], drained;
+    uint32_t tmem;
+    int gave_up;
+};
+
+template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prompt_kernel(PromptArgs p) {
+    agn_pdl_prologue();
+    extern __shared__ unsigned char raw[];
+    PromptSmem<HD> &sm = *reinterpret_cast<PromptSmem<HD> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const AttnArgs &a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.n_q / a.n_kv, head = blockIdx.y;
+    const int64_t r0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * 2 * TILE;  // the longest rows first
+    const int64_t last_row = r0 + 2 * TILE - 1 < p.rows ? r0 + 2 * TILE - 1 : p.rows - 1;
+    const int tiles = (int)((a.pos_start + last_row / G) / TILE) + 1;  // that the CTA's last row sees
+    constexpr uint32_t IMAGE = TILE * HD * 2;
+
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(agn_smem_u32(&sm.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        agn_mbar_init(&sm.q_full, 256);
+        for (int i = 0; i < STAGES; i++) {
+            agn_mbar_init(&sm.k_full[i], 1); agn_mbar_init(&sm.v_full[i], 1);
+            agn_mbar_init(&sm.k_free[i], 1); agn_mbar_init(&sm.v_free[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            agn_mbar_init(&sm.s_full[i], 1); agn_mbar_init(&sm.p_full[i], 128); agn_mbar_init(&sm.o_full[i], 1);
+        }
+        agn_mbar_init(&sm.drained, 1);
+        agn_mbar_init_fence();
+        sm.gave_up = 0;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+    // a bounded wait; once one has run out the CTA's other waits give up after their next poll
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        for (int left = p.spin; left > 0; left -= 1024) {
+            if (agn_mbar_wait(bar, parity, left < 1024 ? left : 1024)) return true;
+            if (*(volatile int *)&sm.gave_up) return false;
+        }
+        *(volatile int *)&sm.gave_up = 1;
+        return false;
+    };
+
+    if (warp == 8) {
+        if (lane == 0) {
+            const unsigned char *k = reinterpret_cast<const unsigned char *>(p.k) + (int64_t)head * p.tiles * IMAGE;
+            const unsigned char *v = reinterpret_cast<const unsigned char *>(p.v) + (int64_t)head * p.tiles * IMAGE;
+            int issued_k = 0, issued_v = 0;
+            for (int j = 0; j < tiles; j++) {
+                const int s = j % STAGES;
+                if (j >= STAGES && !wait(&sm.k_free[s], (j / STAGES - 1) & 1)) break;
+                agn_mbar_expect_tx(&sm.k_full[s], IMAGE);
+                agn_bulk_g2s(sm.k[s], k + (int64_t)j * IMAGE, IMAGE, &sm.k_full[s]);
+                issued_k++;
+                if (j >= STAGES && !wait(&sm.v_free[s], (j / STAGES - 1) & 1)) break;
+                agn_mbar_expect_tx(&sm.v_full[s], IMAGE);
+                agn_bulk_g2s(sm.v[s], v + (int64_t)j * IMAGE, IMAGE, &sm.v_full[s]);
+                issued_v++;
+            }
+            // no copy may be in flight when the CTA ends: the last one of every stage (earlier ones have been waited for by the products)
+            for (int j = issued_k > STAGES ? issued_k - STAGES : 0; j < issued_k; j++) (void)agn_mbar_wait(&sm.k_full[j % STAGES], (j / STAGES) & 1, p.spin);
+            for (int j = issued_v > STAGES ? issued_v - STAGES : 0; j < issued_v; j++) (void)agn_mbar_wait(&sm.v_full[j % STAGES], (j / STAGES) & 1, p.spin);
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            const uint32_t qa = agn_smem_u32(sm.q[0]), ka = agn_smem_u32(sm.k[0]), va = agn_smem_u32(sm.v[0]);
+            auto scores = [&](int i, int j) {  // S_i = Q_i K_j^T
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ks++) {
+                    const uint32_t at = (ks >> 2) * TILE * 128 + (ks & 3) * 32;
+                    mma_ss(tmem + i * 128, smem_operand(qa + i * IMAGE + at, 16), smem_operand(ka + (j % STAGES) * IMAGE + at, 16), mma_shape(TILE, false), ks > 0);
+                }
+                mma_commit(&sm.s_full[i]);
+            };
+            bool ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
+            if (ok) {
+                fence_after();
+                scores(0, 0);
+                scores(1, 0);
+                mma_commit(&sm.k_free[0]);
+            }
+            for (int j = 0; ok && j < tiles; j++) {
+                const int s = j % STAGES;
+                if (!wait(&sm.v_full[s], (j / STAGES) & 1)) break;
+                if (j + 1 < tiles && !wait(&sm.k_full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1)) break;
+                for (int i = 0; i < 2; i++) {
+                    if (!wait(&sm.p_full[i], j & 1)) { ok = false; break; }
+                    fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TILE / 16; ks++)  // O_i += P_i V_j, 16 slots at a time
+                        mma_ts(tmem + 256 + i * 128, tmem + i * 128 + ks * 8, smem_operand(va + s * IMAGE + ks * 2048, TILE * 128), mma_shape(HD, true), j > 0 || ks > 0);
+                    if (j + 1 < tiles) scores(i, j + 1);  // behind that product, which still reads the weights in S_i's place
+                    else mma_commit(&sm.o_full[i]);
+                }
+                mma_commit(&sm.v_free[s]);
+                if (j + 1 < tiles) mma_commit(&sm.k_free[(j + 1) % STAGES]);
+            }
+            mma_commit(&sm.drained);  // every product is done before the tensor memory goes back
+            (void)agn_mbar_wait(&sm.drained, 0, p.spin);
+        }
+        __syncwarp();
+    } else {
+        // ---- a query row per thread
+        const int i = warp >> 2, row = tid & 127;
+        const int64_t r = r0 + i * TILE + row;
+        const bool there = r < p.rows;
+        const int64_t t = (there ? r : p.rows - 1) / G, h = (there ? r : p.rows - 1) % G;
+        const int last = a.pos_start + (int)t;  // the last slot it sees
+        const int64_t at = (t * a.n_q + head * G + h) * HD;
+        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at);
+#pragma unroll
+        for (int c = 0; c < HD / 8; c++)
+            *reinterpret_cast<uint4 *>(sm.q[i] + (c >> 3) * TILE * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = there ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(&sm.q_full);
+
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes of the tensor memory per warp, lane number in the upper half
+        const uint32_t s_at = tmem + i * 128 + lanes, o_at = tmem + 256 + i * 128 + lanes;
+        const float coef = a.scale * 1.4426950408889634f;
+        const int first_last = a.pos_start + (int)((r0 + i * TILE) / G);  // what the tile's first row sees
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < tiles; j++) {
+            if (!(ok = wait(&sm.s_full[i], j & 1))) break;
+            fence_after();
+            // The scores are read twice, 32 at a time: 128 of them beside the rest do not fit the 168 registers of a thread.
+            const int seen = last - j * TILE;  // slots c <= seen of this tile
+            const bool edge = j * TILE + TILE - 1 > first_last;
+            uint32_t s[2][32];
+            float x0 = -INFINITY, x1 = -INFINITY;
+            tmem_load32(s_at, s[0]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_loaded(s[c & 1]);
+                if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                uint32_t *w = s[c & 1];
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (32 * c + k > seen) w[k] = 0xff800000u;
+                }
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x0) : "f"(__uint_as_float(w[k])), "f"(__uint_as_float(w[k + 1])));
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x1) : "f"(__uint_as_float(w[k + 2])), "f"(__uint_as_float(w[k + 3])));
+                }
+            }
+            tmem_load32(s_at, s[0]);
+            const float mt = fmaxf(x0, x1) * coef;
+            const bool grow = mt > m + 8.0f;  // true at the first tile
+            if (__any_sync(0xffffffffu, grow)) {
+                const float f = grow ? ex2(m - mt) : 1.0f;
+                if (grow) m = mt;
+                l *= f;
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(o_at + c, o);
+                        tmem_loaded(o);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_store32(o_at + c, o);
+                    }
+                }
+            }
+            const float mu = m == -INFINITY ? 0.0f : m;
+            float2 sum = make_float2(0.0f, 0.0f);
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_loaded(s[c & 1]);
+                if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
+                uint32_t *x = s[c & 1];
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (32 * c + k > seen) x[k] = 0xff800000u;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), make_float2(coef, coef), make_float2(-mu, -mu));
+                    const float2 y = make_float2(ex2(e.x), ex2(e.y));
+                    sum = __fadd2_rn(sum, y);
+                    const __half2 h2 = __floats2half2_rn(y.x, y.y);
+                    w[16 * (c & 1) + k] = *reinterpret_cast<const uint32_t *>(&h2);
+                }
+                if (c & 1) tmem_store32(s_at + 16 * (c - 1), w);  // over scores that have been read
+            }
+            l += sum.x + sum.y;
+            tmem_stored();
+            fence_before();
+            bar_arrive(&sm.p_full[i]);
+        }
+        if (ok && (ok = wait(&sm.o_full[i], 0))) {
+            fence_after();
+            const float inv = 1.0f / l;
+            const bool any = p.odd[0] != 0;
+            __half *out = static_cast<__half *>(a.out) + at;
+            const int n_odd = a.n_kv * HD;
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                tmem_load32(o_at + c, o);
+                tmem_loaded(o);
+                if (any) {  // values that are not finite reach the rows that see their slot
+                    for (int k = 0; k < 32; k++) {
+                        const int *f = p.odd + 4 + head * HD + c + k;
+                        const bool up = f[0] <= last, down = f[n_odd] <= last, nan = f[2 * n_odd] <= last;
+                        const float bad = nan || (up && down) ? NAN : up ? INFINITY : -INFINITY;
+                        if (up || down || nan) {
+#pragma unroll
+                            for (int q = 0; q < 32; q++)
+                                if (q == k) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv + bad);
+                        }
+                    }
+                }
+                if (there) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {
+                        __half2 h2[4];
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            h2[q] = __floats2half2_rn(__uint_as_float(o[k + 2 * q]) * inv, __uint_as_float(o[k + 2 * q + 1]) * inv);
+                        *reinterpret_cast<uint4 *>(out + c + k) = *reinterpret_cast<const uint4 *>(h2);
+                    }
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+    if (tid == 0 && sm.gave_up) atomicOr(a.flags, AGN_FLAG_TIMEOUT);
+}
+
+int64_t image_bytes(int64_t slots, int n_kv, int hd) { return (slots + TILE - 1) / TILE * TILE * n_kv * hd * 2; }
+int64_t odd_ints(int n_kv, int hd) { return 4 + 3 * (int64_t)n_kv * hd; }
+
+template <int HD> int32_t launch_prompt(agn_ctx *ctx, const PromptArgs &p, int kv_dtype) {
+    const size_t smem = sizeof(PromptSmem<HD>) + 1024;
+    if (agn_ring_ctas_per_sm(ctx, attn_prompt_kernel<HD>, PROMPT_THREADS, smem) < 1)
+        return agn_fail(ctx, AGN_ECUDA, "attention_kv: the prompt kernel does not fit the device's shared memory");
+    const int n = (int)odd_ints(p.a.n_kv, HD);
+    agn_launch(ctx, attn_odd_reset_kernel, dim3((unsigned)((n + 255) / 256 < 64 ? (n + 255) / 256 : 64)), dim3(256), 0, p.odd, n);
+    AGN_LAUNCHED(ctx, "attention_kv_prompt");
+    const dim3 tiles((unsigned)p.tiles, (unsigned)p.a.n_kv, 2);
+    if (kv_dtype == AGN_F16) agn_launch(ctx, attn_unpack_kernel<KV_F16>, tiles, dim3(256), 0, p);
+    else if (kv_dtype == AGN_Q8_0) agn_launch(ctx, attn_unpack_kernel<KV_Q8>, tiles, dim3(256), 0, p);
+    else agn_launch(ctx, attn_unpack_kernel<KV_WORDS>, tiles, dim3(256), 0, p);
+    AGN_LAUNCHED(ctx, "attention_kv_prompt");
+    agn_launch(ctx, attn_prompt_kernel<HD>, dim3((unsigned)((p.rows + 2 * TILE - 1) / (2 * TILE)), (unsigned)p.a.n_kv), dim3(PROMPT_THREADS), smem, p);
+    AGN_LAUNCHED(ctx, "attention_kv_prompt");
+    return AGN_OK;
+}
+
+}  // namespace
+
+bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd) {
+    return (hd == 64 || hd == 128) && T * (n_q / n_kv) >= AGN_PROMPT_MIN_ROWS && T >= AGN_PROMPT_MIN_TOKENS;
+}
+
+int64_t agn_attention_prompt_workspace(int64_t slots, int n_kv, int hd) {
+    return 2 * image_bytes(slots, n_kv, hd) + (odd_ints(n_kv, hd) * 4 + 15) / 16 * 16;
+}
+
+int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace) {
+    PromptArgs p;
+    const int64_t slots = (int64_t)a.pos_start + a.T, image = image_bytes(slots, a.n_kv, a.hd);
+    unsigned char *w = static_cast<unsigned char *>(workspace);
+    p.a = a;
+    p.k = reinterpret_cast<__half *>(w);
+    p.v = reinterpret_cast<__half *>(w + image);
+    p.odd = reinterpret_cast<int *>(w + 2 * image);
+    p.tiles = (slots + TILE - 1) / TILE;
+    p.rows = a.T * (a.n_q / a.n_kv);
+    p.spin = ctx->mbar_spin_limit;
+    return a.hd == 64 ? launch_prompt<64>(ctx, p, kv_dtype) : launch_prompt<128>(ctx, p, kv_dtype);
+}
