@@ -19,23 +19,35 @@
 
 namespace {
 
-constexpr int TILE = 128, PROMPT_THREADS = 320, STAGES = 2;
+constexpr int TILE = 128, PROMPT_THREADS = 320, SLOTS = 5;
 
 struct PromptArgs {
     AttnArgs a;
     __half *k, *v;   // [n_kv][tiles] images of TILE x hd
-    int *odd;        // [0]: any value that is not finite; then per (KV head, dim) the first slot of +inf, -inf, NaN
+    int *odd;        // [n_kv][tiles]: the V tile has a value that is not finite
+    int kv_dtype;
     int64_t tiles, rows;  // tiles of the sequence; rows T * G of a KV head
     int spin;
 };
 
-// One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a row does
-// not see must not meet them in the product.
-template <int KV> __global__ void __launch_bounds__(256) attn_unpack_kernel(PromptArgs p) {
+// What becomes f16 without turning into infinity or NaN.
+__device__ __forceinline__ bool half_finite(float v) { return (__half_as_ushort(__float2half_rn(v)) & 0x7c00) != 0x7c00; }
+// One value of a cache row (dims of all its heads).
+template <int KV> __device__ __forceinline__ float cache_value(const unsigned char *row, int d) {
+    if (KV == KV_F16) return __half2float(reinterpret_cast<const __half *>(row)[d]);
+    const unsigned char *blk = row + (d >> 5) * KvFormat<KV>::BYTES;
+    const int u = blk[KvFormat<KV>::DATA + (d & 31)];
+    return (float)(KV == KV_Q8 ? (int)(signed char)u : u - 128) * block_scale<KV>(blk);
+}
+
+// One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a
+// row does not see must not meet them in the product.
+template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(PromptArgs p) {
     agn_pdl_prologue();
     const AttnArgs &a = p.a;
     const int64_t tile = blockIdx.x;
-    const int head = blockIdx.y, hd = a.hd, chunks = hd / 8, n_odd = a.n_kv * hd;
+    const int head = blockIdx.y, hd = a.hd, chunks = hd / 8;
+    bool odd = false;
     const bool is_v = blockIdx.z;
     const int end = a.pos_start + (int)a.T;
     const unsigned char *src = is_v ? a.v_cache : a.k_cache;
@@ -68,26 +80,19 @@ template <int KV> __global__ void __launch_bounds__(256) attn_unpack_kernel(Prom
         }
         if (is_v) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float f = __half2float(__float2half_rn(v[k]));
-                if ((__float_as_uint(f) & 0x7f800000u) == 0x7f800000u) {
-                    p.odd[0] = 1;
-                    const int kind = f != f ? 2 : f > 0.0f ? 0 : 1;
-                    atomicMin(&p.odd[4 + kind * n_odd + head * hd + c * 8 + k], (int)slot);
+            for (int k = 0; k < 8; k++)
+                if (!half_finite(v[k])) {
+                    odd = true;
                     v[k] = 0.0f;
                 }
-            }
         }
         __half2 h[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
         *reinterpret_cast<uint4 *>(dst + (c >> 3) * TILE * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4 *>(h);
     }
-}
-
-__global__ void __launch_bounds__(256) attn_odd_reset_kernel(int *odd, int n) {
-    agn_pdl_prologue();
-    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) odd[i] = i < 4 ? 0 : 0x7fffffff;
+    odd = __syncthreads_or(odd);
+    if (is_v && threadIdx.x == 0) p.odd[head * p.tiles + tile] = odd;
 }
 
 // ---- tensor-core instructions
@@ -141,8 +146,8 @@ __device__ __forceinline__ void tmem_loaded(uint32_t *r) {
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int HD> struct PromptSmem {
-    unsigned char q[2][TILE * HD * 2], k[STAGES][TILE * HD * 2], v[STAGES][TILE * HD * 2];
-    uint64_t q_full, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], s_full[2], p_full[2], o_full[2], drained;
+    unsigned char q[2][TILE * HD * 2], kv[SLOTS][TILE * HD * 2];  // tiles in the order K0 V0 K1 V1 ..
+    uint64_t q_full, full[SLOTS], free[SLOTS], s_full[2], p_full[2], o_full[2], drained;
     uint32_t tmem;
     int gave_up;
 };
@@ -152,8 +157,8 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     extern __shared__ unsigned char raw[];
     PromptSmem<HD> &sm = *reinterpret_cast<PromptSmem<HD> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const AttnArgs &a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.n_q / a.n_kv, head = blockIdx.y;
-    const int64_t r0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * 2 * TILE;  // the longest rows first
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.n_q / a.n_kv, head = blockIdx.x % a.n_kv;
+    const int64_t r0 = (int64_t)((gridDim.x - 1 - blockIdx.x) / a.n_kv) * 2 * TILE;  // the rows that see most first, so that the last CTAs are short
     const int64_t last_row = r0 + 2 * TILE - 1 < p.rows ? r0 + 2 * TILE - 1 : p.rows - 1;
     const int tiles = (int)((a.pos_start + last_row / G) / TILE) + 1;  // that the CTA's last row sees
     constexpr uint32_t IMAGE = TILE * HD * 2;
@@ -164,9 +169,9 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     }
     if (tid == 0) {
         agn_mbar_init(&sm.q_full, 256);
-        for (int i = 0; i < STAGES; i++) {
-            agn_mbar_init(&sm.k_full[i], 1); agn_mbar_init(&sm.v_full[i], 1);
-            agn_mbar_init(&sm.k_free[i], 1); agn_mbar_init(&sm.v_free[i], 1);
+        for (int i = 0; i < SLOTS; i++) {
+            agn_mbar_init(&sm.full[i], 1);
+            agn_mbar_init(&sm.free[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             agn_mbar_init(&sm.s_full[i], 1); agn_mbar_init(&sm.p_full[i], 128); agn_mbar_init(&sm.o_full[i], 1);
@@ -193,56 +198,56 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         if (lane == 0) {
             const unsigned char *k = reinterpret_cast<const unsigned char *>(p.k) + (int64_t)head * p.tiles * IMAGE;
             const unsigned char *v = reinterpret_cast<const unsigned char *>(p.v) + (int64_t)head * p.tiles * IMAGE;
-            int issued_k = 0, issued_v = 0;
-            for (int j = 0; j < tiles; j++) {
-                const int s = j % STAGES;
-                if (j >= STAGES && !wait(&sm.k_free[s], (j / STAGES - 1) & 1)) break;
-                agn_mbar_expect_tx(&sm.k_full[s], IMAGE);
-                agn_bulk_g2s(sm.k[s], k + (int64_t)j * IMAGE, IMAGE, &sm.k_full[s]);
-                issued_k++;
-                if (j >= STAGES && !wait(&sm.v_free[s], (j / STAGES - 1) & 1)) break;
-                agn_mbar_expect_tx(&sm.v_full[s], IMAGE);
-                agn_bulk_g2s(sm.v[s], v + (int64_t)j * IMAGE, IMAGE, &sm.v_full[s]);
-                issued_v++;
+            int n = 0;
+            for (; n < 2 * tiles; n++) {
+                const int at = n % SLOTS;
+                if (n >= SLOTS && !wait(&sm.free[at], (n / SLOTS - 1) & 1)) break;
+                agn_mbar_expect_tx(&sm.full[at], IMAGE);
+                agn_bulk_g2s(sm.kv[at], (n & 1 ? v : k) + (int64_t)(n >> 1) * IMAGE, IMAGE, &sm.full[at]);
             }
-            // no copy may be in flight when the CTA ends: the last one of every stage (earlier ones have been waited for by the products)
-            for (int j = issued_k > STAGES ? issued_k - STAGES : 0; j < issued_k; j++) (void)agn_mbar_wait(&sm.k_full[j % STAGES], (j / STAGES) & 1, p.spin);
-            for (int j = issued_v > STAGES ? issued_v - STAGES : 0; j < issued_v; j++) (void)agn_mbar_wait(&sm.v_full[j % STAGES], (j / STAGES) & 1, p.spin);
+            // no copy may be in flight when the CTA ends: the last one of every slot (the products have waited for the earlier ones)
+            for (int i = n > SLOTS ? n - SLOTS : 0; i < n; i++) (void)agn_mbar_wait(&sm.full[i % SLOTS], (i / SLOTS) & 1, p.spin);
         }
         __syncwarp();
     } else if (warp == 9) {
         if (lane == 0) {
-            const uint32_t qa = agn_smem_u32(sm.q[0]), ka = agn_smem_u32(sm.k[0]), va = agn_smem_u32(sm.v[0]);
-            auto scores = [&](int i, int j) {  // S_i = Q_i K_j^T
+            const uint32_t qa = agn_smem_u32(sm.q[0]), kva = agn_smem_u32(sm.kv[0]);
+            auto scores = [&](int i, uint32_t tile) {  // S_i = Q_i K^T with the K tile there
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ks++) {
                     const uint32_t at = (ks >> 2) * TILE * 128 + (ks & 3) * 32;
-                    mma_ss(tmem + i * 128, smem_operand(qa + i * IMAGE + at, 16), smem_operand(ka + (j % STAGES) * IMAGE + at, 16), mma_shape(TILE, false), ks > 0);
+                    mma_ss(tmem + i * 128, smem_operand(qa + i * IMAGE + at, 16), smem_operand(tile + at, 16), mma_shape(TILE, false), ks > 0);
                 }
                 mma_commit(&sm.s_full[i]);
             };
-            bool ok = wait(&sm.q_full, 0) && wait(&sm.k_full[0], 0);
+            bool ok = wait(&sm.q_full, 0) && wait(&sm.full[0], 0);
             if (ok) {
                 fence_after();
-                scores(0, 0);
-                scores(1, 0);
-                mma_commit(&sm.k_free[0]);
+                scores(0, kva);
+                scores(1, kva);
+                mma_commit(&sm.free[0]);
             }
+            int v = 1, k = 2;  // slots of V_j and K_(j+1), and how often they have been filled before
+            uint32_t v_turn = 0, k_turn = 0;
             for (int j = 0; ok && j < tiles; j++) {
-                const int s = j % STAGES;
-                if (!wait(&sm.v_full[s], (j / STAGES) & 1)) break;
-                if (j + 1 < tiles && !wait(&sm.k_full[(j + 1) % STAGES], ((j + 1) / STAGES) & 1)) break;
+                const bool more = j + 1 < tiles;
+                const uint32_t vt = kva + v * IMAGE, kt = kva + k * IMAGE;
+                if (!wait(&sm.full[v], v_turn & 1)) break;
                 for (int i = 0; i < 2; i++) {
-                    if (!wait(&sm.p_full[i], j & 1)) { ok = false; break; }
+                    if (!(ok = wait(&sm.p_full[i], j & 1))) break;
                     fence_after();
 #pragma unroll
                     for (int ks = 0; ks < TILE / 16; ks++)  // O_i += P_i V_j, 16 slots at a time
-                        mma_ts(tmem + 256 + i * 128, tmem + i * 128 + ks * 8, smem_operand(va + s * IMAGE + ks * 2048, TILE * 128), mma_shape(HD, true), j > 0 || ks > 0);
-                    if (j + 1 < tiles) scores(i, j + 1);  // behind that product, which still reads the weights in S_i's place
-                    else mma_commit(&sm.o_full[i]);
+                        mma_ts(tmem + 256 + i * 128, tmem + i * 128 + ks * 8, smem_operand(vt + ks * 2048, TILE * 128), mma_shape(HD, true),
+                               j > 0 || ks > 0);
+                    if (i == 1) mma_commit(&sm.free[v]);
+                    if (!more) mma_commit(&sm.o_full[i]);
+                    else if (i == 1 || (ok = wait(&sm.full[k], k_turn & 1))) scores(i, kt);  // behind that product, which reads the weights in S_i's place
+                    else break;
                 }
-                mma_commit(&sm.v_free[s]);
-                if (j + 1 < tiles) mma_commit(&sm.k_free[(j + 1) % STAGES]);
+                if (ok && more) mma_commit(&sm.free[k]);
+                if ((v += 2) >= SLOTS) { v -= SLOTS; v_turn++; }
+                if ((k += 2) >= SLOTS) { k -= SLOTS; k_turn++; }
             }
             mma_commit(&sm.drained);  // every product is done before the tensor memory goes back
             (void)agn_mbar_wait(&sm.drained, 0, p.spin);
@@ -253,13 +258,20 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         const int i = warp >> 2, row = tid & 127;
         const int64_t r = r0 + i * TILE + row;
         const bool there = r < p.rows;
-        const int64_t t = (there ? r : p.rows - 1) / G, h = (there ? r : p.rows - 1) % G;
-        const int last = a.pos_start + (int)t;  // the last slot it sees
-        const int64_t at = (t * a.n_q + head * G + h) * HD;
-        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at);
-#pragma unroll
-        for (int c = 0; c < HD / 8; c++)
-            *reinterpret_cast<uint4 *>(sm.q[i] + (c >> 3) * TILE * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = there ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+        const uint32_t tok = (uint32_t)(there ? r : p.rows - 1) / (uint32_t)G;
+        const int last = a.pos_start + (int)tok;  // the last slot it sees
+        const int64_t own = there ? ((int64_t)tok * a.n_q + head * G + (uint32_t)r % (uint32_t)G) * HD : -1;  // its first value in q and out
+        // the warp's 32 rows, whole rows side by side
+        constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per instruction
+        const int piece = lane % CPR;
+        unsigned char *qs = sm.q[i] + (piece >> 3) * TILE * 128 + (warp & 3) * 32 * 128;
+#pragma unroll 8
+        for (int k = 0; k < 32; k += RPI) {
+            const int wr = k + lane / CPR;
+            const int64_t at = __shfl_sync(0xffffffffu, own, wr);
+            const uint4 x = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at) + piece) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(qs + wr * 128 + (((piece & 7) ^ (wr & 7)) << 4)) = x;
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         bar_arrive(&sm.q_full);
 
@@ -344,36 +356,30 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         if (ok && (ok = wait(&sm.o_full[i], 0))) {
             fence_after();
             const float inv = 1.0f / l;
-            const bool any = p.odd[0] != 0;
-            __half *out = static_cast<__half *>(a.out) + at;
-            const int n_odd = a.n_kv * HD;
+            // The output goes out through the queries' place in shared memory (the last product that reads them is done), whole rows side by side.
+            unsigned char *stage = sm.q[i] + (warp & 3) * 32 * HD * 2;
 #pragma unroll
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 tmem_load32(o_at + c, o);
                 tmem_loaded(o);
-                if (any) {  // values that are not finite reach the rows that see their slot
-                    for (int k = 0; k < 32; k++) {
-                        const int *f = p.odd + 4 + head * HD + c + k;
-                        const bool up = f[0] <= last, down = f[n_odd] <= last, nan = f[2 * n_odd] <= last;
-                        const float bad = nan || (up && down) ? NAN : up ? INFINITY : -INFINITY;
-                        if (up || down || nan) {
 #pragma unroll
-                            for (int q = 0; q < 32; q++)
-                                if (q == k) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv + bad);
-                        }
-                    }
+                for (int k = 0; k < 32; k += 8) {
+                    __half2 h2[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) h2[q] = __floats2half2_rn(__uint_as_float(o[k + 2 * q]) * inv, __uint_as_float(o[k + 2 * q + 1]) * inv);
+                    const int pc = (c + k) / 8;
+                    *reinterpret_cast<uint4 *>(stage + lane * HD * 2 + ((pc ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(h2);
                 }
-                if (there) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        __half2 h2[4];
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            h2[q] = __floats2half2_rn(__uint_as_float(o[k + 2 * q]) * inv, __uint_as_float(o[k + 2 * q + 1]) * inv);
-                        *reinterpret_cast<uint4 *>(out + c + k) = *reinterpret_cast<const uint4 *>(h2);
-                    }
-                }
+            }
+            __syncwarp();
+#pragma unroll 8
+            for (int k = 0; k < 32; k += RPI) {
+                const int wr = k + lane / CPR;
+                const int64_t at = __shfl_sync(0xffffffffu, own, wr);
+                if (at >= 0)
+                    *reinterpret_cast<uint4 *>(static_cast<__half *>(a.out) + at + piece * 8) =
+                        *reinterpret_cast<const uint4 *>(stage + wr * HD * 2 + ((piece ^ (wr & 7)) << 4));
             }
         }
     }
@@ -384,24 +390,50 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
     if (tid == 0 && sm.gave_up) atomicOr(a.flags, AGN_FLAG_TIMEOUT);
+
+    // Rare: V holds values that are not finite.  They were 0 in the product; a row that sees one gets it, two of different signs or a NaN give
+    // NaN.  A thread per output value, slot by slot from the cache.
+    bool any = false;
+    for (int j = tid; j < tiles; j += PROMPT_THREADS) any |= p.odd[head * p.tiles + j] != 0;
+    if (!__syncthreads_or(any)) return;
+    for (int64_t x = tid; x < 2 * TILE * HD; x += PROMPT_THREADS) {
+        const int64_t r = r0 + x / HD;
+        const int d = (int)(x % HD), last = a.pos_start + (int)(r / G);
+        if (r >= p.rows) break;
+        bool up = false, down = false, nan = false;
+        for (int s = 0; s <= last; s++) {
+            if (!p.odd[head * p.tiles + s / TILE]) {
+                s |= TILE - 1;
+                continue;
+            }
+            const unsigned char *row = a.v_cache + (int64_t)s * a.bytes_per_token;
+            const int at = head * HD + d;
+            const float v = p.kv_dtype == AGN_F16 ? cache_value<KV_F16>(row, at) : p.kv_dtype == AGN_Q8_0 ? cache_value<KV_Q8>(row, at) : cache_value<KV_WORDS>(row, at);
+            if (half_finite(v)) continue;
+            if (v != v) nan = true;
+            else if (v > 0.0f) up = true;
+            else down = true;
+        }
+        if (up || down || nan) {
+            __half *o = static_cast<__half *>(a.out) + ((r / G) * a.n_q + head * G + r % G) * HD + d;
+            *o = __float2half_rn(__half2float(*o) + (nan || (up && down) ? NAN : up ? INFINITY : -INFINITY));
+        }
+    }
 }
 
 int64_t image_bytes(int64_t slots, int n_kv, int hd) { return (slots + TILE - 1) / TILE * TILE * n_kv * hd * 2; }
-int64_t odd_ints(int n_kv, int hd) { return 4 + 3 * (int64_t)n_kv * hd; }
+int64_t odd_ints(int64_t slots, int n_kv) { return (slots + TILE - 1) / TILE * n_kv; }
 
 template <int HD> int32_t launch_prompt(agn_ctx *ctx, const PromptArgs &p, int kv_dtype) {
     const size_t smem = sizeof(PromptSmem<HD>) + 1024;
     if (agn_ring_ctas_per_sm(ctx, attn_prompt_kernel<HD>, PROMPT_THREADS, smem) < 1)
         return agn_fail(ctx, AGN_ECUDA, "attention_kv: the prompt kernel does not fit the device's shared memory");
-    const int n = (int)odd_ints(p.a.n_kv, HD);
-    agn_launch(ctx, attn_odd_reset_kernel, dim3((unsigned)((n + 255) / 256 < 64 ? (n + 255) / 256 : 64)), dim3(256), 0, p.odd, n);
-    AGN_LAUNCHED(ctx, "attention_kv_prompt");
     const dim3 tiles((unsigned)p.tiles, (unsigned)p.a.n_kv, 2);
-    if (kv_dtype == AGN_F16) agn_launch(ctx, attn_unpack_kernel<KV_F16>, tiles, dim3(256), 0, p);
-    else if (kv_dtype == AGN_Q8_0) agn_launch(ctx, attn_unpack_kernel<KV_Q8>, tiles, dim3(256), 0, p);
-    else agn_launch(ctx, attn_unpack_kernel<KV_WORDS>, tiles, dim3(256), 0, p);
+    if (kv_dtype == AGN_F16) agn_launch(ctx, attn_unpack_kernel<KV_F16>, tiles, dim3(1024), 0, p);
+    else if (kv_dtype == AGN_Q8_0) agn_launch(ctx, attn_unpack_kernel<KV_Q8>, tiles, dim3(1024), 0, p);
+    else agn_launch(ctx, attn_unpack_kernel<KV_WORDS>, tiles, dim3(1024), 0, p);
     AGN_LAUNCHED(ctx, "attention_kv_prompt");
-    agn_launch(ctx, attn_prompt_kernel<HD>, dim3((unsigned)((p.rows + 2 * TILE - 1) / (2 * TILE)), (unsigned)p.a.n_kv), dim3(PROMPT_THREADS), smem, p);
+    agn_launch(ctx, attn_prompt_kernel<HD>, dim3((unsigned)((p.rows + 2 * TILE - 1) / (2 * TILE) * p.a.n_kv)), dim3(PROMPT_THREADS), smem, p);
     AGN_LAUNCHED(ctx, "attention_kv_prompt");
     return AGN_OK;
 }
@@ -409,11 +441,11 @@ template <int HD> int32_t launch_prompt(agn_ctx *ctx, const PromptArgs &p, int k
 }  // namespace
 
 bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd) {
-    return (hd == 64 || hd == 128) && T * (n_q / n_kv) >= AGN_PROMPT_MIN_ROWS && T >= AGN_PROMPT_MIN_TOKENS;
+    return (hd == 64 || hd == 128) && T * (n_q / n_kv) >= AGN_PROMPT_MIN_ROWS && T >= AGN_PROMPT_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30);
 }
 
 int64_t agn_attention_prompt_workspace(int64_t slots, int n_kv, int hd) {
-    return 2 * image_bytes(slots, n_kv, hd) + (odd_ints(n_kv, hd) * 4 + 15) / 16 * 16;
+    return 2 * image_bytes(slots, n_kv, hd) + (odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;
 }
 
 int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace) {
@@ -426,6 +458,7 @@ int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, 
     p.odd = reinterpret_cast<int *>(w + 2 * image);
     p.tiles = (slots + TILE - 1) / TILE;
     p.rows = a.T * (a.n_q / a.n_kv);
+    p.kv_dtype = kv_dtype;
     p.spin = ctx->mbar_spin_limit;
     return a.hd == 64 ? launch_prompt<64>(ctx, p, kv_dtype) : launch_prompt<128>(ctx, p, kv_dtype);
 }
