@@ -163,6 +163,26 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     const int tiles = (int)((a.pos_start + last_row / G) / TILE) + 1;  // that the CTA's last row sees
     constexpr uint32_t IMAGE = TILE * HD * 2;
 
+    // ---- warps 0-7: the query row of this thread, and Q on its way (a warp's 32 rows, whole rows side by side)
+    const int i = warp >> 2;
+    const int64_t r = r0 + i * TILE + (tid & 127);
+    const bool there = r < p.rows;
+    const uint32_t tok = (uint32_t)(there ? r : p.rows - 1) / (uint32_t)G;
+    const int last = a.pos_start + (int)tok;  // the last slot it sees
+    const int64_t own = there ? ((int64_t)tok * a.n_q + head * G + (uint32_t)r % (uint32_t)G) * HD : -1;  // its first value in q and out
+    constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per instruction
+    const int piece = lane % CPR;
+    if (warp < 8) {
+        const uint32_t qs = agn_smem_u32(sm.q[i]) + (piece >> 3) * TILE * 128 + (warp & 3) * 32 * 128;
+#pragma unroll
+        for (int k = 0; k < 32; k += RPI) {
+            const int wr = k + lane / CPR;
+            const int64_t at = __shfl_sync(0xffffffffu, own, wr);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qs + wr * 128 + (((piece & 7) ^ (wr & 7)) << 4)),
+                         "l"(static_cast<const __half *>(a.q) + (at >= 0 ? at + piece * 8 : 0)), "r"(at >= 0 ? 16 : 0)
+                         : "memory");
+        }
+    }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(agn_smem_u32(&sm.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -255,24 +275,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         __syncwarp();
     } else {
         // ---- a query row per thread
-        const int i = warp >> 2, row = tid & 127;
-        const int64_t r = r0 + i * TILE + row;
-        const bool there = r < p.rows;
-        const uint32_t tok = (uint32_t)(there ? r : p.rows - 1) / (uint32_t)G;
-        const int last = a.pos_start + (int)tok;  // the last slot it sees
-        const int64_t own = there ? ((int64_t)tok * a.n_q + head * G + (uint32_t)r % (uint32_t)G) * HD : -1;  // its first value in q and out
-        // the warp's 32 rows, whole rows side by side
-        constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte pieces of a row, rows per instruction
-        const int piece = lane % CPR;
-        unsigned char *qs = sm.q[i] + (piece >> 3) * TILE * 128 + (warp & 3) * 32 * 128;
-#pragma unroll 8
-        for (int k = 0; k < 32; k += RPI) {
-            const int wr = k + lane / CPR;
-            const int64_t at = __shfl_sync(0xffffffffu, own, wr);
-            const uint4 x = at >= 0 ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at) + piece) : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(qs + wr * 128 + (((piece & 7) ^ (wr & 7)) << 4)) = x;
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("cp.async.wait_all;\nfence.proxy.async.shared::cta;" ::: "memory");  // this thread's share of Q, for the tensor cores
         bar_arrive(&sm.q_full);
 
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // 32 lanes of the tensor memory per warp, lane number in the upper half
