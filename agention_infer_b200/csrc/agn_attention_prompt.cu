@@ -214,6 +214,9 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         return false;
     };
 
+    // the same for a whole warp: its lanes go on together or not at all
+    auto wait_warp = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); };
+
     if (warp == 8) {
         if (lane == 0) {
             const unsigned char *k = reinterpret_cast<const unsigned char *>(p.k) + (int64_t)head * p.tiles * IMAGE;
@@ -285,7 +288,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < tiles; j++) {
-            if (!(ok = wait(&sm.s_full[i], j & 1))) break;
+            if (!(ok = wait_warp(&sm.s_full[i], j & 1))) break;
             fence_after();
             // The scores are read twice, 32 at a time: 128 of them beside the rest do not fit the 168 registers of a thread.
             const int seen = last - j * TILE;  // slots c <= seen of this tile
@@ -356,7 +359,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
             fence_before();
             bar_arrive(&sm.p_full[i]);
         }
-        if (ok && (ok = wait(&sm.o_full[i], 0))) {
+        if (ok && (ok = wait_warp(&sm.o_full[i], 0))) {
             fence_after();
             const float inv = 1.0f / l;
             // The output goes out through the queries' place in shared memory (the last product that reads them is done), whole rows side by side.
