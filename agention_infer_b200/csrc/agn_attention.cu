@@ -120,6 +120,10 @@ int64_t attn_workspace(int64_t T, int n_q, int hd) {
     return T > 0 && T <= ATTN_MAX_SPLIT_ROWS ? (int64_t)2 * 2 * ATTN_MAX_SMS * n_q * (hd + 4) * 4 : 0;
 }
 
+// Few rows of one sequence are cheaper as single rows.
+constexpr int CHUNK_MIN_TOKENS = 4;
+bool chunk_fits(int64_t T, int n_q, int n_kv) { return T >= CHUNK_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30); }
+
 template <typename T>
 int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const void *k_cache, const void *v_cache, int64_t rows,
                      int32_t n_q, int32_t n_kv, int32_t hd, const int32_t *pos, int32_t pos_start, const int32_t *seq,
@@ -143,7 +147,8 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     if (!agn_aligned(k_cache, ca) || !agn_aligned(v_cache, ca))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: caches must be %d-byte aligned", ca);
     const bool prompt = !pos && sizeof(T) == 2 && agn_attention_prompt_fits(rows, n_q, n_kv, hd);
-    const int64_t need = prompt ? agn_attention_prompt_workspace(pos_start + rows, n_kv, hd) : attn_workspace(rows, n_q, hd);
+    const bool chunk = !pos && !prompt && chunk_fits(rows, n_q, n_kv);
+    const int64_t need = prompt ? agn_attention_prompt_workspace(pos_start + rows, n_kv, hd) : chunk ? 0 : attn_workspace(rows, n_q, hd);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !agn_aligned16(workspace)))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     AGN_CUDA(ctx, cudaSetDevice(ctx->device));
@@ -153,6 +158,7 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     a.bytes_per_token = (int)agn_kv_bytes_per_token(kv_dtype, (int64_t)n_kv * hd); a.scale = scale; a.flags = ctx->d_flags;
     ctx->flags_dirty = true;
     if (prompt) return agn_attention_prompt_f16(ctx, a, kv_dtype, workspace);
+    if (chunk) return agn_attention_chunk(ctx, a, kv_dtype, sizeof(T) == 2);
     const int block_bytes = kv_dtype == AGN_F16 ? 64 : kv_dtype == AGN_Q8_0 ? 34 : 36;
     const DecodePlan p = decode_plan(rows, n_q, n_kv, hd, max_seq, block_bytes, kv_dtype == AGN_F16, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);
     DecodeArgs d;

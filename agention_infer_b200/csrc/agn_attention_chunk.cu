@@ -1,0 +1,357 @@
+// Attention of a prompt's rows (consecutive positions of one sequence) over the KV cache, to f32's precision: f32 rows, and f16 rows of head sizes
+// that the tensor-memory form (agn_attention_prompt.cu) does not cover.
+//
+// Bound by the matrix units: per 16 rows, 8 slots and 32 dims 4 products m16n8k16 (f16) for the scores and 8 m16n8k8 (tf32) for the output, which caps the
+// kernel near 190 TFLOP/s for heads of 128.  Precision comes from two-part operands as in the decode kernel: queries as hi + lo f16 against the cached
+// bytes (exact in f16), weights times the block scale as hi + lo tf32 against the cached bytes.  A CTA takes 16 rows per warp of one KV head - row r
+// is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory once for all warps,
+// the next 64 while these are worked on.
+#include <math.h>
+
+#include "agn_attention_decode.cuh"
+
+namespace {
+
+constexpr int SL = 64;  // slots of a tile
+
+template <int NB> struct ChunkShape {
+    static constexpr int HD = NB * 32, WARPS = NB <= 4 ? 8 : 4, THREADS = 32 * WARPS, ROWS = 16 * WARPS, ROW = HD + 8;  // f16 elements of a row in shared memory
+    static constexpr int BLOCKS = (2 * SL * NB + THREADS - 1) / THREADS;  // cache blocks that a thread converts per tile
+};
+
+template <int NB> struct ChunkTiles {
+    using C = ChunkShape<NB>;
+    __half q[2][C::ROWS * C::ROW];  // hi, lo
+    __half k[2][SL * C::ROW], v[2][SL * C::ROW];
+    float ks[2][SL][NB], vs[2][SL][NB], coef[C::ROWS];
+    int odd;
+};
+
+// One block of 32 values on its way from the cache: 16 words of f16, or 8 words of bytes and a scale.
+template <int KV> struct Block {
+    uint32_t w[KV == KV_F16 ? 16 : 8];
+    float scale;
+};
+
+template <int KV> __device__ __forceinline__ void fetch_block(Block<KV> &x, const unsigned char *p, bool there) {
+#pragma unroll
+    for (int i = 0; i < (KV == KV_F16 ? 16 : 8); i++) x.w[i] = KV == KV_WORDS ? 0x80808080u : 0u;
+    x.scale = 0.0f;
+    if (!there) return;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p);
+    if (KV == KV_WORDS) {
+        x.scale = __uint_as_float(w[0]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x.w[i] = w[i + 1];
+    } else if (KV == KV_Q8) {
+        x.scale = __half2float(*reinterpret_cast<const __half *>(p));
+        if (reinterpret_cast<uintptr_t>(p) & 2) {
+            const uint32_t *d = reinterpret_cast<const uint32_t *>(p + 2);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x.w[i] = d[i];
+        } else {  // the bytes begin in the middle of a word and end in the middle of one
+            uint32_t a = w[0];
+#pragma unroll
+            for (int i = 0; i < 7; i++) {
+                const uint32_t b = w[i + 1];
+                x.w[i] = __funnelshift_r(a, b, 16);
+                a = b;
+            }
+            x.w[7] = __funnelshift_r(a, *reinterpret_cast<const uint16_t *>(p + 32), 16);
+        }
+    } else if (!(reinterpret_cast<uintptr_t>(p) & 15)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint4 y = reinterpret_cast<const uint4 *>(p)[i];
+            x.w[4 * i] = y.x; x.w[4 * i + 1] = y.y; x.w[4 * i + 2] = y.z; x.w[4 * i + 3] = y.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) x.w[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t *>(p)[2 * i + 1] << 16;
+    }
+}
+
+// To 32 f16 values; returns whether one of an f16 block is not finite (it becomes 0 where `clean`).
+template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x, __half *to, bool clean) {
+    bool odd = false;
+    uint4 *dst = reinterpret_cast<uint4 *>(to);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t h[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (KV == KV_F16) {
+                h[c] = x.w[4 * i + c];
+                if (clean) {
+                    const bool o0 = (h[c] & 0x7c00u) == 0x7c00u, o1 = (h[c] & 0x7c000000u) == 0x7c000000u;
+                    odd |= o0 || o1;
+                    if (o0) h[c] &= 0xffff0000u;
+                    if (o1) h[c] &= 0x0000ffffu;
+                }
+            } else {
+                const uint32_t u = offset_bytes<KV>(x.w[2 * i + (c >> 1)]);
+                h[c] = bytes_to_half2(u, c & 1 ? 0x4342 : 0x4140);
+            }
+        }
+        dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    return odd;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
+}
+
+template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THREADS, 1) attn_chunk_kernel(const __grid_constant__ DecodeArgs d) {
+    agn_pdl_prologue();
+    using C = ChunkShape<NB>;
+    using F = KvFormat<KV>;
+    extern __shared__ __align__(128) unsigned char raw[];
+    ChunkTiles<NB> &sm = *reinterpret_cast<ChunkTiles<NB> *>(raw);
+    const AttnArgs &a = d.a;
+    constexpr int HD = C::HD, ROW = C::ROW;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, G = a.n_q / a.n_kv, kvh = blockIdx.x % a.n_kv;
+    const int rows = (int)a.T * G, r0 = (int)((gridDim.x - 1 - blockIdx.x) / a.n_kv) * C::ROWS;  // the rows that see most first
+    const int last_row = min(r0 + C::ROWS, rows) - 1, end = a.pos_start + last_row / G + 1, tiles = (end + SL - 1) / SL;
+    if (tid == 0) sm.odd = 0;
+
+    auto fetch = [&](Block<KV> &x, int i, int tile) {
+        const int n = tid + i * C::THREADS, b = n % NB, slot = tile * SL + n / NB % SL;
+        const unsigned char *cache = n < SL * NB ? a.k_cache : a.v_cache;
+        fetch_block<KV>(x, cache + (int64_t)slot * a.bytes_per_token + (kvh * NB + b) * F::BYTES, n < 2 * SL * NB && slot < end);
+    };
+    auto place = [&](const Block<KV> &x, int i, int tile) {
+        const int n = tid + i * C::THREADS, b = n % NB, slot = n / NB % SL;
+        const bool is_k = n < SL * NB;
+        if (n >= 2 * SL * NB) return;
+        const bool odd = place_block<KV>(x, (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, !is_k);
+        if (KV != KV_F16) (is_k ? sm.ks : sm.vs)[tile & 1][slot][b] = x.scale;
+        if (KV == KV_F16 && odd) sm.odd = 1;
+    };
+    constexpr int HELD = NB <= 4 ? C::BLOCKS : 1;  // blocks that wait in registers while a tile is worked on; larger heads have none left for them
+    Block<KV> next[HELD];
+    auto fetch_tile = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < C::BLOCKS; i++) {
+            fetch(next[i % HELD], i, tile);
+            if (NB > 4) place(next[0], i, tile);
+        }
+    };
+    auto place_tile = [&](int tile) {
+        if (NB <= 4) {
+#pragma unroll
+            for (int i = 0; i < C::BLOCKS; i++) place(next[i % HELD], i, tile);
+        }
+    };
+    __syncthreads();
+    fetch_tile(0);
+
+    // ---- Q, a warp's 16 rows: largest value to [1, 2), two f16 parts
+    for (int i = 0; i < 16; i++) {
+        const int r = r0 + warp * 16 + i;
+        const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD;
+        float x[NB], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            x[c] = r >= rows ? 0.0f : d.act16 ? __half2float(static_cast<const __half *>(a.q)[at + c * 32 + lane]) : static_cast<const float *>(a.q)[at + c * 32 + lane];
+            amax = fmaxf(amax, fabsf(x[c]));
+        }
+        amax = agn_warp_max(amax);
+        const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+        if (lane == 0) sm.coef[warp * 16 + i] = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), 1.17549435e-38f);
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            const float v = x[c] * down;
+            const __half h = __float2half_rn(v);
+            sm.q[0][(warp * 16 + i) * ROW + c * 32 + lane] = h;
+            sm.q[1][(warp * 16 + i) * ROW + c * 32 + lane] = __float2half_rn(v - __half2float(h));
+        }
+    }
+    place_tile(0);
+    __syncthreads();
+
+    const int ra = r0 + warp * 16 + g;  // this lane's rows: ra and ra + 8
+    const float coef[2] = {sm.coef[warp * 16 + g], sm.coef[warp * 16 + g + 8]};
+    const int lim[2] = {a.pos_start + min(ra, rows - 1) / G, a.pos_start + min(ra + 8, rows - 1) / G}, warp_first = a.pos_start + min(r0 + warp * 16, rows - 1) / G;
+    const int warp_last = a.pos_start + min(r0 + warp * 16 + 15, rows - 1) / G;
+    float o[4 * NB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4 * NB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+    for (int tile = 0; tile < tiles; tile++) {
+        if (tile + 1 < tiles) fetch_tile(tile + 1);
+        if (tile * SL <= warp_last) {  // a warp whose rows see none of it waits for the others
+            const int buf = tile & 1;
+            float s[SL / 8][4];
+#pragma unroll
+            for (int n = 0; n < SL / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float blk[SL / 8][4];
+#pragma unroll
+                for (int n = 0; n < SL / 8; n++) blk[n][0] = blk[n][1] = blk[n][2] = blk[n][3] = 0.0f;
+                float(*acc)[4] = KV == KV_F16 ? s : blk;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    uint32_t hi[4], lo[4];
+                    const int qa = (warp * 16 + (lane & 15)) * ROW + b * 32 + k * 16 + (lane >> 4) * 8;
+                    ldsm4(hi, sm.q[0] + qa);
+                    ldsm4(lo, sm.q[1] + qa);
+#pragma unroll
+                    for (int n = 0; n < SL / 8; n += 2) {
+                        uint32_t kf[4];  // two groups of eight slots
+                        ldsm4(kf, sm.k[buf] + (n * 8 + (lane & 7) + (lane >> 4) * 8) * ROW + b * 32 + k * 16 + ((lane >> 3) & 1) * 8);
+                        mma_f16(acc[n], hi, kf[0], kf[1]);
+                        mma_f16(acc[n + 1], hi, kf[2], kf[3]);
+                        mma_f16(acc[n], lo, kf[0], kf[1]);
+                        mma_f16(acc[n + 1], lo, kf[2], kf[3]);
+                    }
+                }
+                if (KV != KV_F16) {
+#pragma unroll
+                    for (int n = 0; n < SL / 8; n++) {
+                        const float s0 = sm.ks[buf][8 * n + 2 * t4][b], s1 = sm.ks[buf][8 * n + 2 * t4 + 1][b];
+                        s[n][0] = __fmaf_rn(blk[n][0], s0, s[n][0]);
+                        s[n][1] = __fmaf_rn(blk[n][1], s1, s[n][1]);
+                        s[n][2] = __fmaf_rn(blk[n][2], s0, s[n][2]);
+                        s[n][3] = __fmaf_rn(blk[n][3], s1, s[n][3]);
+                    }
+                }
+            }
+            const bool edge = tile * SL + SL - 1 > warp_first;
+            float mt[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < SL / 8; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (edge && tile * SL + 8 * n + 2 * t4 + (i & 1) > lim[i >> 1]) s[n][i] = -INFINITY;
+                    mt[i >> 1] = fmaxf(mt[i >> 1], s[n][i]);
+                }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 1));
+                mt[i] = fmaxf(mt[i], __shfl_xor_sync(0xffffffffu, mt[i], 2)) * coef[i];
+            }
+            if (__any_sync(0xffffffffu, mt[0] > m[0] + 8.0f || mt[1] > m[1] + 8.0f)) {  // true at the first tile
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    mt[i] = fmaxf(mt[i], m[i]);
+                    const float c = ex2(m[i] - (mt[i] == -INFINITY ? 0.0f : mt[i]));
+                    l[i] *= c;
+                    m[i] = mt[i];
+#pragma unroll
+                    for (int n = 0; n < 4 * NB; n++) { o[n][2 * i] *= c; o[n][2 * i + 1] *= c; }
+                }
+            }
+            const float mu[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int n = 0; n < SL / 8; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    s[n][i] = ex2(__fmaf_rn(s[n][i], coef[i >> 1], -mu[i >> 1]));
+                    l[i >> 1] += s[n][i];
+                }
+            // ---- O += P V; the sums of a tile in the matrix unit (whose adder cuts), the running ones by rounded additions
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float acc[4][4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < SL / 8; n++) {
+                    float hi[4], lo[4], w[4] = {s[n][0], s[n][1], s[n][2], s[n][3]};
+                    if (KV != KV_F16) {
+                        const float s0 = sm.vs[buf][8 * n + 2 * t4][b], s1 = sm.vs[buf][8 * n + 2 * t4 + 1][b];
+                        w[0] *= s0; w[1] *= s1; w[2] *= s0; w[3] *= s1;
+                        if (edge) {  // a scale that is not finite, in a slot that the row does not see
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (tile * SL + 8 * n + 2 * t4 + (i & 1) > lim[i >> 1]) w[i] = 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        hi[i] = __uint_as_float(__float_as_uint(w[i]) & 0xffffe000u);
+                        lo[i] = fminf(w[i] - hi[i], 1e35f);  // with an infinite scale not inf - inf
+                    }
+                    const uint2 x0 = *reinterpret_cast<const uint2 *>(sm.v[buf] + (8 * n + 2 * t4) * ROW + b * 32 + 4 * g);
+                    const uint2 x1 = *reinterpret_cast<const uint2 *>(sm.v[buf] + (8 * n + 2 * t4 + 1) * ROW + b * 32 + 4 * g);
+                    const float2 u0 = __half22float2(*reinterpret_cast<const __half2 *>(&x0.x)), u1 = __half22float2(*reinterpret_cast<const __half2 *>(&x0.y));
+                    const float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&x1.x)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&x1.y));
+                    const float e0[4] = {u0.x, u0.y, u1.x, u1.y}, e1[4] = {v0.x, v0.y, v1.x, v1.y};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) mma_tf32(acc[c], hi[0], hi[2], hi[1], hi[3], e0[c], e1[c]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) mma_tf32(acc[c], lo[0], lo[2], lo[1], lo[3], e0[c], e1[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) add4(o[4 * b + c], acc[c]);
+            }
+        }
+        if (tile + 1 < tiles) place_tile(tile + 1);
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int r = ra + 8 * i;
+        if (r >= rows) continue;
+        const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD;
+        const float inv = 1.0f / l[i];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {  // dims 8 t4 .. 8 t4 + 7 of the block
+            store_act4(d, at, b * 8 + 2 * t4, make_float4(o[4 * b][2 * i] * inv, o[4 * b + 1][2 * i] * inv, o[4 * b + 2][2 * i] * inv, o[4 * b + 3][2 * i] * inv));
+            store_act4(d, at, b * 8 + 2 * t4 + 1,
+                       make_float4(o[4 * b][2 * i + 1] * inv, o[4 * b + 1][2 * i + 1] * inv, o[4 * b + 2][2 * i + 1] * inv, o[4 * b + 3][2 * i + 1] * inv));
+        }
+    }
+    if (KV == KV_F16) {  // rare: V held values that are not finite
+        __syncthreads();
+        if (!sm.odd) return;
+        for (int x = tid; x < C::ROWS * HD; x += C::THREADS) {
+            const int r = r0 + x / HD, dim = x % HD;
+            if (r >= rows) break;
+            const float bad = odd_value(a, AGN_F16, kvh * HD + dim, a.pos_start + r / G, [](int) { return true; }, 1);
+            if (bad == 0.0f) continue;
+            const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD + dim;
+            store_act(d, at, bad + (d.act16 ? __half2float(static_cast<const __half *>(a.out)[at]) : static_cast<const float *>(a.out)[at]));
+        }
+    }
+}
+
+template <int KV, int NB> int32_t launch_chunk(agn_ctx *ctx, const DecodeArgs &d) {
+    using C = ChunkShape<NB>;
+    if (agn_ring_ctas_per_sm(ctx, attn_chunk_kernel<KV, NB>, C::THREADS, sizeof(ChunkTiles<NB>)) < 1)
+        return agn_fail(ctx, AGN_ECUDA, "attention_kv: the chunk kernel does not fit the device's shared memory");
+    const int64_t rows = d.a.T * (d.a.n_q / d.a.n_kv);
+    agn_launch(ctx, attn_chunk_kernel<KV, NB>, dim3((unsigned)((rows + C::ROWS - 1) / C::ROWS * d.a.n_kv)), dim3(C::THREADS), sizeof(ChunkTiles<NB>), d);
+    AGN_LAUNCHED(ctx, "attention_kv_chunk");
+    return AGN_OK;
+}
+
+template <int KV> int32_t launch_chunk_kv(agn_ctx *ctx, const DecodeArgs &d) {
+    switch (d.a.hd / 32) {
+    case 1: return launch_chunk<KV, 1>(ctx, d);
+    case 2: return launch_chunk<KV, 2>(ctx, d);
+    case 3: return launch_chunk<KV, 3>(ctx, d);
+    case 4: return launch_chunk<KV, 4>(ctx, d);
+    case 5: return launch_chunk<KV, 5>(ctx, d);
+    case 6: return launch_chunk<KV, 6>(ctx, d);
+    case 7: return launch_chunk<KV, 7>(ctx, d);
+    default: return launch_chunk<KV, 8>(ctx, d);
+    }
+}
+
+}  // namespace
+
+int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16) {
+    DecodeArgs d = {};
+    d.a = a;
+    d.act16 = act16;
+    if (kv_dtype == AGN_F16) return launch_chunk_kv<KV_F16>(ctx, d);
+    if (kv_dtype == AGN_Q8_0) return launch_chunk_kv<KV_Q8>(ctx, d);
+    return launch_chunk_kv<KV_WORDS>(ctx, d);
+}

@@ -30,16 +30,6 @@ struct PromptArgs {
     int spin;
 };
 
-// What becomes f16 without turning into infinity or NaN.
-__device__ __forceinline__ bool half_finite(float v) { return (__half_as_ushort(__float2half_rn(v)) & 0x7c00) != 0x7c00; }
-// One value of a cache row (dims of all its heads).
-template <int KV> __device__ __forceinline__ float cache_value(const unsigned char *row, int d) {
-    if (KV == KV_F16) return __half2float(reinterpret_cast<const __half *>(row)[d]);
-    const unsigned char *blk = row + (d >> 5) * KvFormat<KV>::BYTES;
-    const int u = blk[KvFormat<KV>::DATA + (d & 31)];
-    return (float)(KV == KV_Q8 ? (int)(signed char)u : u - 128) * block_scale<KV>(blk);
-}
-
 // One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a
 // row does not see must not meet them in the product.
 template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(PromptArgs p) {
@@ -397,8 +387,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     }
     if (tid == 0 && sm.gave_up) atomicOr(a.flags, AGN_FLAG_TIMEOUT);
 
-    // Rare: V holds values that are not finite.  They were 0 in the product; a row that sees one gets it, two of different signs or a NaN give
-    // NaN.  A thread per output value, slot by slot from the cache.
+    // Rare: V holds values that are not finite.  They were 0 in the product.
     bool any = false;
     for (int j = tid; j < tiles; j += PROMPT_THREADS) any |= p.odd[head * p.tiles + j] != 0;
     if (!__syncthreads_or(any)) return;
@@ -406,23 +395,10 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         const int64_t r = r0 + x / HD;
         const int d = (int)(x % HD), last = a.pos_start + (int)(r / G);
         if (r >= p.rows) break;
-        bool up = false, down = false, nan = false;
-        for (int s = 0; s <= last; s++) {
-            if (!p.odd[head * p.tiles + s / TILE]) {
-                s |= TILE - 1;
-                continue;
-            }
-            const unsigned char *row = a.v_cache + (int64_t)s * a.bytes_per_token;
-            const int at = head * HD + d;
-            const float v = p.kv_dtype == AGN_F16 ? cache_value<KV_F16>(row, at) : p.kv_dtype == AGN_Q8_0 ? cache_value<KV_Q8>(row, at) : cache_value<KV_WORDS>(row, at);
-            if (half_finite(v)) continue;
-            if (v != v) nan = true;
-            else if (v > 0.0f) up = true;
-            else down = true;
-        }
-        if (up || down || nan) {
+        const float bad = odd_value(a, p.kv_dtype, head * HD + d, last, [&](int slot) { return p.odd[head * p.tiles + slot / TILE] != 0; }, TILE);
+        if (bad != 0.0f) {
             __half *o = static_cast<__half *>(a.out) + ((r / G) * a.n_q + head * G + r % G) * HD + d;
-            *o = __float2half_rn(__half2float(*o) + (nan || (up && down) ? NAN : up ? INFINITY : -INFINITY));
+            *o = __float2half_rn(__half2float(*o) + bad);
         }
     }
 }
