@@ -182,6 +182,7 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <int N> struct agn_int { static constexpr int value = N; };
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(agn_smem_u32(dst)), "l"(src) : "memory");
 }
@@ -192,12 +193,44 @@ template <int DK> struct PrepSmem {
     union {
         __half op[4][CH * ROW];  // k hi, k lo, q hi, q lo
         struct {
-            float kk[CH][CH + 1], qk[CH][CH + 1], r[CH][CH + 1], A[CH][CH + 1], N[CH][CH + 1], Y[3][16][17];
+            float kk[CH][CH + 1], qk[CH][CH + 1], A[CH][CH + 1], N[CH][CH + 1];
         } t;
     };
-    float a[CH], beta[CH], c[CH];
+    float a[CH], beta[CH], whole[4], tail[CH];  // products of a over 16 rows, over the rows behind a column up to the end of its 16
     int odd_kq, odd;
 };
+
+// The blocks N_21 of size B below the diagonal blocks of size B: 64 / 2B of them, every thread 2 x 2 (B = 32) or 2 x 1 (B = 16) values.
+template <int B> __device__ __forceinline__ void lower_block(float (&A)[CH][CH + 1], float (&N)[CH][CH + 1], int tid) {
+    constexpr int W = B == 32 ? 2 : 1, TR = B / 2, TC = B / W;  // values across per thread; threads down and across
+    const int blk = tid / (TR * TC), base = blk * 2 * B, row = tid / TC % TR, col = tid % TC;
+    float y[2][W];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < W; j++) y[i][j] = 0.0f;
+#pragma unroll 8
+        for (int l = 0; l < B; l++) {
+            float u[2], w[W];
+#pragma unroll
+            for (int i = 0; i < 2; i++) u[i] = half ? -N[base + B + row + TR * i][base + B + l] : A[base + B + row + TR * i][base + l];
+#pragma unroll
+            for (int j = 0; j < W; j++) w[j] = half ? A[base + B + l][base + col + TC * j] : N[base + l][base + col + TC * j];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < W; j++) y[i][j] = __fmaf_rn(u[i], w[j], y[i][j]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < W; j++) (half ? N : A)[base + B + row + TR * i][base + col + TC * j] = y[i][j];
+        __syncthreads();
+    }
+}
 
 template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare_kernel(ChunkArgs x) {
     agn_pdl_prologue();
@@ -222,30 +255,41 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
     if (tid == 0) sm.odd_kq = 0;
     __syncthreads();
 
-    // q and k, a warp per row
+    // q and k, eight rows per warp, all loads ahead of the first use
     constexpr int V = DK / 32;
-    for (int i = warp; i < CH; i += 8) {
-        float v[2][V], ss[2] = {0.0f, 0.0f};
+    float v[8][2][V];
+#pragma unroll
+    for (int n = 0; n < 8; n++) {
+        const int i = warp * 8 + n;
 #pragma unroll
         for (int w = 0; w < 2; w++) {
             const float *src = w == 0 ? d.k + (first + i) * d.k_stride + hk * DK : d.q + (first + i) * d.q_stride + hk * DK;
 #pragma unroll
             for (int j = 0; j < V / 2; j++) {
                 const float2 y = i < rows ? *reinterpret_cast<const float2 *>(src + 2 * (lane + 32 * j)) : make_float2(0.0f, 0.0f);
-                v[w][2 * j] = y.x;
-                v[w][2 * j + 1] = y.y;
-                ss[w] = __fmaf_rn(y.x, y.x, __fmaf_rn(y.y, y.y, ss[w]));
+                v[n][w][2 * j] = y.x;
+                v[n][w][2 * j + 1] = y.y;
             }
-            ss[w] = agn_warp_sum(ss[w]);
-            const float f = d.eps >= 0.0f ? rsqrtf(ss[w] + d.eps) : 1.0f;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; n++) {
+        const int i = warp * 8 + n;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; j++) ss = __fmaf_rn(v[n][w][j], v[n][w][j], ss);
+            ss = agn_warp_sum(ss);
+            const float f = d.eps >= 0.0f ? rsqrtf(ss + d.eps) : 1.0f;
             // the normalised row's norm is at most 1 unless a sum of squares overflowed or was not a number
-            if (lane == 0 && !(d.eps >= 0.0f ? ss[w] < INFINITY && (ss[w] + d.eps > 0.0f || i >= rows) : ss[w] < 1.01f)) sm.odd_kq = 1;
+            if (lane == 0 && !(d.eps >= 0.0f ? ss < INFINITY && (ss + d.eps > 0.0f || i >= rows) : ss < 1.01f)) sm.odd_kq = 1;
             __half *g = x.kq + (((slot * d.n_k + hk) * 4 + 2 * w) * CH + i) * DK;
+            const float u = i < rows ? f * KQ_UP : 0.0f;
 #pragma unroll
             for (int j = 0; j < V / 2; j++) {
                 uint32_t h2, l2;
-                const float u = i < rows ? f * KQ_UP : 0.0f;
-                split2(v[w][2 * j] * u, v[w][2 * j + 1] * u, h2, l2);
+                split2(v[n][w][2 * j] * u, v[n][w][2 * j + 1] * u, h2, l2);
                 const int at = 2 * (lane + 32 * j);
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w][i * ROW + at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w + 1][i * ROW + at]) = l2;
@@ -307,74 +351,64 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
             if (!(a <= 1.0f) || !(be >= 0.0f && be <= 2.0f)) sm.odd = 1;
         }
         __syncthreads();
+        const int seg = tid >> 6, col = tid & 63;  // 16 rows and a column per thread
         if (tid < CH) {
             float r = 1.0f;
-            for (int i = 0; i < CH; i++) {
-                if (i > tid) r *= sm.a[i];
-                sm.t.r[i][tid] = i >= tid ? r : 0.0f;
-            }
-        } else if (tid == CH) {
-            float c = 1.0f;
-            for (int i = 0; i < CH; i++) sm.c[i] = c *= sm.a[i];
+            for (int i = col + 1; i < (col | 15) + 1; i++) r *= sm.a[i];
+            sm.tail[col] = r;
+            if ((col & 15) == 0) sm.whole[col >> 4] = r * sm.a[col];
         }
         __syncthreads();
         __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * CH;
-        for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
-            const int row = i >> 5, col = 2 * (i & 31);
-            const float r0 = sm.t.r[row][col], r1 = sm.t.r[row][col + 1], be = sm.beta[row];
-            sm.t.A[row][col] = row > col ? be * r0 * sm.t.kk[row][col] : 0.0f;
-            sm.t.A[row][col + 1] = row > col + 1 ? be * r1 * sm.t.kk[row][col + 1] : 0.0f;
-            sm.t.N[row][col] = sm.t.N[row][col + 1] = 0.0f;
-            uint32_t h2, l2;
-            split2(row >= col ? r0 * sm.t.qk[row][col] * NP_UP : 0.0f, row >= col + 1 ? r1 * sm.t.qk[row][col + 1] * NP_UP : 0.0f, h2, l2);
-            *reinterpret_cast<uint32_t *>(np + 2 * CH * CH + row * CH + col) = h2;
-            *reinterpret_cast<uint32_t *>(np + 3 * CH * CH + row * CH + col) = l2;
+        float *decay = x.decay + (slot * d.n_v + hv) * 2 * CH;
+        {
+            // r_ij down the 16 rows, beginning with the product up to the row above them
+            float r = seg > (col >> 4) ? sm.tail[col] : 1.0f;
+            for (int k = (col >> 4) + 1; k < seg; k++) r *= sm.whole[k];
+            float c = 1.0f;  // c_i, by the first column's threads
+            for (int k = 0; k < seg; k++) c *= sm.whole[k];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const int i = 16 * seg + k;
+                const float ai = sm.a[i];
+                if (i > col) r *= ai;
+                sm.t.A[i][col] = i > col ? sm.beta[i] * r * sm.t.kk[i][col] : 0.0f;
+                sm.t.N[i][col] = 0.0f;
+                const float pv = i >= col ? r * sm.t.qk[i][col] * NP_UP : 0.0f;
+                const __half h = __float2half_rn(pv);
+                np[2 * CH * CH + i * CH + col] = h;
+                np[3 * CH * CH + i * CH + col] = __float2half_rn(pv - __half2float(h));
+                if (col == 0) decay[i] = c *= ai;
+                if (i == CH - 1) decay[CH + col] = r;
+            }
         }
         __syncthreads();
         // (I + A)^-1: the four 16 x 16 blocks of the diagonal by substitution, a column per thread
         if (tid < CH) {
-            const int o = tid & ~15, col = tid & 15;
+            const int o = tid & ~15, cc = tid & 15;
             float y[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                float s = i == col ? 1.0f : 0.0f;
+                float s0 = i == cc ? 1.0f : 0.0f, s1 = 0.0f;
 #pragma unroll
-                for (int l = 0; l < 16; l++)
-                    if (l < i) s = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s);
-                y[i] = s;
-                sm.t.N[o + i][o + col] = s;
+                for (int l = 0; l < i; l++) {
+                    if (l & 1) s1 = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s1);
+                    else s0 = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s0);
+                }
+                y[i] = s0 + s1;
+                sm.t.N[o + i][o + cc] = y[i];
             }
         }
         __syncthreads();
-        // the blocks below it, distance by distance: N_ij = -N_ii sum_l A_il N_lj
-        const int br = tid >> 4, bc = tid & 15;
-        for (int dist = 1; dist < 4; dist++) {
-            for (int j = 0; j + dist < 4; j++) {
-                const int i = j + dist;
-                float s = 0.0f;
-                for (int l = 16 * j; l < 16 * i; l++) s = __fmaf_rn(sm.t.A[16 * i + br][l], sm.t.N[l][16 * j + bc], s);
-                sm.t.Y[j][br][bc] = s;
-            }
-            __syncthreads();
-            for (int j = 0; j + dist < 4; j++) {
-                const int i = j + dist;
-                float s = 0.0f;
-#pragma unroll
-                for (int l = 0; l < 16; l++) s = __fmaf_rn(-sm.t.N[16 * i + br][16 * i + l], sm.t.Y[j][l][bc], s);
-                sm.t.N[16 * i + br][16 * j + bc] = s;
-            }
-            __syncthreads();
-        }
+        // then the blocks below it, twice the size each time: N_21 = -N_22 (A_21 N_11).  A_21's place takes the inner product.
+        lower_block<16>(sm.t.A, sm.t.N, tid);
+        lower_block<32>(sm.t.A, sm.t.N, tid);
         for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
             const int row = i >> 5, col = 2 * (i & 31);
             uint32_t h2, l2;
             split2(sm.t.N[row][col] * sm.beta[col] * NP_UP, sm.t.N[row][col + 1] * sm.beta[col + 1] * NP_UP, h2, l2);
             *reinterpret_cast<uint32_t *>(np + row * CH + col) = h2;
             *reinterpret_cast<uint32_t *>(np + CH * CH + row * CH + col) = l2;
-        }
-        if (tid < CH) {
-            x.decay[(slot * d.n_v + hv) * 2 * CH + tid] = sm.c[tid];
-            x.decay[(slot * d.n_v + hv) * 2 * CH + CH + tid] = sm.t.r[CH - 1][tid];
         }
         if (tid == 0) x.odd[slot * d.n_v + hv] = sm.odd | sm.odd_kq;
         __syncthreads();
@@ -478,19 +512,24 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
         }
         if (tid < 32) cp16(sm.decay[c & 1] + tid * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + tid * 4);
     };
-    auto fetched = [] { asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory"); };
+    // Three groups a chunk, each on its way while the ones before are worked on: v, k, q; N; P.
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    auto arrived_but = [](auto pending) { asm volatile("cp.async.wait_group %0;" ::"n"(decltype(pending)::value) : "memory"); };
 
     if (chunks > 0) {
         load_v(0);
         load_kq(0, 0, sm.k[0][0], sm.k[0][1]);
         load_kq(0, 2, sm.q[0], sm.q[1]);
+        commit();
         load_np(0, 0, sm.n[0], sm.n[1]);
+        commit();
         load_np(0, 2, sm.p[0], sm.p[1]);
+        commit();
     }
     for (int64_t c = 0; c < chunks; c++) {
         const int64_t first = b + c * CH;
         const int rows = (int)(e - first < CH ? e - first : CH);
-        fetched();
+        arrived_but(agn_int<2>());
         __syncthreads();
         // ---- the largest magnitude of state and values, as bits: NaN above infinity above the numbers
         uint32_t most = 0;
@@ -507,6 +546,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
         for (int w = 0; w < 8; w++) most = max(most, sm.most[w]);
         const bool more = c + 1 < chunks;
         if (odd || most >= 0x7f800000u) {
+            arrived_but(agn_int<0>());
+            __syncthreads();  // nobody's copies into these buffers are on their way any more
             float *Sf = reinterpret_cast<float *>(sm.q), *tmp = reinterpret_cast<float *>(sm.n);  // q, N are not needed
 #pragma unroll
             for (int n = 0; n < NU; n++)
@@ -523,9 +564,12 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 load_v(c + 1);
                 load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
                 load_kq(c + 1, 2, sm.q[0], sm.q[1]);
-                load_np(c + 1, 0, sm.n[0], sm.n[1]);
-                load_np(c + 1, 2, sm.p[0], sm.p[1]);
             }
+            commit();
+            if (more) load_np(c + 1, 0, sm.n[0], sm.n[1]);
+            commit();
+            if (more) load_np(c + 1, 2, sm.p[0], sm.p[1]);
+            commit();
             continue;
         }
         // up = 2^(5 - exponent): the largest becomes 2^5 .. 2^6, V - c K S at most 2^10, D at most 2^15
@@ -581,12 +625,14 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 qs[n][2 * i] *= cg[i];
                 qs[n][2 * i + 1] *= cg[i];
             }
+        arrived_but(agn_int<1>());  // N
         __syncthreads();
         if (more) {  // q has been read, the other buffers of k and v were last chunk's
             load_v(c + 1);
             load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
             load_kq(c + 1, 2, sm.q[0], sm.q[1]);
         }
+        commit();
 
         // ---- D = N X: a lower triangle, so up to the warp's own rows
         float dd[2][4] = {}, po[2][4] = {};
@@ -619,8 +665,10 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 *reinterpret_cast<uint32_t *>(&sm.dr[0][at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.dr[1][at]) = l2;
             }
+        arrived_but(agn_int<1>());  // P
         __syncthreads();
         if (more) load_np(c + 1, 0, sm.n[0], sm.n[1]);
+        commit();
 
         // ---- S' = c_C S + K^T (r D)
         float up_s[NU][4];
@@ -680,7 +728,9 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 }
         __syncthreads();  // P and D have been read
         if (more) load_np(c + 1, 2, sm.p[0], sm.p[1]);
+        commit();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n)) = make_float2(S[n][0], S[n][1]);
