@@ -154,12 +154,18 @@ template <int DK> __global__ void __launch_bounds__(128) delta_recurrent_kernel(
 constexpr int CH = 64, CHUNK_THREADS = 256;
 constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals
 
+// The workspace holds the operands as they stand in shared memory, rows 16 bytes off a multiple of 128 (so that the eight rows of a fragment do not collide):
+// a chunk's K, Q, N or P is one bulk copy.
+__host__ __device__ constexpr int kq_row(int dk) { return dk + 8; }
+constexpr int NP_ROW = CH + 8;
+
 struct ChunkArgs {
     DeltaArgs d;
-    __half *kq;    // [slots][n_k][k hi, k lo, q hi, q lo][64][head_k], times KQ_UP
-    __half *np;    // [slots][n_v][N hi, N lo, P hi, P lo][64][64], times NP_UP
+    __half *kq;    // [slots][n_k][k hi, k lo, q hi, q lo][64][kq_row], times KQ_UP
+    __half *np;    // [slots][n_v][N hi, N lo, P hi, P lo][64][NP_ROW], times NP_UP
     float *decay;  // [slots][n_v][128]: c_i, then r_Cj
     int *odd;      // [slots][n_v]: the chunk breaks the bounds
+    int spin;
 };
 
 // A sequence's chunks have slots of their own: sequence s from slot b_s / 64 + s on.
@@ -182,14 +188,13 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <int N> struct agn_int { static constexpr int value = N; };
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(agn_smem_u32(dst)), "l"(src) : "memory");
 }
 
 // One CTA per (chunk slot, key head); the value heads of the key head share its two products.
 template <int DK> struct PrepSmem {
-    static constexpr int ROW = DK + 8;  // f16 elements: 16 bytes off a multiple of 128, so that eight rows of a fragment do not collide
+    static constexpr int ROW = kq_row(DK);
     union {
         __half op[4][CH * ROW];  // k hi, k lo, q hi, q lo
         struct {
@@ -284,7 +289,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
             const float f = d.eps >= 0.0f ? rsqrtf(ss + d.eps) : 1.0f;
             // the normalised row's norm is at most 1 unless a sum of squares overflowed or was not a number
             if (lane == 0 && !(d.eps >= 0.0f ? ss < INFINITY && (ss + d.eps > 0.0f || i >= rows) : ss < 1.01f)) sm.odd_kq = 1;
-            __half *g = x.kq + (((slot * d.n_k + hk) * 4 + 2 * w) * CH + i) * DK;
+            __half *g = x.kq + (((slot * d.n_k + hk) * 4 + 2 * w) * CH + i) * ROW;
             const float u = i < rows ? f * KQ_UP : 0.0f;
 #pragma unroll
             for (int j = 0; j < V / 2; j++) {
@@ -294,7 +299,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w][i * ROW + at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w + 1][i * ROW + at]) = l2;
                 *reinterpret_cast<uint32_t *>(g + at) = h2;
-                *reinterpret_cast<uint32_t *>(g + (int64_t)CH * DK + at) = l2;
+                *reinterpret_cast<uint32_t *>(g + CH * ROW + at) = l2;
             }
         }
     }
@@ -359,7 +364,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
             if ((col & 15) == 0) sm.whole[col >> 4] = r * sm.a[col];
         }
         __syncthreads();
-        __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * CH;
+        __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * NP_ROW;
         float *decay = x.decay + (slot * d.n_v + hv) * 2 * CH;
         {
             // r_ij down the 16 rows, beginning with the product up to the row above them
@@ -376,8 +381,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
                 sm.t.N[i][col] = 0.0f;
                 const float pv = i >= col ? r * sm.t.qk[i][col] * NP_UP : 0.0f;
                 const __half h = __float2half_rn(pv);
-                np[2 * CH * CH + i * CH + col] = h;
-                np[3 * CH * CH + i * CH + col] = __float2half_rn(pv - __half2float(h));
+                np[(2 * CH + i) * NP_ROW + col] = h;
+                np[(3 * CH + i) * NP_ROW + col] = __float2half_rn(pv - __half2float(h));
                 if (col == 0) decay[i] = c *= ai;
                 if (i == CH - 1) decay[CH + col] = r;
             }
@@ -407,8 +412,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
             const int row = i >> 5, col = 2 * (i & 31);
             uint32_t h2, l2;
             split2(sm.t.N[row][col] * sm.beta[col] * NP_UP, sm.t.N[row][col + 1] * sm.beta[col + 1] * NP_UP, h2, l2);
-            *reinterpret_cast<uint32_t *>(np + row * CH + col) = h2;
-            *reinterpret_cast<uint32_t *>(np + CH * CH + row * CH + col) = l2;
+            *reinterpret_cast<uint32_t *>(np + row * NP_ROW + col) = h2;
+            *reinterpret_cast<uint32_t *>(np + (CH + row) * NP_ROW + col) = l2;
         }
         if (tid == 0) x.odd[slot * d.n_v + hv] = sm.odd | sm.odd_kq;
         __syncthreads();
@@ -416,11 +421,12 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
 }
 
 template <int DK> struct ChunkSmem {
-    static constexpr int KROW = DK + 8, NROW = CH + 8, SROW = 40, VROW = 40;  // elements; rows whose fragments do not collide
+    static constexpr int KROW = kq_row(DK), NROW = NP_ROW, SROW = 40, VROW = 40;  // elements; rows whose fragments do not collide
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
     __half s[2][DK * SROW], xx[2][CH * SROW], dd[2][CH * SROW], dr[2][CH * SROW];  // B operands: S, V - c K S, D, r D (hi, lo)
     float v[2][CH * VROW], decay[2][2 * CH];
     uint32_t most[8];
+    uint64_t kq_full, n_full, p_full;
 };
 
 // Rows of an odd chunk one by one in f32: the 32 columns of the state are in shared memory as [DK][33] floats.
@@ -487,20 +493,17 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
         S[n][0] = u.x; S[n][1] = u.y; S[n][2] = w.x; S[n][3] = w.y;
     }
 
-    auto load_kq = [&](int64_t c, int w, __half *dst0, __half *dst1) {  // k (w = 0) or q (w = 2) of chunk c, both parts
-        const __half *src = x.kq + ((slot0 + c) * d.n_k + hk) * 4 * CH * DK + (int64_t)w * CH * DK;
-        constexpr int CPR = DK / 8;
-        for (int i = tid; i < 2 * CH * CPR; i += CHUNK_THREADS) {
-            const int part = i / (CH * CPR), row = i / CPR % CH, at = i % CPR * 8;
-            cp16((part ? dst1 : dst0) + row * KROW + at, src + (int64_t)i * 8);
-        }
+    // One thread's bulk copies: K and Q of a chunk, N, P.
+    constexpr uint32_t KQ_BYTES = 2 * CH * KROW * 2, NP_BYTES = 2 * CH * NROW * 2;
+    auto load_kq = [&](int64_t c) {
+        const __half *src = x.kq + ((slot0 + c) * d.n_k + hk) * 4 * CH * KROW;
+        agn_mbar_expect_tx(&sm.kq_full, 2 * KQ_BYTES);
+        agn_bulk_g2s(sm.k[c & 1], src, KQ_BYTES, &sm.kq_full);
+        agn_bulk_g2s(sm.q, src + 2 * CH * KROW, KQ_BYTES, &sm.kq_full);
     };
-    auto load_np = [&](int64_t c, int w, __half *dst0, __half *dst1) {
-        const __half *src = x.np + ((slot0 + c) * d.n_v + hv) * 4 * CH * CH + (int64_t)w * CH * CH;
-        for (int i = tid; i < 2 * CH * 8; i += CHUNK_THREADS) {
-            const int part = i / (CH * 8), row = i / 8 % CH, at = i % 8 * 8;
-            cp16((part ? dst1 : dst0) + row * NROW + at, src + (int64_t)i * 8);
-        }
+    auto load_np = [&](int64_t c, int w, void *dst, uint64_t *bar) {
+        agn_mbar_expect_tx(bar, NP_BYTES);
+        agn_bulk_g2s(dst, x.np + (((slot0 + c) * d.n_v + hv) * 4 + w) * CH * NROW, NP_BYTES, bar);
     };
     auto load_v = [&](int64_t c) {
         const int64_t first = b + c * CH;
@@ -512,25 +515,29 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
         }
         if (tid < 32) cp16(sm.decay[c & 1] + tid * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + tid * 4);
     };
-    // Three groups a chunk, each on its way while the ones before are worked on: v, k, q; N; P.
-    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    auto arrived_but = [](auto pending) { asm volatile("cp.async.wait_group %0;" ::"n"(decltype(pending)::value) : "memory"); };
-
+    if (tid == 0) {
+        agn_mbar_init(&sm.kq_full, 1);
+        agn_mbar_init(&sm.n_full, 1);
+        agn_mbar_init(&sm.p_full, 1);
+        agn_mbar_init_fence();
+    }
+    __syncthreads();
     if (chunks > 0) {
         load_v(0);
-        load_kq(0, 0, sm.k[0][0], sm.k[0][1]);
-        load_kq(0, 2, sm.q[0], sm.q[1]);
-        commit();
-        load_np(0, 0, sm.n[0], sm.n[1]);
-        commit();
-        load_np(0, 2, sm.p[0], sm.p[1]);
-        commit();
+        if (tid == 0) {
+            load_kq(0);
+            load_np(0, 0, sm.n, &sm.n_full);
+            load_np(0, 2, sm.p, &sm.p_full);
+        }
     }
+    int odd = chunks > 0 ? x.odd[slot0 * d.n_v + hv] : 0;
+    bool gave_up = false;  // a copy's wait ran out, for all threads alike
     for (int64_t c = 0; c < chunks; c++) {
         const int64_t first = b + c * CH;
         const int rows = (int)(e - first < CH ? e - first : CH);
-        arrived_but(agn_int<2>());
-        __syncthreads();
+        const uint32_t turn = c & 1;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.kq_full, turn, x.spin)))) break;
         // ---- the largest magnitude of state and values, as bits: NaN above infinity above the numbers
         uint32_t most = 0;
         const float *v = sm.v[c & 1];
@@ -541,13 +548,13 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
             for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(S[n][i]) & 0x7fffffffu);
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) sm.most[warp] = most;
-        const int odd = x.odd[(slot0 + c) * d.n_v + hv];
+        const int odd_next = c + 1 < chunks ? x.odd[(slot0 + c + 1) * d.n_v + hv] : 0;
         __syncthreads();
         for (int w = 0; w < 8; w++) most = max(most, sm.most[w]);
         const bool more = c + 1 < chunks;
         if (odd || most >= 0x7f800000u) {
-            arrived_but(agn_int<0>());
-            __syncthreads();  // nobody's copies into these buffers are on their way any more
+            // nobody's copies into these buffers may be on their way any more
+            if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.n_full, turn, x.spin) || !agn_mbar_wait(&sm.p_full, turn, x.spin)))) break;
             float *Sf = reinterpret_cast<float *>(sm.q), *tmp = reinterpret_cast<float *>(sm.n);  // q, N are not needed
 #pragma unroll
             for (int n = 0; n < NU; n++)
@@ -560,18 +567,20 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[n][i] = Sf[(16 * mt + g + (i >> 1) * 8) * 33 + 8 * (n0 + n) + 2 * t4 + (i & 1)];
             __syncthreads();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // these writes come before the next copies' ones
+            __syncthreads();
             if (more) {
                 load_v(c + 1);
-                load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
-                load_kq(c + 1, 2, sm.q[0], sm.q[1]);
+                if (tid == 0) {
+                    load_kq(c + 1);
+                    load_np(c + 1, 0, sm.n, &sm.n_full);
+                    load_np(c + 1, 2, sm.p, &sm.p_full);
+                }
             }
-            commit();
-            if (more) load_np(c + 1, 0, sm.n[0], sm.n[1]);
-            commit();
-            if (more) load_np(c + 1, 2, sm.p[0], sm.p[1]);
-            commit();
+            odd = odd_next;
             continue;
         }
+        odd = odd_next;
         // up = 2^(5 - exponent): the largest becomes 2^5 .. 2^6, V - c K S at most 2^10, D at most 2^15
         const int ex = max((int)(most >> 23), 24);
         const float up = __uint_as_float((uint32_t)(259 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 5) << 23);
@@ -625,30 +634,36 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 qs[n][2 * i] *= cg[i];
                 qs[n][2 * i + 1] *= cg[i];
             }
-        arrived_but(agn_int<1>());  // N
-        __syncthreads();
+        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.n_full, turn, x.spin)))) break;
         if (more) {  // q has been read, the other buffers of k and v were last chunk's
+            if (tid == 0) load_kq(c + 1);
             load_v(c + 1);
-            load_kq(c + 1, 0, sm.k[(c + 1) & 1][0], sm.k[(c + 1) & 1][1]);
-            load_kq(c + 1, 2, sm.q[0], sm.q[1]);
         }
-        commit();
 
         // ---- D = N X: a lower triangle, so up to the warp's own rows
         float dd[2][4] = {}, po[2][4] = {};
-        for (int kk = 0; kk <= wm; kk++) {
-            uint32_t a0[4], a1[4], bh[4], bl[4];
-            const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
-            ldsm4(a0, sm.n[0] + arow);
-            ldsm4(a1, sm.n[1] + arow);
-            ldsm4t(bh, sm.xx[0] + brow);
-            ldsm4t(bl, sm.xx[1] + brow);
+        {
+            float t1[2][4] = {}, t2[2][4] = {};  // the three products apart: short chains
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                mma16(dd[n], a0, bh[2 * n], bh[2 * n + 1]);
-                mma16(dd[n], a0, bl[2 * n], bl[2 * n + 1]);
-                mma16(dd[n], a1, bh[2 * n], bh[2 * n + 1]);
+            for (int kk = 0; kk < CH / 16; kk++) {
+                if (kk > wm) break;
+                uint32_t a0[4], a1[4], bh[4], bl[4];
+                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
+                ldsm4(a0, sm.n[0] + arow);
+                ldsm4(a1, sm.n[1] + arow);
+                ldsm4t(bh, sm.xx[0] + brow);
+                ldsm4t(bl, sm.xx[1] + brow);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    mma16(dd[n], a0, bh[2 * n], bh[2 * n + 1]);
+                    mma16(t1[n], a0, bl[2 * n], bl[2 * n + 1]);
+                    mma16(t2[n], a1, bh[2 * n], bh[2 * n + 1]);
+                }
             }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) dd[n][i] += t1[n][i] + t2[n][i];
         }
         const float rc[2] = {dec[CH + r0], dec[CH + r0 + 8]};
 #pragma unroll
@@ -665,10 +680,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 *reinterpret_cast<uint32_t *>(&sm.dr[0][at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.dr[1][at]) = l2;
             }
-        arrived_but(agn_int<1>());  // P
-        __syncthreads();
-        if (more) load_np(c + 1, 0, sm.n[0], sm.n[1]);
-        commit();
+        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.p_full, turn, x.spin)))) break;
+        if (more && tid == 0) load_np(c + 1, 0, sm.n, &sm.n_full);
 
         // ---- S' = c_C S + K^T (r D)
         float up_s[NU][4];
@@ -701,19 +714,28 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
             for (int i = 0; i < 4; i++) S[n][i] = __fmaf_rn(up_s[n][i], f, cc * S[n][i]);
 
         // ---- O = c Q S + P D
-        for (int kk = 0; kk <= wm; kk++) {
-            uint32_t a0[4], a1[4], bh[4], bl[4];
-            const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
-            ldsm4(a0, sm.p[0] + arow);
-            ldsm4(a1, sm.p[1] + arow);
-            ldsm4t(bh, sm.dd[0] + brow);
-            ldsm4t(bl, sm.dd[1] + brow);
+        {
+            float t1[2][4] = {}, t2[2][4] = {};  // the three products apart: short chains
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                mma16(po[n], a0, bh[2 * n], bh[2 * n + 1]);
-                mma16(po[n], a0, bl[2 * n], bl[2 * n + 1]);
-                mma16(po[n], a1, bh[2 * n], bh[2 * n + 1]);
+            for (int kk = 0; kk < CH / 16; kk++) {
+                if (kk > wm) break;
+                uint32_t a0[4], a1[4], bh[4], bl[4];
+                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
+                ldsm4(a0, sm.p[0] + arow);
+                ldsm4(a1, sm.p[1] + arow);
+                ldsm4t(bh, sm.dd[0] + brow);
+                ldsm4t(bl, sm.dd[1] + brow);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    mma16(po[n], a0, bh[2 * n], bh[2 * n + 1]);
+                    mma16(t1[n], a0, bl[2 * n], bl[2 * n + 1]);
+                    mma16(t2[n], a1, bh[2 * n], bh[2 * n + 1]);
+                }
             }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) po[n][i] += t1[n][i] + t2[n][i];
         }
         const float fo = d.scale * down;
 #pragma unroll
@@ -727,10 +749,21 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                     *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) = y;
                 }
         __syncthreads();  // P and D have been read
-        if (more) load_np(c + 1, 2, sm.p[0], sm.p[1]);
-        commit();
+        if (more && tid == 0) load_np(c + 1, 2, sm.p, &sm.p_full);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (gave_up) {  // no copy may be in flight when the CTA ends; each barrier's last phase is awaited once more
+        if (tid == 0) {
+            atomicOr(d.flags, AGN_FLAG_TIMEOUT);
+            for (uint32_t p = 0; p < 2; p++) {
+                (void)agn_mbar_wait(&sm.kq_full, p, x.spin);
+                (void)agn_mbar_wait(&sm.n_full, p, x.spin);
+                (void)agn_mbar_wait(&sm.p_full, p, x.spin);
+            }
+        }
+        __syncthreads();
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n)) = make_float2(S[n][0], S[n][1]);
@@ -749,8 +782,8 @@ ChunkLayout chunk_layout(int64_t T, int64_t n_seqs, int n_k, int n_v, int dk) {
     ChunkLayout l;
     l.slots = T / CH + n_seqs;
     l.kq = 0;
-    l.np = l.kq + l.slots * n_k * 4 * CH * dk * 2;
-    l.decay = l.np + l.slots * n_v * 4 * CH * CH * 2;
+    l.np = l.kq + l.slots * n_k * 4 * CH * kq_row(dk) * 2;
+    l.decay = l.np + l.slots * n_v * 4 * CH * NP_ROW * 2;
     l.odd = l.decay + l.slots * n_v * 2 * CH * 4;
     l.bytes = (l.odd + l.slots * n_v * 4 + 15) / 16 * 16;
     return l;
@@ -765,9 +798,11 @@ template <int DK> int32_t launch_chunked(agn_ctx *ctx, const DeltaArgs &d, void 
     x.np = reinterpret_cast<__half *>(w + l.np);
     x.decay = reinterpret_cast<float *>(w + l.decay);
     x.odd = reinterpret_cast<int *>(w + l.odd);
+    x.spin = ctx->mbar_spin_limit;
     if (agn_ring_ctas_per_sm(ctx, delta_prepare_kernel<DK>, CHUNK_THREADS, sizeof(PrepSmem<DK>)) < 1 ||
         agn_ring_ctas_per_sm(ctx, delta_chunk_kernel<DK>, CHUNK_THREADS, sizeof(ChunkSmem<DK>)) < 1)
         return agn_fail(ctx, AGN_ECUDA, "gated_delta_rule: the chunk kernels do not fit the device's shared memory");
+    ctx->flags_dirty = true;
     agn_launch(ctx, delta_prepare_kernel<DK>, dim3((unsigned)l.slots, (unsigned)d.n_k), dim3(CHUNK_THREADS), sizeof(PrepSmem<DK>), x);
     AGN_LAUNCHED(ctx, "gated_delta_chunk");
     agn_launch(ctx, delta_chunk_kernel<DK>, dim3((unsigned)(d.dv / 32), (unsigned)d.n_v, (unsigned)n_seqs), dim3(CHUNK_THREADS), sizeof(ChunkSmem<DK>), x);
