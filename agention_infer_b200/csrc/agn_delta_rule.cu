@@ -151,7 +151,7 @@ template <int DK> __global__ void __launch_bounds__(128) delta_recurrent_kernel(
 // entries of N and P have known bounds; states and values are scaled by a power of two taken from their largest magnitude in front of
 // every chunk.  Those bounds hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that breaks them is
 // computed row by row in f32 instead.
-constexpr int CH = 64, CHUNK_THREADS = 256;
+constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 32;
 constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals
 
 // The workspace holds the operands as they stand in shared memory, rows 16 bytes off a multiple of 128 (so that the eight rows of a fragment do not collide):
@@ -425,9 +425,20 @@ template <int DK> struct ChunkSmem {
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
     __half s[2][DK * SROW], xx[2][CH * SROW], dd[2][CH * SROW], dr[2][CH * SROW];  // B operands: S, V - c K S, D, r D (hi, lo)
     float v[2][CH * VROW], decay[2][2 * CH];
-    uint32_t most[8];
-    uint64_t kq_full, n_full, p_full;
+    uint32_t most[9];
+    uint64_t kq_full, v_full, n_full, p_full, kq_free, n_free, p_free;
+    int gave_up;
 };
+
+// Warps 0-7 work, warp 8 fetches.  The workers' own barrier (1) never waits for the fetching warp; the two sides tell each other through mbarriers: *_full, the data
+// of a chunk is there; *_free, its place may be filled again.
+__device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool workers_sync_or(bool x) {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 1, 256, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((uint32_t)x) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(agn_smem_u32(bar)) : "memory"); }
 
 // Rows of an odd chunk one by one in f32: the 32 columns of the state are in shared memory as [DK][33] floats.
 template <int DK> __device__ __noinline__ void delta_rows_by_one(const DeltaArgs &d, float *S, float *tmp, int64_t first, int rows, int hk, int hv, int c0) {
@@ -451,7 +462,7 @@ template <int DK> __device__ __noinline__ void delta_rows_by_one(const DeltaArgs
         }
         tmp[part * 64 + col] = dk;
         tmp[part * 64 + 32 + col] = dq;
-        __syncthreads();
+        workers_sync();
         dk = dq = 0.0f;
         for (int w = 0; w < 8; w++) {
             dk += tmp[w * 64 + col];
@@ -461,11 +472,11 @@ template <int DK> __device__ __noinline__ void delta_rows_by_one(const DeltaArgs
         const float dl = be * __fmaf_rn(-al, dk, d.v[t * d.v_stride + hv * d.dv + c0 + col]);
         if (part == 0) d.out[(t * d.n_v + hv) * d.dv + c0 + col] = __fmaf_rn(qk, dl, al * dq);
         for (int j = part * PER; j < (part + 1) * PER; j++) S[j * 33 + col] = __fmaf_rn(kr[j] * fk, dl, al * S[j * 33 + col]);
-        __syncthreads();
+        workers_sync();
     }
 }
 
-template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_kernel(ChunkArgs x) {
+template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_kernel(const __grid_constant__ ChunkArgs x) {
     agn_pdl_prologue();
     extern __shared__ __align__(128) unsigned char raw[];
     using SM = ChunkSmem<DK>;
@@ -479,14 +490,15 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
     int64_t b, e;
     delta_rows(d, s, &b, &e);
     const int64_t slot0 = delta_slot(b, s), chunks = (e - b + CH - 1) / CH;
-    const int mt = warp % MT, n0 = warp / MT * NU;  // this warp's tiles of the state: rows 16 mt .., columns 8 (n0 + n) ..
+    const bool fetches = warp == 8;
+    const int mt = warp % MT, n0 = (warp & 7) / MT * NU;  // this warp's tiles of the state: rows 16 mt .., columns 8 (n0 + n) ..
 
     float S[NU][4];
     const int64_t soff = ((s * d.n_v + hv) * DK + 16 * mt + g) * d.dv + c0 + 2 * t4;
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         float2 u = make_float2(0.0f, 0.0f), w = u;
-        if (d.state_in) {
+        if (d.state_in && !fetches) {
             u = *reinterpret_cast<const float2 *>(d.state_in + soff + 8 * (n0 + n));
             w = *reinterpret_cast<const float2 *>(d.state_in + soff + 8 * (n0 + n) + (int64_t)8 * d.dv);
         }
@@ -505,78 +517,128 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
         agn_mbar_expect_tx(bar, NP_BYTES);
         agn_bulk_g2s(dst, x.np + (((slot0 + c) * d.n_v + hv) * 4 + w) * CH * NROW, NP_BYTES, bar);
     };
-    auto load_v = [&](int64_t c) {
+    auto load_v = [&](int64_t c) {  // by the fetching warp
         const int64_t first = b + c * CH;
         float *dst = sm.v[c & 1];
-        for (int i = tid; i < CH * 8; i += CHUNK_THREADS) {
-            const int row = i >> 3, at = (i & 7) * 4;
-            if (first + row < e) cp16(dst + row * VROW + at, d.v + (first + row) * d.v_stride + (int64_t)hv * d.dv + c0 + at);
+        const float *src = d.v + first * d.v_stride + (int64_t)hv * d.dv + c0;
+#pragma unroll
+        for (int i = 0; i < CH * 8 / 32; i++) {
+            const int row = (lane >> 3) + 4 * i, at = (lane & 7) * 4;
+            if (first + row < e) cp16(dst + row * VROW + at, src + row * d.v_stride + at);
             else *reinterpret_cast<float4 *>(dst + row * VROW + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        if (tid < 32) cp16(sm.decay[c & 1] + tid * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + tid * 4);
+        cp16(sm.decay[c & 1] + lane * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + lane * 4);
+    };
+    auto tell_largest = [&](uint32_t most) {  // magnitudes as bits: NaN above infinity above the numbers
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) sm.most[warp] = most;
+    };
+    // a bounded wait; once one has run out the CTA's other waits give up after their next poll
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        for (int left = x.spin; left > 0; left -= 1024) {
+            if (agn_mbar_wait(bar, parity, left < 1024 ? left : 1024)) return true;
+            if (*(volatile int *)&sm.gave_up) return false;
+        }
+        *(volatile int *)&sm.gave_up = 1;
+        return false;
     };
     if (tid == 0) {
         agn_mbar_init(&sm.kq_full, 1);
+        agn_mbar_init(&sm.v_full, 1);
         agn_mbar_init(&sm.n_full, 1);
         agn_mbar_init(&sm.p_full, 1);
+        agn_mbar_init(&sm.kq_free, 8);
+        agn_mbar_init(&sm.n_free, 8);
+        agn_mbar_init(&sm.p_free, 8);
         agn_mbar_init_fence();
+        sm.gave_up = 0;
     }
     __syncthreads();
-    if (chunks > 0) {
-        load_v(0);
-        if (tid == 0) {
-            load_kq(0);
-            load_np(0, 0, sm.n, &sm.n_full);
-            load_np(0, 2, sm.p, &sm.p_full);
+
+    if (fetches) {
+        int64_t kq_issued = 0, n_issued = 0, p_issued = 0;
+        for (int64_t c = 0; c < chunks; c++) {
+            const uint32_t before = (c - 1) & 1;  // the turn in which these places were last used
+            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.kq_free, before))) break;
+            if (lane == 0) load_kq(c);
+            kq_issued++;
+            __syncwarp();
+            load_v(c);
+            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.n_free, before))) break;
+            if (lane == 0) load_np(c, 0, sm.n, &sm.n_full);
+            n_issued++;
+            __syncwarp();
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            const float *v = sm.v[c & 1];
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < CH * 8 / 32; i++) {
+                const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
+                most = max(most, max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
+                                     max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu)));
+            }
+            tell_largest(most);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.v_full);
+            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.p_free, before))) break;
+            if (lane == 0) load_np(c, 2, sm.p, &sm.p_full);
+            p_issued++;
+            __syncwarp();
         }
-    }
-    int odd = chunks > 0 ? x.odd[slot0 * d.n_v + hv] : 0;
-    bool gave_up = false;  // a copy's wait ran out, for all threads alike
-    for (int64_t c = 0; c < chunks; c++) {
-        const int64_t first = b + c * CH;
-        const int rows = (int)(e - first < CH ? e - first : CH);
-        const uint32_t turn = c & 1;
+        // no copy may be in flight when the CTA ends
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.kq_full, turn, x.spin)))) break;
-        // ---- the largest magnitude of state and values, as bits: NaN above infinity above the numbers
+        if (kq_issued) (void)agn_mbar_wait(&sm.kq_full, (kq_issued - 1) & 1, x.spin);
+        if (n_issued) (void)agn_mbar_wait(&sm.n_full, (n_issued - 1) & 1, x.spin);
+        if (p_issued) (void)agn_mbar_wait(&sm.p_full, (p_issued - 1) & 1, x.spin);
+        if (lane == 0 && sm.gave_up) atomicOr(d.flags, AGN_FLAG_TIMEOUT);
+        return;
+    }
+
+    int odd = chunks > 0 ? x.odd[slot0 * d.n_v + hv] : 0;
+    bool gave_up = false;  // a wait ran out, for all workers alike
+    auto freed = [&](uint64_t *bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    auto tell_state = [&] {
         uint32_t most = 0;
-        const float *v = sm.v[c & 1];
-        for (int i = tid; i < CH * 32; i += CHUNK_THREADS) most = max(most, __float_as_uint(v[(i >> 5) * VROW + (i & 31)]) & 0x7fffffffu);
 #pragma unroll
         for (int n = 0; n < NU; n++)
 #pragma unroll
             for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(S[n][i]) & 0x7fffffffu);
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 0) sm.most[warp] = most;
+        tell_largest(most);
+    };
+    tell_state();
+    for (int64_t c = 0; c < chunks; c++) {
+        const int64_t first = b + c * CH;
+        const int rows = (int)(e - first < CH ? e - first : CH);
+        const uint32_t turn = c & 1;
+        if ((gave_up = workers_sync_or(!(wait(&sm.kq_full, turn) && wait(&sm.v_full, turn))))) break;
+        uint32_t most = 0;
+#pragma unroll
+        for (int w = 0; w < 9; w++) most = max(most, sm.most[w]);
         const int odd_next = c + 1 < chunks ? x.odd[(slot0 + c + 1) * d.n_v + hv] : 0;
-        __syncthreads();
-        for (int w = 0; w < 8; w++) most = max(most, sm.most[w]);
-        const bool more = c + 1 < chunks;
+        const float *v = sm.v[c & 1];
         if (odd || most >= 0x7f800000u) {
             // nobody's copies into these buffers may be on their way any more
-            if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.n_full, turn, x.spin) || !agn_mbar_wait(&sm.p_full, turn, x.spin)))) break;
+            if ((gave_up = workers_sync_or(!(wait(&sm.n_full, turn) && wait(&sm.p_full, turn))))) break;
             float *Sf = reinterpret_cast<float *>(sm.q), *tmp = reinterpret_cast<float *>(sm.n);  // q, N are not needed
 #pragma unroll
             for (int n = 0; n < NU; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) Sf[(16 * mt + g + (i >> 1) * 8) * 33 + 8 * (n0 + n) + 2 * t4 + (i & 1)] = S[n][i];
-            __syncthreads();
+            workers_sync();
             delta_rows_by_one<DK>(d, Sf, tmp, first, rows, hk, hv, c0);
 #pragma unroll
             for (int n = 0; n < NU; n++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) S[n][i] = Sf[(16 * mt + g + (i >> 1) * 8) * 33 + 8 * (n0 + n) + 2 * t4 + (i & 1)];
-            __syncthreads();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // these writes come before the next copies' ones
-            __syncthreads();
-            if (more) {
-                load_v(c + 1);
-                if (tid == 0) {
-                    load_kq(c + 1);
-                    load_np(c + 1, 0, sm.n, &sm.n_full);
-                    load_np(c + 1, 2, sm.p, &sm.p_full);
-                }
-            }
+            freed(&sm.kq_free);
+            freed(&sm.n_free);
+            freed(&sm.p_free);
+            workers_sync();  // the maxima have been read
+            tell_state();
             odd = odd_next;
             continue;
         }
@@ -594,7 +656,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 *reinterpret_cast<uint32_t *>(&sm.s[0][at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.s[1][at]) = l2;
             }
-        __syncthreads();
+        workers_sync();
 
         // ---- K S and Q S: 16 rows and 16 columns per warp
         const int wm = warp & 3, wn = (warp >> 2) * 16;
@@ -634,11 +696,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 qs[n][2 * i] *= cg[i];
                 qs[n][2 * i + 1] *= cg[i];
             }
-        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.n_full, turn, x.spin)))) break;
-        if (more) {  // q has been read, the other buffers of k and v were last chunk's
-            if (tid == 0) load_kq(c + 1);
-            load_v(c + 1);
-        }
+        freed(&sm.kq_free);  // q has been read; the other buffers of k and v were last chunk's
+        if ((gave_up = workers_sync_or(!wait(&sm.n_full, turn)))) break;
 
         // ---- D = N X: a lower triangle, so up to the warp's own rows
         float dd[2][4] = {}, po[2][4] = {};
@@ -680,8 +739,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                 *reinterpret_cast<uint32_t *>(&sm.dr[0][at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.dr[1][at]) = l2;
             }
-        if ((gave_up = __syncthreads_or(!agn_mbar_wait(&sm.p_full, turn, x.spin)))) break;
-        if (more && tid == 0) load_np(c + 1, 0, sm.n, &sm.n_full);
+        freed(&sm.n_free);
+        if ((gave_up = workers_sync_or(!wait(&sm.p_full, turn)))) break;
 
         // ---- S' = c_C S + K^T (r D)
         float up_s[NU][4];
@@ -748,22 +807,10 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_chunk_k
                     y.y = __fmaf_rn(po[n][2 * i + 1], 1.0f / NP_UP, qs[n][2 * i + 1]) * fo;
                     *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) = y;
                 }
-        __syncthreads();  // P and D have been read
-        if (more && tid == 0) load_np(c + 1, 2, sm.p, &sm.p_full);
+        freed(&sm.p_free);
+        tell_state();
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (gave_up) {  // no copy may be in flight when the CTA ends; each barrier's last phase is awaited once more
-        if (tid == 0) {
-            atomicOr(d.flags, AGN_FLAG_TIMEOUT);
-            for (uint32_t p = 0; p < 2; p++) {
-                (void)agn_mbar_wait(&sm.kq_full, p, x.spin);
-                (void)agn_mbar_wait(&sm.n_full, p, x.spin);
-                (void)agn_mbar_wait(&sm.p_full, p, x.spin);
-            }
-        }
-        __syncthreads();
-        return;
-    }
+    if (gave_up) return;  // reported by the fetching warp, whose waits end as well
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n)) = make_float2(S[n][0], S[n][1]);
@@ -800,12 +847,12 @@ template <int DK> int32_t launch_chunked(agn_ctx *ctx, const DeltaArgs &d, void 
     x.odd = reinterpret_cast<int *>(w + l.odd);
     x.spin = ctx->mbar_spin_limit;
     if (agn_ring_ctas_per_sm(ctx, delta_prepare_kernel<DK>, CHUNK_THREADS, sizeof(PrepSmem<DK>)) < 1 ||
-        agn_ring_ctas_per_sm(ctx, delta_chunk_kernel<DK>, CHUNK_THREADS, sizeof(ChunkSmem<DK>)) < 1)
+        agn_ring_ctas_per_sm(ctx, delta_chunk_kernel<DK>, CARRY_THREADS, sizeof(ChunkSmem<DK>)) < 1)
         return agn_fail(ctx, AGN_ECUDA, "gated_delta_rule: the chunk kernels do not fit the device's shared memory");
     ctx->flags_dirty = true;
     agn_launch(ctx, delta_prepare_kernel<DK>, dim3((unsigned)l.slots, (unsigned)d.n_k), dim3(CHUNK_THREADS), sizeof(PrepSmem<DK>), x);
     AGN_LAUNCHED(ctx, "gated_delta_chunk");
-    agn_launch(ctx, delta_chunk_kernel<DK>, dim3((unsigned)(d.dv / 32), (unsigned)d.n_v, (unsigned)n_seqs), dim3(CHUNK_THREADS), sizeof(ChunkSmem<DK>), x);
+    agn_launch(ctx, delta_chunk_kernel<DK>, dim3((unsigned)(d.dv / 32), (unsigned)d.n_v, (unsigned)n_seqs), dim3(CARRY_THREADS), sizeof(ChunkSmem<DK>), x);
     AGN_LAUNCHED(ctx, "gated_delta_chunk");
     return AGN_OK;
 }
