@@ -151,7 +151,7 @@ template <int DK> __global__ void __launch_bounds__(128) delta_recurrent_kernel(
 // entries of N and P have known bounds; states and values are scaled by a power of two taken from their largest magnitude in front of
 // every chunk.  Those bounds hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that breaks them is
 // computed row by row in f32 instead.
-constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 32;
+constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 128;
 constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals
 
 // The workspace holds the operands as they stand in shared memory, rows 16 bytes off a multiple of 128 (so that the eight rows of a fragment do not collide):
@@ -193,51 +193,51 @@ __device__ __forceinline__ void cp16(void *dst, const void *src) {
 }
 
 // One CTA per (chunk slot, key head); the value heads of the key head share its two products.
+constexpr int TROW = CH + 4;  // floats: four of them at a multiple of 16 bytes
 template <int DK> struct PrepSmem {
     static constexpr int ROW = kq_row(DK);
     union {
         __half op[4][CH * ROW];  // k hi, k lo, q hi, q lo
         struct {
-            float kk[CH][CH + 1], qk[CH][CH + 1], A[CH][CH + 1], N[CH][CH + 1];
+            float kk[CH][TROW], qk[CH][TROW], A[CH][TROW], N[CH][TROW];
         } t;
     };
-    float a[CH], beta[CH], whole[4], tail[CH];  // products of a over 16 rows, over the rows behind a column up to the end of its 16
+    float a[CH], beta[CH], whole[8], tail[CH];  // products of a over eight rows, over the rows behind a column up to the end of its eight
     int odd_kq, odd;
 };
 
-// The blocks N_21 of size B below the diagonal blocks of size B: 64 / 2B of them, every thread 2 x 2 (B = 32) or 2 x 1 (B = 16) values.
-template <int B> __device__ __forceinline__ void lower_block(float (&A)[CH][CH + 1], float (&N)[CH][CH + 1], int tid) {
-    constexpr int W = B == 32 ? 2 : 1, TR = B / 2, TC = B / W;  // values across per thread; threads down and across
-    const int blk = tid / (TR * TC), base = blk * 2 * B, row = tid / TC % TR, col = tid % TC;
-    float y[2][W];
+// The blocks N_21 = -N_22 (A_21 N_11) of size B below the diagonal blocks of size B, four values side by side per thread; A_21's place takes the inner product.
+template <int B> __device__ __forceinline__ void lower_block(float (&A)[CH][TROW], float (&N)[CH][TROW], int tid) {
+    constexpr int TPB = B * B / 4;  // threads of a block
+    const int base = tid / TPB * 2 * B, row = tid % TPB / (B / 4), col = tid % (B / 4) * 4;
+    const bool on = tid < CH / (2 * B) * TPB;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (on) {
+            const float *u = half ? &N[base + B + row][base + B] : &A[base + B + row][base];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int l = 0; l < B; l += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(u + l);
+                const float fs[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-            for (int j = 0; j < W; j++) y[i][j] = 0.0f;
-#pragma unroll 8
-        for (int l = 0; l < B; l++) {
-            float u[2], w[W];
-#pragma unroll
-            for (int i = 0; i < 2; i++) u[i] = half ? -N[base + B + row + TR * i][base + B + l] : A[base + B + row + TR * i][base + l];
-#pragma unroll
-            for (int j = 0; j < W; j++) w[j] = half ? A[base + B + l][base + col + TC * j] : N[base + l][base + col + TC * j];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < W; j++) y[i][j] = __fmaf_rn(u[i], w[j], y[i][j]);
+                for (int k = 0; k < 4; k++) {
+                    const float4 w = *reinterpret_cast<const float4 *>(half ? &A[base + B + l + k][base + col] : &N[base + l + k][base + col]);
+                    y.x = __fmaf_rn(fs[k], w.x, y.x); y.y = __fmaf_rn(fs[k], w.y, y.y);
+                    y.z = __fmaf_rn(fs[k], w.z, y.z); y.w = __fmaf_rn(fs[k], w.w, y.w);
+                }
+            }
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < W; j++) (half ? N : A)[base + B + row + TR * i][base + col + TC * j] = y[i][j];
+        if (on) {
+            if (half) *reinterpret_cast<float4 *>(&N[base + B + row][base + col]) = make_float4(-y.x, -y.y, -y.z, -y.w);
+            else *reinterpret_cast<float4 *>(&A[base + B + row][base + col]) = y;
+        }
         __syncthreads();
     }
 }
 
-template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare_kernel(ChunkArgs x) {
+template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prepare_kernel(const __grid_constant__ ChunkArgs x) {
     agn_pdl_prologue();
     extern __shared__ __align__(128) unsigned char raw[];
     PrepSmem<DK> &sm = *reinterpret_cast<PrepSmem<DK> *>(raw);
@@ -333,7 +333,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
     }
     __syncthreads();  // the operands are done with: the tables take their place
     {
-        float(*to)[CH + 1] = which ? sm.t.qk : sm.t.kk;
+        float(*to)[TROW] = which ? sm.t.qk : sm.t.kk;
         constexpr float DOWN = 1.0f / (KQ_UP * KQ_UP);
 #pragma unroll
         for (int n = 0; n < 8; n++) {
@@ -356,56 +356,59 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS) delta_prepare
             if (!(a <= 1.0f) || !(be >= 0.0f && be <= 2.0f)) sm.odd = 1;
         }
         __syncthreads();
-        const int seg = tid >> 6, col = tid & 63;  // 16 rows and a column per thread
+        const int seg = tid >> 5, col = 2 * (tid & 31), own = col >> 3;  // eight rows and two columns per thread
         if (tid < CH) {
             float r = 1.0f;
-            for (int i = col + 1; i < (col | 15) + 1; i++) r *= sm.a[i];
-            sm.tail[col] = r;
-            if ((col & 15) == 0) sm.whole[col >> 4] = r * sm.a[col];
+            for (int i = tid + 1; i < (tid | 7) + 1; i++) r *= sm.a[i];
+            sm.tail[tid] = r;
+            if ((tid & 7) == 0) sm.whole[tid >> 3] = r * sm.a[tid];
         }
         __syncthreads();
         __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * NP_ROW;
         float *decay = x.decay + (slot * d.n_v + hv) * 2 * CH;
         {
-            // r_ij down the 16 rows, beginning with the product up to the row above them
-            float r = seg > (col >> 4) ? sm.tail[col] : 1.0f;
-            for (int k = (col >> 4) + 1; k < seg; k++) r *= sm.whole[k];
-            float c = 1.0f;  // c_i, by the first column's threads
-            for (int k = 0; k < seg; k++) c *= sm.whole[k];
+            // r_ij down the eight rows, beginning with the product up to the row above them
+            float r[2] = {1.0f, 1.0f}, between = 1.0f, c = 1.0f;
+            for (int k = own + 1; k < seg; k++) between *= sm.whole[k];
+            if (seg > own) {
+                r[0] = sm.tail[col] * between;
+                r[1] = sm.tail[col + 1] * between;
+            }
+            for (int k = 0; k < seg; k++) c *= sm.whole[k];  // c_i, by the first columns' threads
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const int i = 16 * seg + k;
-                const float ai = sm.a[i];
-                if (i > col) r *= ai;
-                sm.t.A[i][col] = i > col ? sm.beta[i] * r * sm.t.kk[i][col] : 0.0f;
-                sm.t.N[i][col] = 0.0f;
-                const float pv = i >= col ? r * sm.t.qk[i][col] * NP_UP : 0.0f;
-                const __half h = __float2half_rn(pv);
-                np[(2 * CH + i) * NP_ROW + col] = h;
-                np[(3 * CH + i) * NP_ROW + col] = __float2half_rn(pv - __half2float(h));
+            for (int k = 0; k < 8; k++) {
+                const int i = 8 * seg + k;
+                const float ai = sm.a[i], be = sm.beta[i];
+                const float2 kk = *reinterpret_cast<const float2 *>(&sm.t.kk[i][col]), qk = *reinterpret_cast<const float2 *>(&sm.t.qk[i][col]);
+                if (i > col) r[0] *= ai;
+                if (i > col + 1) r[1] *= ai;
+                *reinterpret_cast<float2 *>(&sm.t.A[i][col]) = make_float2(i > col ? be * r[0] * kk.x : 0.0f, i > col + 1 ? be * r[1] * kk.y : 0.0f);
+                *reinterpret_cast<float2 *>(&sm.t.N[i][col]) = make_float2(0.0f, 0.0f);
+                uint32_t h2, l2;
+                split2(i >= col ? r[0] * qk.x * NP_UP : 0.0f, i >= col + 1 ? r[1] * qk.y * NP_UP : 0.0f, h2, l2);
+                *reinterpret_cast<uint32_t *>(np + (2 * CH + i) * NP_ROW + col) = h2;
+                *reinterpret_cast<uint32_t *>(np + (3 * CH + i) * NP_ROW + col) = l2;
                 if (col == 0) decay[i] = c *= ai;
-                if (i == CH - 1) decay[CH + col] = r;
+                if (i == CH - 1) *reinterpret_cast<float2 *>(decay + CH + col) = make_float2(r[0], r[1]);
             }
         }
         __syncthreads();
-        // (I + A)^-1: the four 16 x 16 blocks of the diagonal by substitution, a column per thread
+        // (I + A)^-1: the eight 8 x 8 blocks of the diagonal by substitution, a column per thread
         if (tid < CH) {
-            const int o = tid & ~15, cc = tid & 15;
-            float y[16];
+            const int o = tid & ~7, cc = tid & 7;
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float s0 = i == cc ? 1.0f : 0.0f, s1 = 0.0f;
+            for (int i = 0; i < 8; i++) {
+                float sum = i == cc ? 1.0f : 0.0f;
 #pragma unroll
-                for (int l = 0; l < i; l++) {
-                    if (l & 1) s1 = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s1);
-                    else s0 = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], s0);
-                }
-                y[i] = s0 + s1;
-                sm.t.N[o + i][o + cc] = y[i];
+                for (int l = 0; l < i; l++) sum = __fmaf_rn(-sm.t.A[o + i][o + l], y[l], sum);
+                y[i] = sum;
+                sm.t.N[o + i][o + cc] = sum;
             }
         }
         __syncthreads();
-        // then the blocks below it, twice the size each time: N_21 = -N_22 (A_21 N_11).  A_21's place takes the inner product.
+        // then the blocks below it, twice the size each time
+        lower_block<8>(sm.t.A, sm.t.N, tid);
         lower_block<16>(sm.t.A, sm.t.N, tid);
         lower_block<32>(sm.t.A, sm.t.N, tid);
         for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
@@ -430,7 +433,8 @@ template <int DK> struct ChunkSmem {
     int gave_up;
 };
 
-// Warps 0-7 work, warp 8 fetches.  The workers' own barrier (1) never waits for the fetching warp; the two sides tell each other through mbarriers: *_full, the data
+// Warps 0-7 work, warps 8-11 fetch values, K and Q, N, P (a bulk copy takes its thread about 300 ns to start, whatever its size, so that one thread for all of
+// them would be behind).  The workers' own barrier (1) never waits for the fetching warps; the two sides tell each other through mbarriers: *_full, the data
 // of a chunk is there; *_free, its place may be filled again.
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool workers_sync_or(bool x) {
@@ -490,7 +494,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
     int64_t b, e;
     delta_rows(d, s, &b, &e);
     const int64_t slot0 = delta_slot(b, s), chunks = (e - b + CH - 1) / CH;
-    const bool fetches = warp == 8;
+    const bool fetches = warp >= 8;
     const int mt = warp % MT, n0 = (warp & 7) / MT * NU;  // this warp's tiles of the state: rows 16 mt .., columns 8 (n0 + n) ..
 
     float S[NU][4];
@@ -517,7 +521,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         agn_mbar_expect_tx(bar, NP_BYTES);
         agn_bulk_g2s(dst, x.np + (((slot0 + c) * d.n_v + hv) * 4 + w) * CH * NROW, NP_BYTES, bar);
     };
-    auto load_v = [&](int64_t c) {  // by the fetching warp
+    auto load_v = [&](int64_t c) {
         const int64_t first = b + c * CH;
         float *dst = sm.v[c & 1];
         const float *src = d.v + first * d.v_stride + (int64_t)hv * d.dv + c0;
@@ -556,40 +560,34 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
     __syncthreads();
 
     if (fetches) {
-        int64_t kq_issued = 0, n_issued = 0, p_issued = 0;
-        for (int64_t c = 0; c < chunks; c++) {
-            const uint32_t before = (c - 1) & 1;  // the turn in which these places were last used
-            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.kq_free, before))) break;
-            if (lane == 0) load_kq(c);
-            kq_issued++;
-            __syncwarp();
-            load_v(c);
-            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.n_free, before))) break;
-            if (lane == 0) load_np(c, 0, sm.n, &sm.n_full);
-            n_issued++;
-            __syncwarp();
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            const float *v = sm.v[c & 1];
-            uint32_t most = 0;
+        uint64_t *const full[4] = {&sm.v_full, &sm.kq_full, &sm.n_full, &sm.p_full}, *const free[4] = {&sm.kq_free, &sm.kq_free, &sm.n_free, &sm.p_free};
+        const int what = warp - 8;
+        int64_t c = 0;
+        for (; c < chunks; c++) {
+            if (c > 0 && !__all_sync(0xffffffffu, wait(free[what], (c - 1) & 1))) break;  // the turn in which the place was last used
+            if (what == 0) {
+                load_v(c);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                const float *v = sm.v[c & 1];
+                uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < CH * 8 / 32; i++) {
-                const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
-                most = max(most, max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
-                                     max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu)));
+                for (int i = 0; i < CH * 8 / 32; i++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
+                    most = max(most, max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
+                                         max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu)));
+                }
+                tell_largest(most);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.v_full);
+            } else if (lane == 0) {
+                if (what == 1) load_kq(c);
+                else if (what == 2) load_np(c, 0, sm.n, &sm.n_full);
+                else load_np(c, 2, sm.p, &sm.p_full);
             }
-            tell_largest(most);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.v_full);
-            if (c > 0 && !__all_sync(0xffffffffu, wait(&sm.p_free, before))) break;
-            if (lane == 0) load_np(c, 2, sm.p, &sm.p_full);
-            p_issued++;
             __syncwarp();
         }
         // no copy may be in flight when the CTA ends
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        if (kq_issued) (void)agn_mbar_wait(&sm.kq_full, (kq_issued - 1) & 1, x.spin);
-        if (n_issued) (void)agn_mbar_wait(&sm.n_full, (n_issued - 1) & 1, x.spin);
-        if (p_issued) (void)agn_mbar_wait(&sm.p_full, (p_issued - 1) & 1, x.spin);
+        if (lane == 0 && what > 0 && c > 0) (void)agn_mbar_wait(full[what], (c - 1) & 1, x.spin);
         if (lane == 0 && sm.gave_up) atomicOr(d.flags, AGN_FLAG_TIMEOUT);
         return;
     }
@@ -699,7 +697,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         freed(&sm.kq_free);  // q has been read; the other buffers of k and v were last chunk's
         if ((gave_up = workers_sync_or(!wait(&sm.n_full, turn)))) break;
 
-        // ---- D = N X: a lower triangle, so up to the warp's own rows
+        // ---- D = N X.  (N is a lower triangle, but leaving its empty blocks out would only make the warps uneven: the slowest one does them all.)
         float dd[2][4] = {}, po[2][4] = {};
         {
             float t1[2][4] = {}, t2[2][4] = {};  // the three products apart: short chains
