@@ -11,77 +11,96 @@
 
 namespace {
 
-// Joins the parts of the rows that attn_decode_kernel shared out over several CTAs, and writes the rows that see nothing: a CTA
-// per (row, query head); the parts' weights first, one part per thread, then blockDim.x / (32 NB) shares of the parts are summed
-// side by side, a value per thread.
-constexpr int JOIN_THREADS = 512;
+// Joins the parts of the rows that attn_decode_kernel shared out over several CTAs, and writes the rows that see nothing.  A CTA per (row, query head); a warp takes
+// every 16th part, four at a time (all their loads at once: the kernel is a few waits for memory long), each with maximum and sums of its own, and the warps'
+// results are joined in shared memory.
+constexpr int JOIN_THREADS = 512, JOIN_TEAMS = JOIN_THREADS / 32;
 __global__ void __launch_bounds__(JOIN_THREADS) attn_join_kernel(const __grid_constant__ DecodeArgs d) {
     agn_pdl_prologue();
-    __shared__ int64_t warp_sums[JOIN_THREADS / 32], mine[2], all;
-    __shared__ float weight[2 * ATTN_MAX_SMS], sums[JOIN_THREADS], red[2][JOIN_THREADS / 32];
-    __shared__ int slot[2 * ATTN_MAX_SMS];
+    __shared__ int64_t warp_sums[JOIN_TEAMS], mine[2];
+    __shared__ __align__(16) float sums[JOIN_TEAMS][256];
+    __shared__ float ms[JOIN_TEAMS], ls[JOIN_TEAMS];
     const AttnArgs &a = d.a;
     const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, tid = threadIdx.x, hd = a.hd;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.hd;
     const int64_t out = (t * a.n_q + h) * hd;
-    int64_t r0, r1, pre, total;
-    scan_rows(a, d.tt, warp_sums, &r0, &r1, &pre, &total);
-    if (r0 <= t && t < r1) {
-        for (int64_t r = r0; r < t; r++) pre += attn_tiles(a, r, d.tt);
-        mine[0] = pre;
-        mine[1] = attn_tiles(a, t, d.tt);
-        all = total;
+    int64_t w = 0, n, all;
+    if (a.T == 1) {
+        n = all = attn_tiles(a, 0, d.tt);
+    } else {
+        int64_t r0, r1, pre;
+        scan_rows(a, d.tt, warp_sums, &r0, &r1, &pre, &all);
+        if (r0 <= t && t < r1) {
+            for (int64_t r = r0; r < t; r++) pre += attn_tiles(a, r, d.tt);
+            mine[0] = pre;
+            mine[1] = attn_tiles(a, t, d.tt);
+        }
+        __syncthreads();
+        w = mine[0];
+        n = mine[1];
     }
-    __syncthreads();
-    const int64_t w = mine[0], n = mine[1];
     if (n == 0) {
         if (tid < hd) store_act(d, out + tid, 0.0f);
         return;
     }
     const AttnShares shares(all, d.parts);
-    const int x0 = shares.part(w), x1 = shares.part(w + n - 1), nx = x1 - x0 + 1;
-    if (nx == 1) return;
+    const int x0 = a.T == 1 ? 0 : shares.part(w), x1 = a.T == 1 ? d.parts - 1 : shares.part(w + n - 1);
+    if (shares.start(x0) <= w && w + n <= shares.start(x0 + 1)) return;  // in one part: written there
     const float *part = d.part + (int64_t)h * (hd + 4);
-    float m = -INFINITY, l = 0.0f;
-    if (tid < nx) {  // at most 2 * 148 parts
-        const int64_t begin = shares.start(x0 + tid), end = shares.start(x0 + tid + 1);
-        // its first run of tiles is this row's unless the CTA began in an earlier row; a CTA without tiles left nothing
-        const int s = begin < end ? 2 * (x0 + tid) + (begin < w ? 1 : 0) : -1;
-        slot[tid] = s;
-        if (s >= 0) {
-            m = part[(int64_t)s * d.slot_floats + hd];
-            l = part[(int64_t)s * d.slot_floats + hd + 1];
+    float M = -INFINITY, L = 0.0f;
+    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    for (int x = x0 + warp; x <= x1; x += 4 * JOIN_TEAMS) {
+        float m[4], l[4];
+        float4 v[4][2];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int y = x + k * JOIN_TEAMS;
+            const int64_t begin = shares.start(y);
+            const bool there = y <= x1 && begin < shares.start(y + 1);  // a CTA without tiles left nothing
+            // its first run of tiles is this row's unless the CTA began in an earlier row
+            const float *p = part + (2 * (int64_t)y + (begin < w ? 1 : 0)) * d.slot_floats;
+            m[k] = there ? p[hd] : -INFINITY;
+            l[k] = there ? p[hd + 1] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                v[k][i] = there && 4 * lane + 128 * i < hd ? *reinterpret_cast<const float4 *>(p + 4 * lane + 128 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        const float top = fmaxf(fmaxf(M, fmaxf(m[0], m[1])), fmaxf(m[2], m[3])), mu = top == -INFINITY ? 0.0f : top, c = ex2(M - mu);
+        M = top;
+        L *= c;
+#pragma unroll
+        for (int i = 0; i < 2; i++) { o[i].x *= c; o[i].y *= c; o[i].z *= c; o[i].w *= c; }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = ex2(m[k] - mu);
+            L = __fmaf_rn(f, l[k], L);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                o[i].x = __fmaf_rn(f, v[k][i].x, o[i].x); o[i].y = __fmaf_rn(f, v[k][i].y, o[i].y);
+                o[i].z = __fmaf_rn(f, v[k][i].z, o[i].z); o[i].w = __fmaf_rn(f, v[k][i].w, o[i].w);
+            }
         }
     }
-    float M = agn_warp_max(m);
-    if ((tid & 31) == 0) red[0][tid >> 5] = M;
-    __syncthreads();
-    for (int i = 0; i < JOIN_THREADS / 32; i++) M = fmaxf(M, red[0][i]);
-    const float c = ex2(m - (M == -INFINITY ? 0.0f : M));
-    if (tid < nx) {
-        weight[tid] = slot[tid] >= 0 ? c : 0.0f;
+    if (lane == 0) {
+        ms[warp] = M;
+        ls[warp] = L;
     }
-    float L = agn_warp_sum(tid < nx ? l * c : 0.0f);
-    if ((tid & 31) == 0) red[1][tid >> 5] = L;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (4 * lane + 128 * i < hd) *reinterpret_cast<float4 *>(&sums[warp][4 * lane + 128 * i]) = o[i];
     __syncthreads();
-    L = 0.0f;
-    for (int i = 0; i < JOIN_THREADS / 32; i++) L += red[1][i];
-    const int teams = JOIN_THREADS / hd, team = tid / hd, i = tid % hd;
-    float o = 0.0f;
-    if (team < teams) {
-#pragma unroll 8
-        for (int x = team; x < nx; x += teams) {
-            const float f = weight[x];
-            const float v = f != 0.0f ? part[(int64_t)slot[x] * d.slot_floats + i] : 0.0f;
-            o = __fmaf_rn(f, v, o);
-        }
+    if (tid >= hd) return;
+    float top = -INFINITY, sum = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < JOIN_TEAMS; k++) top = fmaxf(top, ms[k]);
+    const float mu = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < JOIN_TEAMS; k++) {
+        const float f = ex2(ms[k] - mu);
+        sum = __fmaf_rn(f, ls[k], sum);
+        y = __fmaf_rn(f, sums[k][tid], y);
     }
-    sums[tid] = o;
-    __syncthreads();
-    if (tid < hd) {
-        for (int k = 1; k < teams; k++) o += sums[tid + k * hd];
-        store_act(d, out + tid, o / L);
-    }
+    store_act(d, out + tid, y / sum);
 }
 
 // The decode kernel's shape for a call: heads to a CTA, warps to a head, tiles, stages.
@@ -121,7 +140,7 @@ int64_t attn_workspace(int64_t T, int n_q, int hd) {
 }
 
 // Few rows of one sequence are cheaper as single rows.
-constexpr int CHUNK_MIN_TOKENS = 4;
+constexpr int CHUNK_MIN_TOKENS = 16;
 bool chunk_fits(int64_t T, int n_q, int n_kv) { return T >= CHUNK_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30); }
 
 template <typename T>
@@ -148,7 +167,10 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: caches must be %d-byte aligned", ca);
     const bool prompt = !pos && sizeof(T) == 2 && agn_attention_prompt_fits(rows, n_q, n_kv, hd);
     const bool chunk = !pos && !prompt && chunk_fits(rows, n_q, n_kv);
-    const int64_t need = prompt ? agn_attention_prompt_workspace(pos_start + rows, n_kv, hd) : chunk ? 0 : attn_workspace(rows, n_q, hd);
+    const int sms = ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS;
+    const int64_t end = (int64_t)pos_start + rows;
+    const int64_t need = prompt ? agn_attention_prompt_workspace(end, rows, n_q, n_kv, hd, sms)
+                         : chunk ? agn_attention_chunk_workspace(end, rows, n_q, n_kv, hd, sms) : attn_workspace(rows, n_q, hd);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !agn_aligned16(workspace)))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     AGN_CUDA(ctx, cudaSetDevice(ctx->device));
@@ -158,9 +180,9 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     a.bytes_per_token = (int)agn_kv_bytes_per_token(kv_dtype, (int64_t)n_kv * hd); a.scale = scale; a.flags = ctx->d_flags;
     ctx->flags_dirty = true;
     if (prompt) return agn_attention_prompt_f16(ctx, a, kv_dtype, workspace);
-    if (chunk) return agn_attention_chunk(ctx, a, kv_dtype, sizeof(T) == 2);
+    if (chunk) return agn_attention_chunk(ctx, a, kv_dtype, sizeof(T) == 2, workspace);
     const int block_bytes = kv_dtype == AGN_F16 ? 64 : kv_dtype == AGN_Q8_0 ? 34 : 36;
-    const DecodePlan p = decode_plan(rows, n_q, n_kv, hd, max_seq, block_bytes, kv_dtype == AGN_F16, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);
+    const DecodePlan p = decode_plan(rows, n_q, n_kv, hd, max_seq, block_bytes, kv_dtype == AGN_F16, sms);
     DecodeArgs d;
     d.a = a; d.part = static_cast<float *>(workspace); d.parts = p.parts; d.act16 = sizeof(T) == 2; d.tt = p.tt; d.stages = p.stages; d.hc = p.hc;
     d.groups = p.groups; d.row_stride = p.row_stride; d.col_groups = p.col_groups; d.slot_floats = n_q * (hd + 4);
@@ -185,10 +207,14 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
 extern "C" int64_t agn_attention_kv_workspace_bytes(int64_t T, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int64_t max_seq_len,
                                                     int32_t has_pos) {
     if (!attn_shape_ok(T, n_q_heads, n_kv_heads, head_dim, max_seq_len)) return 0;
-    const int64_t decode = attn_workspace(T, n_q_heads, head_dim);
-    if (has_pos || !agn_attention_prompt_fits(T, n_q_heads, n_kv_heads, head_dim)) return decode;
-    const int64_t prompt = agn_attention_prompt_workspace(max_seq_len, n_kv_heads, head_dim);
-    return prompt > decode ? prompt : decode;
+    int64_t need = attn_workspace(T, n_q_heads, head_dim);
+    if (has_pos) return need;
+    // for whichever activation type the rows have, and for rows that end anywhere in the cache
+    const int64_t chunk = chunk_fits(T, n_q_heads, n_kv_heads) ? agn_attention_chunk_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS) : 0;
+    const int64_t prompt = agn_attention_prompt_fits(T, n_q_heads, n_kv_heads, head_dim)
+                               ? agn_attention_prompt_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS) : 0;
+    if (chunk > need) need = chunk;
+    return prompt > need ? prompt : need;
 }
 
 extern "C" int32_t agn_attention_kv_f32(agn_ctx *ctx, const float *q, float *out, int32_t kv_dtype, const void *k_cache, const void *v_cache,

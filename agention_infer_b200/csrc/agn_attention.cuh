@@ -15,15 +15,41 @@ struct AttnArgs {
     uint32_t *flags;
 };
 
+constexpr int ATTN_MAX_SMS = 148;
+
+// A prompt's rows over a long cache are too few CTAs when the rows are few: the slots are then shared out as well.  Split x of a row leaves part[x][row][hd + 4] (row =
+// token * n_q + head): the sums of weighted values, the reference maximum (log2) and the sum of weights; agn_attention_join adds them up.
+struct AttnSplit {
+    float *part;
+    int splits;  // 1: rows are written as they are
+};
+// The number of splits, up to one CTA per SM, that is the quickest by a model of two terms: the tiles that follow one another in a CTA (tile_us each), and,
+// where there are splits, 6 us for one more launch and the shares' way through memory at 2.5 TB/s.  (32 rows of 28/4 heads of 128 over 8000 q8_0 slots, f16: one share
+// 161 us, 37 shares 40 us; 512 rows over 1000 slots: one share 42 us, two 62 us.)
+inline int attn_splits(int64_t ctas, int64_t tiles, double tile_us, int64_t rows, int hd, int sms) {
+    int best = 1;
+    double least = tiles * tile_us;
+    for (int64_t n = 2; n <= sms / (ctas > 0 ? ctas : 1) && n <= tiles; n++) {
+        const double us = (double)((tiles + n - 1) / n) * tile_us + 6.0 + (double)(rows * n) * (hd + 4) * 8 / 2.5e6;
+        if (us < least) {
+            least = us;
+            best = (int)n;
+        }
+    }
+    return best;
+}
+inline int64_t attn_part_bytes(int splits, int64_t T, int n_q, int hd) { return splits > 1 ? (int64_t)splits * T * n_q * (hd + 4) * 4 : 0; }
+// odd: [n_kv][odd_tiles] flags of groups of `group` slots whose values are not all finite (they were taken as 0), or null: look at every slot.
+int32_t agn_attention_join(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, AttnSplit split, const int *odd, int64_t odd_tiles, int group);
+
 // Rows of a prompt in f16 on the tensor cores (agn_attention_prompt.cu), where that form covers the call.
-#define AGN_PROMPT_MIN_ROWS 128
-#define AGN_PROMPT_MIN_TOKENS 16
 bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd);
-int64_t agn_attention_prompt_workspace(int64_t slots, int n_kv, int hd);
+int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms);
 int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace);
 
 // Rows of a prompt that the form above does not cover: f32 rows, other head sizes (agn_attention_chunk.cu).
-int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16);
+int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms);
+int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, void *workspace);
 
 constexpr int KV_F16 = 0, KV_Q8 = 1, KV_WORDS = 2;
 template <int KV> struct KvFormat;  // a block of 32 values of one head: BYTES, with the values DATA bytes behind its start

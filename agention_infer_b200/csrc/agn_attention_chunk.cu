@@ -102,7 +102,7 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
 }
 
-template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THREADS, 1) attn_chunk_kernel(const __grid_constant__ DecodeArgs d) {
+template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THREADS, 1) attn_chunk_kernel(const __grid_constant__ DecodeArgs d, AttnSplit split, int row_tiles, int *odd_flags) {
     agn_pdl_prologue();
     using C = ChunkShape<NB>;
     using F = KvFormat<KV>;
@@ -111,8 +111,10 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     const AttnArgs &a = d.a;
     constexpr int HD = C::HD, ROW = C::ROW;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, G = a.n_q / a.n_kv, kvh = blockIdx.x % a.n_kv;
-    const int rows = (int)a.T * G, r0 = (int)((gridDim.x - 1 - blockIdx.x) / a.n_kv) * C::ROWS;  // the rows that see most first
-    const int last_row = min(r0 + C::ROWS, rows) - 1, end = a.pos_start + last_row / G + 1, tiles = (end + SL - 1) / SL;
+    const int share = blockIdx.x / a.n_kv % split.splits;
+    const int rows = (int)a.T * G, r0 = (row_tiles - 1 - (int)(blockIdx.x / a.n_kv / split.splits)) * C::ROWS;  // the rows that see most first
+    const int last_row = min(r0 + C::ROWS, rows) - 1, end = a.pos_start + last_row / G + 1, seen_tiles = (end + SL - 1) / SL;
+    const int per_share = (seen_tiles + split.splits - 1) / split.splits, tile0 = min(share * per_share, seen_tiles), tiles = min(seen_tiles, tile0 + per_share);  // tile0 .. tiles - 1
     if (tid == 0) sm.odd = 0;
 
     auto fetch = [&](Block<KV> &x, int i, int tile) {
@@ -144,7 +146,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
         }
     };
     __syncthreads();
-    fetch_tile(0);
+    if (tile0 < tiles) fetch_tile(tile0);
 
     // ---- Q, a warp's 16 rows: largest value to [1, 2), two f16 parts
     for (int i = 0; i < 16; i++) {
@@ -168,7 +170,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
             sm.q[1][(warp * 16 + i) * ROW + c * 32 + lane] = __float2half_rn(v - __half2float(h));
         }
     }
-    place_tile(0);
+    if (tile0 < tiles) place_tile(tile0);
     __syncthreads();
 
     const int ra = r0 + warp * 16 + g;  // this lane's rows: ra and ra + 8
@@ -179,7 +181,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
 #pragma unroll
     for (int i = 0; i < 4 * NB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-    for (int tile = 0; tile < tiles; tile++) {
+    for (int tile = tile0; tile < tiles; tile++) {
         if (tile + 1 < tiles) fetch_tile(tile + 1);
         if (tile * SL <= warp_last) {  // a warp whose rows see none of it waits for the others
             const int buf = tile & 1;
@@ -300,7 +302,17 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
         const int r = ra + 8 * i;
         if (r >= rows) continue;
         const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD;
-        const float inv = 1.0f / l[i];
+        if (split.splits > 1) {  // a share: what agn_attention_join needs
+            float *to = split.part + ((int64_t)share * a.T * a.n_q + at / HD) * (HD + 4);
+            if (t4 == 0) *reinterpret_cast<float2 *>(to + HD) = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                *reinterpret_cast<float4 *>(to + b * 32 + 8 * t4) = make_float4(o[4 * b][2 * i], o[4 * b + 1][2 * i], o[4 * b + 2][2 * i], o[4 * b + 3][2 * i]);
+                *reinterpret_cast<float4 *>(to + b * 32 + 8 * t4 + 4) = make_float4(o[4 * b][2 * i + 1], o[4 * b + 1][2 * i + 1], o[4 * b + 2][2 * i + 1], o[4 * b + 3][2 * i + 1]);
+            }
+            continue;
+        }
+        const float inv = m[i] == -INFINITY ? NAN : 1.0f / l[i];  // all scores -inf: 0 / 0
 #pragma unroll
         for (int b = 0; b < NB; b++) {  // dims 8 t4 .. 8 t4 + 7 of the block
             store_act4(d, at, b * 8 + 2 * t4, make_float4(o[4 * b][2 * i] * inv, o[4 * b + 1][2 * i] * inv, o[4 * b + 2][2 * i] * inv, o[4 * b + 3][2 * i] * inv));
@@ -311,6 +323,10 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     if (KV == KV_F16) {  // rare: V held values that are not finite
         __syncthreads();
         if (!sm.odd) return;
+        if (split.splits > 1) {
+            if (tid == 0) odd_flags[kvh] = 1;  // by agn_attention_join
+            return;
+        }
         for (int x = tid; x < C::ROWS * HD; x += C::THREADS) {
             const int r = r0 + x / HD, dim = x % HD;
             if (r >= rows) break;
@@ -322,36 +338,65 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     }
 }
 
-template <int KV, int NB> int32_t launch_chunk(agn_ctx *ctx, const DecodeArgs &d) {
+__global__ void attn_clear_kernel(int *p, int n) {
+    agn_pdl_prologue();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
+}
+
+int chunk_rows(int hd) { return hd <= 128 ? 128 : 64; }
+struct ChunkLayout {
+    int row_tiles, splits;
+    int64_t odd, bytes;
+};
+ChunkLayout chunk_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) {
+    ChunkLayout l;
+    l.row_tiles = (int)((T * (n_q / n_kv) + chunk_rows(hd) - 1) / chunk_rows(hd));
+    l.splits = attn_splits((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 0.5 + 0.045 * hd, T * n_q, hd, sms);
+    l.odd = attn_part_bytes(l.splits, T, n_q, hd);
+    l.bytes = l.splits > 1 ? l.odd + (n_kv * 4 + 15) / 16 * 16 : 0;
+    return l;
+}
+
+template <int KV, int NB> int32_t launch_chunk(agn_ctx *ctx, const DecodeArgs &d, const ChunkLayout &l, void *workspace) {
+    static_assert(ChunkShape<NB>::ROWS == (NB <= 4 ? 128 : 64), "chunk_rows");
     using C = ChunkShape<NB>;
     if (agn_ring_ctas_per_sm(ctx, attn_chunk_kernel<KV, NB>, C::THREADS, sizeof(ChunkTiles<NB>)) < 1)
         return agn_fail(ctx, AGN_ECUDA, "attention_kv: the chunk kernel does not fit the device's shared memory");
-    const int64_t rows = d.a.T * (d.a.n_q / d.a.n_kv);
-    agn_launch(ctx, attn_chunk_kernel<KV, NB>, dim3((unsigned)((rows + C::ROWS - 1) / C::ROWS * d.a.n_kv)), dim3(C::THREADS), sizeof(ChunkTiles<NB>), d);
+    AttnSplit split = {static_cast<float *>(workspace), l.splits};
+    int *odd = l.splits > 1 && KV == KV_F16 ? reinterpret_cast<int *>(static_cast<unsigned char *>(workspace) + l.odd) : nullptr;
+    if (odd) {
+        agn_launch(ctx, attn_clear_kernel, dim3(1), dim3(256), 0, odd, d.a.n_kv);
+        AGN_LAUNCHED(ctx, "attention_kv_chunk");
+    }
+    agn_launch(ctx, attn_chunk_kernel<KV, NB>, dim3((unsigned)((int64_t)l.row_tiles * d.a.n_kv * l.splits)), dim3(C::THREADS), sizeof(ChunkTiles<NB>), d, split, l.row_tiles, odd);
     AGN_LAUNCHED(ctx, "attention_kv_chunk");
-    return AGN_OK;
+    // one flag per KV head: a group of all slots
+    return l.splits > 1 ? agn_attention_join(ctx, d.a, AGN_F16, d.act16, split, odd, 1, 1 << 30) : AGN_OK;
 }
 
-template <int KV> int32_t launch_chunk_kv(agn_ctx *ctx, const DecodeArgs &d) {
+template <int KV> int32_t launch_chunk_kv(agn_ctx *ctx, const DecodeArgs &d, const ChunkLayout &l, void *workspace) {
     switch (d.a.hd / 32) {
-    case 1: return launch_chunk<KV, 1>(ctx, d);
-    case 2: return launch_chunk<KV, 2>(ctx, d);
-    case 3: return launch_chunk<KV, 3>(ctx, d);
-    case 4: return launch_chunk<KV, 4>(ctx, d);
-    case 5: return launch_chunk<KV, 5>(ctx, d);
-    case 6: return launch_chunk<KV, 6>(ctx, d);
-    case 7: return launch_chunk<KV, 7>(ctx, d);
-    default: return launch_chunk<KV, 8>(ctx, d);
+    case 1: return launch_chunk<KV, 1>(ctx, d, l, workspace);
+    case 2: return launch_chunk<KV, 2>(ctx, d, l, workspace);
+    case 3: return launch_chunk<KV, 3>(ctx, d, l, workspace);
+    case 4: return launch_chunk<KV, 4>(ctx, d, l, workspace);
+    case 5: return launch_chunk<KV, 5>(ctx, d, l, workspace);
+    case 6: return launch_chunk<KV, 6>(ctx, d, l, workspace);
+    case 7: return launch_chunk<KV, 7>(ctx, d, l, workspace);
+    default: return launch_chunk<KV, 8>(ctx, d, l, workspace);
     }
 }
 
 }  // namespace
 
-int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16) {
+int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) { return chunk_layout(slots, T, n_q, n_kv, hd, sms).bytes; }
+
+int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, void *workspace) {
+    const ChunkLayout l = chunk_layout((int64_t)a.pos_start + a.T, a.T, a.n_q, a.n_kv, a.hd, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);
     DecodeArgs d = {};
     d.a = a;
     d.act16 = act16;
-    if (kv_dtype == AGN_F16) return launch_chunk_kv<KV_F16>(ctx, d);
-    if (kv_dtype == AGN_Q8_0) return launch_chunk_kv<KV_Q8>(ctx, d);
-    return launch_chunk_kv<KV_WORDS>(ctx, d);
+    if (kv_dtype == AGN_F16) return launch_chunk_kv<KV_F16>(ctx, d, l, workspace);
+    if (kv_dtype == AGN_Q8_0) return launch_chunk_kv<KV_Q8>(ctx, d, l, workspace);
+    return launch_chunk_kv<KV_WORDS>(ctx, d, l, workspace);
 }

@@ -18,7 +18,7 @@
 
 #include "agn_attention.cuh"
 
-constexpr int ATTN_MAX_SMS = 148, ATTN_THREADS = 256, ATTN_WARPS = 8, ATTN_MAX_SPLIT_ROWS = 512;
+constexpr int ATTN_THREADS = 256, ATTN_WARPS = 8, ATTN_MAX_SPLIT_ROWS = 512;
 
 struct DecodeArgs {
     AttnArgs a;
@@ -101,8 +101,8 @@ __device__ __forceinline__ float byte_to_float(uint32_t u, int i) {
 // p = hi + lo, hi with tf32's 11 bits (cut) and lo what is left of it.  The values it is multiplied by may not be finite, or the scale in
 // it: with an infinite value lo must not be 0 (0 * inf), with an infinite p it must not be inf - inf, for the sum of
 // the two products to be what the one product would be.
-template <int KV> __device__ __forceinline__ void split_tf32(float p, float &hi, float &lo) {
-    hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
+template <int KV> __device__ __forceinline__ void split_tf32(float p, float &hi, float &lo, uint32_t half = 0) {
+    hi = __uint_as_float((__float_as_uint(p) + half) & 0xffffe000u);  // half: half a step of hi, for a hi that is rounded and used alone
     lo = KV == KV_F16 ? fmaxf(p - hi, 1.17549435e-38f) : fminf(p - hi, 1e35f);
 }
 // four / eight bytes at an address that is a multiple of 4, or (odd) 2 behind one
@@ -201,22 +201,33 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
         if (left == 0 && active && group == 0)  // a row that sees nothing
             for (int i = lane; i < cols * HD; i += 32) store_act(d, (cur.row * a.n_q + head) * HD + i, 0.0f);
     } else {
-        int64_t r0, r1, pre, total;
-        scan_rows(a, TT, warp_sums, &r0, &r1, &pre, &total);
-        const AttnShares shares(total, d.parts);
-        const int64_t w0 = shares.start(blockIdx.x), w1 = shares.start(blockIdx.x + 1);
-        for (int64_t t = r0; t < r1; t++) {
-            const int64_t n = attn_tiles(a, t, TT);
-            if (w0 >= pre && w0 < pre + n) { first_row = t; first_pre = pre; }
-            pre += n;
+        cur.row = 0;
+        cur.n = attn_row(a, 0, &cur.off);  // of a single row, or one that the scan below moves on from
+        int64_t w0, w1, pre0 = 0;
+        if (a.T == 1) {
+            const AttnShares shares(((uint32_t)cur.n + (uint32_t)TT - 1) / (uint32_t)TT, d.parts);
+            w0 = shares.start(blockIdx.x);
+            w1 = shares.start(blockIdx.x + 1);
+        } else {
+            int64_t r0, r1, pre, total;
+            scan_rows(a, TT, warp_sums, &r0, &r1, &pre, &total);
+            const AttnShares shares(total, d.parts);
+            w0 = shares.start(blockIdx.x);
+            w1 = shares.start(blockIdx.x + 1);
+            for (int64_t t = r0; t < r1; t++) {
+                const int64_t n = attn_tiles(a, t, TT);
+                if (w0 >= pre && w0 < pre + n) { first_row = t; first_pre = pre; }
+                pre += n;
+            }
+            __syncthreads();
+            if (w1 > w0) {
+                cur.row = first_row;
+                pre0 = first_pre;
+                cur.n = attn_row(a, cur.row, &cur.off);
+            }
         }
-        __syncthreads();
         left = (int)(w1 - w0);
-        if (left > 0) {
-            cur.row = first_row;
-            cur.n = attn_row(a, cur.row, &cur.off);
-            cur.j = (int)(w0 - first_pre) * TT;
-        }
+        cur.j = (int)(w0 - pre0) * TT;
     }
     if (left <= 0) return;
 
@@ -313,6 +324,7 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
     const int lane_k = unit * NB * F::BYTES + (group * PER + (g >> 1) + (g & 1) * 4) * RS;  // the slot whose key this lane reads
     const int lane_s = unit * NB * F::BYTES + (group * PER + t4) * RS;                      // the first slot whose score and value it holds
     const bool lo = !d.act16;
+    const uint32_t half = lo ? 0u : 0x1000u;
 
     // Slots cur.j + group * PER + 8 u + t4 (+ 4); EDGE: some of them are behind the row's end.
     auto slots = [&](auto edge) {
@@ -379,8 +391,8 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
         if (KV == KV_F16) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                split_tf32<KV>(sc[u][0], ph[u][0], pl[u][0]);
-                split_tf32<KV>(sc[u][1], ph[u][1], pl[u][1]);
+                split_tf32<KV>(sc[u][0], ph[u][0], pl[u][0], half);
+                split_tf32<KV>(sc[u][1], ph[u][1], pl[u][1], half);
             }
         }
 #pragma unroll
@@ -402,7 +414,7 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                         const uint32_t w = offset_bytes<KV>(load4_at(blk + F::DATA + g * 4, odd));
 #pragma unroll
                         for (int c = 0; c < 4; c++) f[i][c] = byte_to_float(w, c);
-                        split_tf32<KV>(sc[u][i] * block_scale<KV>(blk), ph[u][i], pl[u][i]);
+                        split_tf32<KV>(sc[u][i] * block_scale<KV>(blk), ph[u][i], pl[u][i], half);
                     }
                 }
                 mma_tf32(acc0, f[0][0], f[0][1], f[1][0], f[1][1], ph[u][0], ph[u][1]);

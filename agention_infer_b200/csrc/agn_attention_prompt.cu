@@ -27,7 +27,8 @@ struct PromptArgs {
     int *odd;        // [n_kv][tiles]: the V tile has a value that is not finite
     int kv_dtype;
     int64_t tiles, rows;  // tiles of the sequence; rows T * G of a KV head
-    int spin;
+    int spin, row_tiles;
+    AttnSplit split;
 };
 
 // One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a
@@ -147,10 +148,12 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     extern __shared__ unsigned char raw[];
     PromptSmem<HD> &sm = *reinterpret_cast<PromptSmem<HD> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const AttnArgs &a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.n_q / a.n_kv, head = blockIdx.x % a.n_kv;
-    const int64_t r0 = (int64_t)((gridDim.x - 1 - blockIdx.x) / a.n_kv) * 2 * TILE;  // the rows that see most first, so that the last CTAs are short
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.n_q / a.n_kv, head = blockIdx.x % a.n_kv, share = blockIdx.x / a.n_kv % p.split.splits;
+    const int64_t r0 = (int64_t)(p.row_tiles - 1 - (int)(blockIdx.x / a.n_kv / p.split.splits)) * 2 * TILE;  // the rows that see most first, so that the last CTAs are short
     const int64_t last_row = r0 + 2 * TILE - 1 < p.rows ? r0 + 2 * TILE - 1 : p.rows - 1;
-    const int tiles = (int)((a.pos_start + last_row / G) / TILE) + 1;  // that the CTA's last row sees
+    const int seen_tiles = (int)((a.pos_start + last_row / G) / TILE) + 1;  // by the CTA's last row
+    const int per_share = (seen_tiles + p.split.splits - 1) / p.split.splits, tile0 = min(share * per_share, seen_tiles);
+    const int tiles = min(seen_tiles - tile0, per_share);  // of this CTA's share, from tile0 on
     constexpr uint32_t IMAGE = TILE * HD * 2;
 
     // ---- warps 0-7: the query row of this thread, and Q on its way (a warp's 32 rows, whole rows side by side)
@@ -209,8 +212,8 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
 
     if (warp == 8) {
         if (lane == 0) {
-            const unsigned char *k = reinterpret_cast<const unsigned char *>(p.k) + (int64_t)head * p.tiles * IMAGE;
-            const unsigned char *v = reinterpret_cast<const unsigned char *>(p.v) + (int64_t)head * p.tiles * IMAGE;
+            const unsigned char *k = reinterpret_cast<const unsigned char *>(p.k) + (head * p.tiles + tile0) * IMAGE;
+            const unsigned char *v = reinterpret_cast<const unsigned char *>(p.v) + (head * p.tiles + tile0) * IMAGE;
             int n = 0;
             for (; n < 2 * tiles; n++) {
                 const int at = n % SLOTS;
@@ -233,7 +236,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
                 }
                 mma_commit(&sm.s_full[i]);
             };
-            bool ok = wait(&sm.q_full, 0) && wait(&sm.full[0], 0);
+            bool ok = tiles > 0 && wait(&sm.q_full, 0) && wait(&sm.full[0], 0);
             if (ok) {
                 fence_after();
                 scores(0, kva);
@@ -281,8 +284,8 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
             if (!(ok = wait_warp(&sm.s_full[i], j & 1))) break;
             fence_after();
             // The scores are read twice, 32 at a time: 128 of them beside the rest do not fit the 168 registers of a thread.
-            const int seen = last - j * TILE;  // slots c <= seen of this tile
-            const bool edge = j * TILE + TILE - 1 > first_last;
+            const int seen = last - (tile0 + j) * TILE;  // slots c <= seen of this tile
+            const bool edge = (tile0 + j) * TILE + TILE - 1 > first_last;
             uint32_t s[2][32];
             float x0 = -INFINITY, x1 = -INFINITY;
             tmem_load32(s_at, s[0]);
@@ -349,9 +352,26 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
             fence_before();
             bar_arrive(&sm.p_full[i]);
         }
-        if (ok && (ok = wait_warp(&sm.o_full[i], 0))) {
+        if (p.split.splits > 1) {
+            // a share: what agn_attention_join needs
+            float *to = p.split.part + ((int64_t)share * a.T * a.n_q + (there ? own / HD : 0)) * (HD + 4);
+            if (there) *reinterpret_cast<float2 *>(to + HD) = make_float2(m, l);
+            if (tiles > 0 && ok && (ok = wait_warp(&sm.o_full[i], 0))) {
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_at + c, o);
+                    tmem_loaded(o);
+                    if (there) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) *reinterpret_cast<uint4 *>(to + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    }
+                }
+            }
+        } else if (ok && (ok = wait_warp(&sm.o_full[i], 0))) {
             fence_after();
-            const float inv = 1.0f / l;
+            const float inv = m == -INFINITY ? NAN : 1.0f / l;  // all scores -inf: 0 / 0
             // The output goes out through the queries' place in shared memory (the last product that reads them is done), whole rows side by side.
             unsigned char *stage = sm.q[i] + (warp & 3) * 32 * HD * 2;
 #pragma unroll
@@ -388,6 +408,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     if (tid == 0 && sm.gave_up) atomicOr(a.flags, AGN_FLAG_TIMEOUT);
 
     // Rare: V holds values that are not finite.  They were 0 in the product.
+    if (p.split.splits > 1) return;  // by agn_attention_join
     bool any = false;
     for (int j = tid; j < tiles; j += PROMPT_THREADS) any |= p.odd[head * p.tiles + j] != 0;
     if (!__syncthreads_or(any)) return;
@@ -415,29 +436,48 @@ template <int HD> int32_t launch_prompt(agn_ctx *ctx, const PromptArgs &p, int k
     else if (kv_dtype == AGN_Q8_0) agn_launch(ctx, attn_unpack_kernel<KV_Q8>, tiles, dim3(1024), 0, p);
     else agn_launch(ctx, attn_unpack_kernel<KV_WORDS>, tiles, dim3(1024), 0, p);
     AGN_LAUNCHED(ctx, "attention_kv_prompt");
-    agn_launch(ctx, attn_prompt_kernel<HD>, dim3((unsigned)((p.rows + 2 * TILE - 1) / (2 * TILE) * p.a.n_kv)), dim3(PROMPT_THREADS), smem, p);
+    agn_launch(ctx, attn_prompt_kernel<HD>, dim3((unsigned)((int64_t)p.row_tiles * p.a.n_kv * p.split.splits)), dim3(PROMPT_THREADS), smem, p);
     AGN_LAUNCHED(ctx, "attention_kv_prompt");
-    return AGN_OK;
+    return p.split.splits > 1 ? agn_attention_join(ctx, p.a, kv_dtype, 1, p.split, p.odd, p.tiles, TILE) : AGN_OK;
 }
 
 }  // namespace
 
-bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd) {
-    return (hd == 64 || hd == 128) && T * (n_q / n_kv) >= AGN_PROMPT_MIN_ROWS && T >= AGN_PROMPT_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30);
-}
+// From so few tokens on the prompt form is the faster one (rows of 28/4 heads of 128 over 8000 q8_0 slots, single rows / prompt form: PROMPT_FIGURES).
+constexpr int PROMPT_MIN_TOKENS = 8;
+bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd) { return (hd == 64 || hd == 128) && T >= PROMPT_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30); }
 
-int64_t agn_attention_prompt_workspace(int64_t slots, int n_kv, int hd) {
-    return 2 * image_bytes(slots, n_kv, hd) + (odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;
+namespace {
+struct PromptLayout {
+    int64_t image, odd, part, bytes;  // bytes of an image set; byte offsets
+    int row_tiles, splits;
+};
+PromptLayout prompt_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) {
+    PromptLayout l;
+    l.image = image_bytes(slots, n_kv, hd);
+    l.odd = 2 * l.image;
+    l.part = l.odd + (odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;
+    l.row_tiles = (int)((T * (n_q / n_kv) + 2 * TILE - 1) / (2 * TILE));
+    l.splits = attn_splits((int64_t)l.row_tiles * n_kv, (slots + TILE - 1) / TILE, 2.4, T * n_q, hd, sms);
+    l.bytes = l.part + attn_part_bytes(l.splits, T, n_q, hd);
+    return l;
 }
+}  // namespace
+
+int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) { return prompt_layout(slots, T, n_q, n_kv, hd, sms).bytes; }
 
 int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace) {
     PromptArgs p;
-    const int64_t slots = (int64_t)a.pos_start + a.T, image = image_bytes(slots, a.n_kv, a.hd);
+    const int64_t slots = (int64_t)a.pos_start + a.T;
+    const PromptLayout l = prompt_layout(slots, a.T, a.n_q, a.n_kv, a.hd, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);
     unsigned char *w = static_cast<unsigned char *>(workspace);
     p.a = a;
     p.k = reinterpret_cast<__half *>(w);
-    p.v = reinterpret_cast<__half *>(w + image);
-    p.odd = reinterpret_cast<int *>(w + 2 * image);
+    p.v = reinterpret_cast<__half *>(w + l.image);
+    p.odd = reinterpret_cast<int *>(w + l.odd);
+    p.split.part = reinterpret_cast<float *>(w + l.part);
+    p.split.splits = l.splits;
+    p.row_tiles = l.row_tiles;
     p.tiles = (slots + TILE - 1) / TILE;
     p.rows = a.T * (a.n_q / a.n_kv);
     p.kv_dtype = kv_dtype;
