@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int TILE = 128, PROMPT_THREADS = 320, SLOTS = 5;
+constexpr int TILE = 128, PROMPT_THREADS = 320, SLOTS = 5, DRAIN_POLLS = AGN_MBAR_SPIN_LIMIT_DEFAULT;  // the last waits are not cut short by the option
 
 struct PromptArgs {
     AttnArgs a;
@@ -222,7 +222,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
                 agn_bulk_g2s(sm.kv[at], (n & 1 ? v : k) + (int64_t)(n >> 1) * IMAGE, IMAGE, &sm.full[at]);
             }
             // no copy may be in flight when the CTA ends: the last one of every slot (the products have waited for the earlier ones)
-            for (int i = n > SLOTS ? n - SLOTS : 0; i < n; i++) (void)agn_mbar_wait(&sm.full[i % SLOTS], (i / SLOTS) & 1, p.spin);
+            for (int i = n > SLOTS ? n - SLOTS : 0; i < n; i++) (void)agn_mbar_wait(&sm.full[i % SLOTS], (i / SLOTS) & 1, DRAIN_POLLS);
         }
         __syncwarp();
     } else if (warp == 9) {
@@ -266,7 +266,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
                 if ((k += 2) >= SLOTS) { k -= SLOTS; k_turn++; }
             }
             mma_commit(&sm.drained);  // every product is done before the tensor memory goes back
-            (void)agn_mbar_wait(&sm.drained, 0, p.spin);
+            (void)agn_mbar_wait(&sm.drained, 0, DRAIN_POLLS);
         }
         __syncwarp();
     } else {

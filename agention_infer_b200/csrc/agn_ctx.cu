@@ -324,7 +324,7 @@ int32_t agn_sync(agn_ctx *ctx) {
             if (f & AGN_FLAG_OOB_EXPERT) msg += "gather_rows_by_expert: expert index out of range (those pairs are dropped); ";
             if (f & AGN_FLAG_OOB_SLOT) msg += "kv_write: position outside the cache (those tokens are not written); ";
             if (f & AGN_FLAG_OOB_ATTN) msg += "attention_kv: position or sequence outside the cache (those output rows are zero); ";
-            if (f & AGN_FLAG_BAD_SEQLENS) msg += "gated_delta_rule: sequence offsets outside the rows or out of order (they were cut); ";
+            if (f & AGN_FLAG_BAD_SEQLENS) msg += "gated_delta_rule: sequence offsets outside the rows or out of order (results are unspecified); ";
             if (msg.empty()) msg = "a kernel reported an index out of range; ";
             msg.resize(msg.size() - 2);
             return agn_fail(ctx, AGN_EOOB_ID, "%s", msg.c_str());

@@ -588,7 +588,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
             __syncwarp();
         }
         // no copy may be in flight when the CTA ends
-        if (lane == 0 && what > 0 && c > 0) (void)agn_mbar_wait(full[what], (c - 1) & 1, x.spin);
+        if (lane == 0 && what > 0 && c > 0) (void)agn_mbar_wait(full[what], (c - 1) & 1, AGN_MBAR_SPIN_LIMIT_DEFAULT);  // not cut short by the option
         if (lane == 0 && sm.gave_up) atomicOr(d.flags, AGN_FLAG_TIMEOUT);
         return;
     }

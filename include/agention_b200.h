@@ -344,7 +344,8 @@ AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
  * `attention_output` and their `_q8_0` forms, src/ops/kernels_wgpu.rs:749-980), CPU `attention_into`
  * (src/model/llama/cpu_path.rs:160-192), without the scores in memory:
  *   out[t,h] = sum_j softmax_j(scale * q[t,h] . K[s,j,h/G]) V[s,j,h/G],  j = 0 .. p,  G = n_q_heads / n_kv_heads
- * q, out: [T, n_q_heads, head_dim], f32 or f16 (the accumulation and the softmax are f32 in both); caches: n_seqs
+ * q, out: [T, n_q_heads, head_dim], f32 or f16.  Sums and softmax are f32 in both; f32 rows keep f32's precision (two-part operands of
+ * 22 bits), f16 rows round the weights and, on prompts, keys and values to f16 (which have to stay below 65504).  Caches: n_seqs
  * sequences of [max_seq_len, agn_kv_bytes_per_token(kv_dtype, n_kv_heads * head_dim)] bytes, one after the other;
  * kv_dtype AGN_F16, AGN_Q8_0 or AGN_KV_Q8_0_WORDS.  Two forms:
  *   pos != NULL: row t is the token of position p = pos[t] (device int32) of sequence s = seq[t] (device int32; NULL:
@@ -380,8 +381,8 @@ AGN_API int32_t agn_attention_kv_f16(agn_ctx *ctx, const void *q, void *out, int
  * meant to be one: g <= 0.
  * state_in [n_seqs, n_v_heads, head_k, head_v] (NULL: zeros) -> state_out, which may be the same buffer.
  * cu_seqlens: device int32 [n_seqs + 1], sequence s is the rows cu_seqlens[s] .. cu_seqlens[s+1] (none: its state is copied);
- * NULL: T / n_seqs rows each.  Rows behind the last sequence are left as they are.  Offsets outside [0, T] or out of order are cut
- * and make the next agn_sync return AGN_EOOB_ID.
+ * NULL: T / n_seqs rows each.  Rows behind the last sequence are left as they are.  Offsets outside [0, T] or out of order make the next
+ * agn_sync return AGN_EOOB_ID; what the call writes then stays inside its buffers but is otherwise unspecified.
  * head_k 64 or 128, head_v a multiple of 32 up to 256.  workspace as in agn_attention_kv_f32. */
 AGN_API int64_t agn_gated_delta_rule_workspace_bytes(int64_t T, int64_t n_seqs, int32_t n_k_heads, int32_t n_v_heads,
                                                      int32_t head_k, int32_t head_v);
