@@ -136,6 +136,20 @@ __device__ __forceinline__ void tmem_loaded(uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_load16(uint32_t at, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : TMEM_R4(r, 0), TMEM_R4(r, 4), TMEM_R4(r, 8), TMEM_R4(r, 12)
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_loaded16(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TMEM_RW4(r, 0), TMEM_RW4(r, 4), TMEM_RW4(r, 8), TMEM_RW4(r, 12)::"memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::TMEM_W4(r, 0), TMEM_W4(r, 4), TMEM_W4(r, 8),
+                 TMEM_W4(r, 12), "r"(at)
+                 : "memory");
+}
+
 template <int HD> struct PromptSmem {
     unsigned char q[2][TILE * HD * 2], kv[SLOTS][TILE * HD * 2];  // tiles in the order K0 V0 K1 V1 ..
     uint64_t q_full, full[SLOTS], free[SLOTS], s_full[2], p_full[2], o_full[2], drained;
@@ -283,69 +297,83 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         for (int j = 0; j < tiles; j++) {
             if (!(ok = wait_warp(&sm.s_full[i], j & 1))) break;
             fence_after();
-            // The scores are read twice, 32 at a time: 128 of them beside the rest do not fit the 168 registers of a thread.
+            // 32 scores at a time: while the weights of one piece are taken, the next one's maximum is found and the one after it is on its way.
             const int seen = last - (tile0 + j) * TILE;  // slots c <= seen of this tile
             const bool edge = (tile0 + j) * TILE + TILE - 1 > first_last;
             uint32_t s[2][32];
-            float x0 = -INFINITY, x1 = -INFINITY;
-            tmem_load32(s_at, s[0]);
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_loaded(s[c & 1]);
-                if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                uint32_t *w = s[c & 1];
-                if (edge) {
-#pragma unroll
-                    for (int k = 0; k < 32; k++)
-                        if (32 * c + k > seen) w[k] = 0xff800000u;
-                }
-#pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x0) : "f"(__uint_as_float(w[k])), "f"(__uint_as_float(w[k + 1])));
-                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x1) : "f"(__uint_as_float(w[k + 2])), "f"(__uint_as_float(w[k + 3])));
-                }
-            }
-            tmem_load32(s_at, s[0]);
-            const float mt = fmaxf(x0, x1) * coef;
-            const bool grow = mt > m + 8.0f;  // true at the first tile
-            if (__any_sync(0xffffffffu, grow)) {
-                const float f = grow ? ex2(m - mt) : 1.0f;
-                if (grow) m = mt;
-                l *= f;
-                if (j > 0) {
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tmem_load32(o_at + c, o);
-                        tmem_loaded(o);
-#pragma unroll
-                        for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                        tmem_store32(o_at + c, o);
-                    }
-                }
-            }
-            const float mu = m == -INFINITY ? 0.0f : m;
             float2 sum = make_float2(0.0f, 0.0f);
-            uint32_t w[32];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_loaded(s[c & 1]);
-                if (c < 3) tmem_load32(s_at + 32 * (c + 1), s[(c + 1) & 1]);
-                uint32_t *x = s[c & 1];
+            auto piece_max = [&](uint32_t *x, int c) {
                 if (edge) {
 #pragma unroll
                     for (int k = 0; k < 32; k++)
                         if (32 * c + k > seen) x[k] = 0xff800000u;
                 }
+                float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x0) : "f"(__uint_as_float(x[k])), "f"(__uint_as_float(x[k + 1])));
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(x1) : "f"(__uint_as_float(x[k + 2])), "f"(__uint_as_float(x[k + 3])));
+                }
+                return fmaxf(x0, x1) * coef;
+            };
+            // Where a row's maximum has grown by more than 2^8 (its first piece, and rarely after that), everything taken against the old one is scaled: the sums, the
+            // output of earlier tiles, the weights of this tile's first `done` pieces.
+            auto grown = [&](float mt, int done) {
+                const bool grow = mt > m + 8.0f;
+                if (!__any_sync(0xffffffffu, grow)) return;
+                const float f = grow ? ex2(m - mt) : 1.0f;
+                if (grow) m = mt;
+                l *= f;
+                sum.x *= f;
+                sum.y *= f;
+                if (j > 0) {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t o[16];
+                        tmem_load16(o_at + c, o);
+                        tmem_loaded16(o);
+#pragma unroll
+                        for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                        tmem_store16(o_at + c, o);
+                    }
+                }
+                const __half2 f2 = __floats2half2_rn(f, f);
+                for (int c = 0; c < done; c++) {
+                    uint32_t w[16];
+                    tmem_stored();
+                    tmem_load16(s_at + 16 * c, w);
+                    tmem_loaded16(w);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&w[k]), f2);
+                        w[k] = *reinterpret_cast<const uint32_t *>(&y);
+                    }
+                    tmem_store16(s_at + 16 * c, w);
+                }
+            };
+            tmem_load32(s_at, s[0]);
+            tmem_loaded(s[0]);
+            tmem_load32(s_at + 32, s[1]);
+            float mt = piece_max(s[0], 0);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                grown(mt, c);
+                if (c < 3) {
+                    tmem_loaded(s[(c + 1) & 1]);
+                    mt = piece_max(s[(c + 1) & 1], c + 1);
+                }
+                const float mu = m == -INFINITY ? 0.0f : m;
+                uint32_t *x = s[c & 1], w[16];
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
                     const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), make_float2(coef, coef), make_float2(-mu, -mu));
                     const float2 y = make_float2(ex2(e.x), ex2(e.y));
                     sum = __fadd2_rn(sum, y);
                     const __half2 h2 = __floats2half2_rn(y.x, y.y);
-                    w[16 * (c & 1) + k] = *reinterpret_cast<const uint32_t *>(&h2);
+                    w[k] = *reinterpret_cast<const uint32_t *>(&h2);
                 }
-                if (c & 1) tmem_store32(s_at + 16 * (c - 1), w);  // over scores that have been read
+                tmem_store16(s_at + 16 * c, w);  // over scores that have been read
+                if (c < 2) tmem_load32(s_at + 32 * (c + 2), s[c & 1]);
             }
             l += sum.x + sum.y;
             tmem_stored();
