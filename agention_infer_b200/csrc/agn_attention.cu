@@ -170,8 +170,8 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     const bool chunk = !pos && !prompt && chunk_fits(rows, n_q, n_kv);
     const int sms = ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS;
     const int64_t end = (int64_t)pos_start + rows;
-    const int64_t need = prompt ? agn_attention_prompt_workspace(end, rows, n_q, n_kv, hd, sms)
-                         : chunk ? agn_attention_chunk_workspace(end, rows, n_q, n_kv, hd, sms) : attn_workspace(rows, n_q, hd);
+    const int64_t need = prompt ? agn_attention_prompt_workspace(end, rows, n_q, n_kv, hd, sms, false)
+                         : chunk ? agn_attention_chunk_workspace(end, rows, n_q, n_kv, hd, sms, false) : attn_workspace(rows, n_q, hd);
     if (need > 0 && (!workspace || (int64_t)workspace_bytes < need || !agn_aligned16(workspace)))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: needs %lld bytes of 16-byte aligned workspace", (long long)need);
     AGN_CUDA(ctx, cudaSetDevice(ctx->device));
@@ -211,9 +211,9 @@ extern "C" int64_t agn_attention_kv_workspace_bytes(int64_t T, int32_t n_q_heads
     int64_t need = attn_workspace(T, n_q_heads, head_dim);
     if (has_pos) return need;
     // for whichever activation type the rows have, and for rows that end anywhere in the cache
-    const int64_t chunk = chunk_fits(T, n_q_heads, n_kv_heads) ? agn_attention_chunk_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS) : 0;
+    const int64_t chunk = chunk_fits(T, n_q_heads, n_kv_heads) ? agn_attention_chunk_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS, true) : 0;
     const int64_t prompt = agn_attention_prompt_fits(T, n_q_heads, n_kv_heads, head_dim)
-                               ? agn_attention_prompt_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS) : 0;
+                               ? agn_attention_prompt_workspace(max_seq_len, T, n_q_heads, n_kv_heads, head_dim, ATTN_MAX_SMS, true) : 0;
     if (chunk > need) need = chunk;
     return prompt > need ? prompt : need;
 }

@@ -38,17 +38,27 @@ inline int attn_splits(int64_t ctas, int64_t tiles, double tile_us, int64_t rows
     }
     return best;
 }
+// A bound on that number for rows that end anywhere in `tiles` tiles: splits have to save more than they cost.  (The number itself does not only grow with the tiles:
+// 10 tiles may go to 10 CTAs, 12 tiles to 6.)
+inline int attn_splits_most(int64_t ctas, int64_t tiles, double tile_us, int64_t rows, int hd, int sms) {
+    int64_t n = sms / (ctas > 0 ? ctas : 1);
+    const double paid = (tiles * tile_us - 6.0) / ((double)rows * (hd + 4) * 8 / 2.5e6);
+    if (n > tiles) n = tiles;
+    if ((double)n > paid) n = paid > 1.0 ? (int64_t)paid : 1;
+    return n > 1 ? (int)n : 1;
+}
 inline int64_t attn_part_bytes(int splits, int64_t T, int n_q, int hd) { return splits > 1 ? (int64_t)splits * T * n_q * (hd + 4) * 4 : 0; }
 // odd: [n_kv][odd_tiles] flags of groups of `group` slots whose values are not all finite (they were taken as 0), or null: look at every slot.
 int32_t agn_attention_join(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, AttnSplit split, const int *odd, int64_t odd_tiles, int group);
 
 // Rows of a prompt in f16 on the tensor cores (agn_attention_prompt.cu), where that form covers the call.
 bool agn_attention_prompt_fits(int64_t T, int n_q, int n_kv, int hd);
-int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms);
+// `anywhere`: enough for rows that end at any slot up to that one; otherwise what rows that end there take.
+int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere);
 int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace);
 
 // Rows of a prompt that the form above does not cover: f32 rows, other head sizes (agn_attention_chunk.cu).
-int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms);
+int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere);
 int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, void *workspace);
 
 constexpr int KV_F16 = 0, KV_Q8 = 1, KV_WORDS = 2;

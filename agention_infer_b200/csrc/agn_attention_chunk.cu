@@ -348,10 +348,10 @@ struct ChunkLayout {
     int row_tiles, splits;
     int64_t odd, bytes;
 };
-ChunkLayout chunk_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) {
+ChunkLayout chunk_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere = false) {
     ChunkLayout l;
     l.row_tiles = (int)((T * (n_q / n_kv) + chunk_rows(hd) - 1) / chunk_rows(hd));
-    l.splits = attn_splits((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 0.5 + 0.045 * hd, T * n_q, hd, sms);
+    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 0.5 + 0.045 * hd, T * n_q, hd, sms);
     l.odd = attn_part_bytes(l.splits, T, n_q, hd);
     l.bytes = l.splits > 1 ? l.odd + (n_kv * 4 + 15) / 16 * 16 : 0;
     return l;
@@ -389,7 +389,9 @@ template <int KV> int32_t launch_chunk_kv(agn_ctx *ctx, const DecodeArgs &d, con
 
 }  // namespace
 
-int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) { return chunk_layout(slots, T, n_q, n_kv, hd, sms).bytes; }
+int64_t agn_attention_chunk_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere) {
+    return chunk_layout(slots, T, n_q, n_kv, hd, sms, anywhere).bytes;
+}
 
 int32_t agn_attention_chunk(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, int act16, void *workspace) {
     const ChunkLayout l = chunk_layout((int64_t)a.pos_start + a.T, a.T, a.n_q, a.n_kv, a.hd, ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS);

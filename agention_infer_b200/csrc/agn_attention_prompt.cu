@@ -481,19 +481,21 @@ struct PromptLayout {
     int64_t image, odd, part, bytes;  // bytes of an image set; byte offsets
     int row_tiles, splits;
 };
-PromptLayout prompt_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) {
+PromptLayout prompt_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere = false) {
     PromptLayout l;
     l.image = image_bytes(slots, n_kv, hd);
     l.odd = 2 * l.image;
     l.part = l.odd + (odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;
     l.row_tiles = (int)((T * (n_q / n_kv) + 2 * TILE - 1) / (2 * TILE));
-    l.splits = attn_splits((int64_t)l.row_tiles * n_kv, (slots + TILE - 1) / TILE, 2.4, T * n_q, hd, sms);
+    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + TILE - 1) / TILE, 2.4, T * n_q, hd, sms);
     l.bytes = l.part + attn_part_bytes(l.splits, T, n_q, hd);
     return l;
 }
 }  // namespace
 
-int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms) { return prompt_layout(slots, T, n_q, n_kv, hd, sms).bytes; }
+int64_t agn_attention_prompt_workspace(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere) {
+    return prompt_layout(slots, T, n_q, n_kv, hd, sms, anywhere).bytes;
+}
 
 int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, void *workspace) {
     PromptArgs p;

@@ -357,7 +357,7 @@ AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
  * head_dim: a multiple of 32 up to 256; scale > 0 and finite; q and out 16-byte aligned and not the same buffer.
  * workspace: at least agn_attention_kv_workspace_bytes(...) bytes of device memory, 16-byte aligned, whose contents
  * need not be kept between calls; calls that can overlap on the GPU need a workspace each.  NULL if that is 0.
- * The function takes the call's own sizes (has_pos: pos != NULL), needs no context and returns 0 for sizes the op refuses. */
+ * The function takes the call's own sizes (has_pos: pos != NULL; any pos_start), needs no context and returns 0 for sizes the op refuses. */
 AGN_API int64_t agn_attention_kv_workspace_bytes(int64_t T, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
                                                  int64_t max_seq_len, int32_t has_pos);
 AGN_API int32_t agn_attention_kv_f32(agn_ctx *ctx, const float *q, float *out, int32_t kv_dtype, const void *k_cache,

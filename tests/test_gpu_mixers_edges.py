@@ -278,3 +278,18 @@ def test_layer_of_each_kind(backend):
         wy = ref.gated_norm(got.reshape(-1, 128), z, be.read(gates, np.float32, (128,)), 1e-6)
         assert np.all(np.abs(y - wy) <= 1e-5 * np.abs(wy).max(-1, keepdims=True))
         at += T
+
+
+@pytest.mark.parametrize("T,nq,nkv,hd,slots", [(277, 16, 2, 64, 600), (250, 7, 1, 128, 900), (38, 4, 1, 64, 5000), (64, 4, 1, 256, 3000)])
+def test_one_workspace_for_rows_that_end_anywhere(backend, T, nq, nkv, hd, slots):
+    rng = np.random.default_rng(T)
+    c = Cache(backend, rng, "q8_0", 1, slots, nkv, hd, [slots])
+    ws = backend.empty(max(16, backend.attention_kv_workspace_bytes(T, nq, nkv, hd, slots, False)))
+    k, v = c.values(0, slots)
+    for act in ("f32", "f16"):
+        q = rng.standard_normal((T, nq, hd)).astype(np_act(act))
+        dq, out = backend.upload(q), backend.empty(q.nbytes)
+        for start in list(range(0, slots - T, max(64, (slots - T) // 16 // 64 * 64))) + [slots - T]:
+            backend.launch_attention_kv(dq, c.bufs[0], c.bufs[1], c.kv, T, nq, nkv, hd, slots, pos_start=start, act_dtype=ACT[act], out=out, workspace=ws)
+        want, mag = ref.attention(q, k, v, [start + t for t in range(T)], hd ** -0.5)
+        close(backend.read(out, np_act(act), q.shape), want, mag, q, k, slots, hd ** -0.5, act)

@@ -33,3 +33,10 @@ def test_workspace_sizes_are_not_negative(lib):
         for n in (1, 3, 64):
             assert lib.agn_gated_delta_rule_workspace_bytes(T, n, 16, 32, 128, 128) >= 0
     assert lib.agn_gated_delta_rule_workspace_bytes(10, 1, 3, 4, 128, 128) == 0
+
+
+@pytest.mark.parametrize("T,nq,nkv,hd", [(277, 16, 2, 64), (250, 7, 1, 128), (38, 4, 1, 64), (556, 14, 2, 64), (64, 4, 1, 256), (129, 8, 1, 96)])
+def test_a_longer_cache_never_asks_for_less_workspace(lib, T, nq, nkv, hd):
+    """Rows may end anywhere in the cache, so that a size is enough for every shorter one."""
+    sizes = [lib.agn_attention_kv_workspace_bytes(T, nq, nkv, hd, slots, 0) for slots in range(T, T + 6000, 16)]
+    assert all(b >= a for a, b in zip(sizes, sizes[1:]))
