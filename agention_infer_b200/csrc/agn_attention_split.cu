@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_split_join_kernel(const 
     for (int x = lane; x < split.splits; x += 32) {
         const float c = ex2(weight[warp][x] - (M == -INFINITY ? 0.0f : M));
         weight[warp][x] = c;
-        if (c != 0.0f) L = __fmaf_rn(c, part[x * stride + hd + 1], L);
+        L = __fmaf_rn(c, part[x * stride + hd + 1], L);  // NaN where all of a share's scores are: its maximum is still -inf
     }
     L = agn_warp_sum(L);
     __syncwarp();

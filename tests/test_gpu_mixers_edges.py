@@ -293,3 +293,22 @@ def test_one_workspace_for_rows_that_end_anywhere(backend, T, nq, nkv, hd, slots
             backend.launch_attention_kv(dq, c.bufs[0], c.bufs[1], c.kv, T, nq, nkv, hd, slots, pos_start=start, act_dtype=ACT[act], out=out, workspace=ws)
         want, mag = ref.attention(q, k, v, [start + t for t in range(T)], hd ** -0.5)
         close(backend.read(out, np_act(act), q.shape), want, mag, q, k, slots, hd ** -0.5, act)
+
+
+@pytest.mark.parametrize("form", ["f32", "f16", "f32 rows of their own", "f16 rows of their own"])
+def test_keys_of_nan_in_the_last_share_alone(backend, form):
+    """Every score that a row has in one of its shares is NaN: so is its result, in that head alone."""
+    rng = np.random.default_rng(8)
+    act = form[:3]
+    T, start, nq, nkv, hd = 40, 2048, 4, 2, 64
+    k, v = (rng.standard_normal((start + T, nkv, hd)).astype(np.float16) for _ in range(2))
+    k[start:, 0] = np.nan
+    q = rng.standard_normal((T, nq, hd)).astype(np_act(act))
+    bufs = [backend.upload(x) for x in (q, k, v)]
+    kw = dict(pos=backend.upload(np.arange(start, start + T, dtype=np.int32))) if "own" in form else dict(pos_start=start)
+    out = backend.launch_attention_kv(bufs[0], bufs[1], bufs[2], AGN_F16, T, nq, nkv, hd, start + T, act_dtype=ACT[act], **kw)
+    got = backend.read(out, np_act(act), q.shape)
+    assert np.isnan(got[:, :2]).all()
+    k, v = k.astype(np.float64), v.astype(np.float64)
+    want, mag = ref.attention(q[:, 2:], k[:, 1:], v[:, 1:], [start + t for t in range(T)], hd ** -0.5)
+    close(got[:, 2:], want, mag, q[:, 2:], k[:, 1:], start + T, hd ** -0.5, act)
