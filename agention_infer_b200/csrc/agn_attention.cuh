@@ -92,7 +92,7 @@ template <typename Look> __device__ __forceinline__ float odd_value(const AttnAr
     bool up = false, down = false;
     for (int s = 0; s <= last; s++) {
         if (!look(s)) {
-            s |= group - 1;
+            s += group - 1 - s % group;
             continue;
         }
         const unsigned char *row = a.v_cache + (int64_t)s * a.bytes_per_token;

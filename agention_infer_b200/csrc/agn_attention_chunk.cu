@@ -371,7 +371,7 @@ template <int KV, int NB> int32_t launch_chunk(agn_ctx *ctx, const DecodeArgs &d
     agn_launch(ctx, attn_chunk_kernel<KV, NB>, dim3((unsigned)((int64_t)l.row_tiles * d.a.n_kv * l.splits)), dim3(C::THREADS), sizeof(ChunkTiles<NB>), d, split, l.row_tiles, odd);
     AGN_LAUNCHED(ctx, "attention_kv_chunk");
     // one flag per KV head: a group of all slots
-    return l.splits > 1 ? agn_attention_join(ctx, d.a, AGN_F16, d.act16, split, odd, 1, 1 << 30) : AGN_OK;
+    return l.splits > 1 ? agn_attention_join(ctx, d.a, AGN_F16, d.act16, split, odd, 1, 0x7fffffff) : AGN_OK;
 }
 
 template <int KV> int32_t launch_chunk_kv(agn_ctx *ctx, const DecodeArgs &d, const ChunkLayout &l, void *workspace) {
