@@ -1,6 +1,6 @@
 """B200-native (sm_100a) CUDA backend for the layer-op hot path of the gguf-rs engine:
-RMSNorm, rotary embedding, SwiGLU silu*mul, row softmax and quantised-embedding
-get_rows, behind the C ABI of include/agention_b200.h.
+RMSNorm, rotary embedding, SwiGLU silu*mul, row softmax, quantised-embedding
+get_rows, the KV cache with the attention over it and the gated delta rule, behind the C ABI of include/agention_b200.h.
 
 Importing the package does not load the CUDA library; constructing `CudaBackend`
 does, and fails loudly when the library or a GPU is missing (no fallback path).
