@@ -6,7 +6,7 @@
 // bytes (exact in f16), weights times the block scale as hi + lo tf32 against the cached bytes.  A CTA takes 16 rows per warp of one KV head - row r
 // is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory once for all warps,
 // the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 36.7 us (128 CTAs, eight tiles one after the other); 2048 tokens of 28/4 heads of 128:
-// 400 us, 150 TFLOP/s.  Blocks of four warps, two to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
+// 374 us, 80 TFLOP/s.  Blocks of four warps, two to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
 #include <math.h>
 
 #include "agn_attention_decode.cuh"
@@ -28,38 +28,30 @@ template <int NB> struct ChunkTiles {
     int odd;
 };
 
-// One block of 32 values on its way from the cache: 16 words of f16, or 8 words of bytes and a scale.
+// One block of 32 values on its way from the cache: 16 words of f16, or 8 words of bytes and a scale.  q8_0 as the words lie in memory: a block that begins at a
+// multiple of 4 is 8 words (scale and bytes) and the last two bytes, one that does not is the scale and 8 words.  Taking them apart is left to place_block, since a
+// use of a loaded word here would wait for it (2048 rows of 28/4 heads of 128: 397 us, so 374).
 template <int KV> struct Block {
     uint32_t w[KV == KV_F16 ? 16 : 8];
-    float scale;
+    uint32_t more;  // q8_0: the two bytes outside the words; words: the scale
 };
 
 template <int KV> __device__ __forceinline__ void fetch_block(Block<KV> &x, const unsigned char *p, bool there) {
 #pragma unroll
     for (int i = 0; i < (KV == KV_F16 ? 16 : 8); i++) x.w[i] = KV == KV_WORDS ? 0x80808080u : 0u;
-    x.scale = 0.0f;
+    x.more = 0;
     if (!there) return;
     const uint32_t *w = reinterpret_cast<const uint32_t *>(p);
     if (KV == KV_WORDS) {
-        x.scale = __uint_as_float(w[0]);
+        x.more = w[0];
 #pragma unroll
         for (int i = 0; i < 8; i++) x.w[i] = w[i + 1];
     } else if (KV == KV_Q8) {
-        x.scale = __half2float(*reinterpret_cast<const __half *>(p));
-        if (reinterpret_cast<uintptr_t>(p) & 2) {
-            const uint32_t *d = reinterpret_cast<const uint32_t *>(p + 2);
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 2);
+        const uint32_t *d = reinterpret_cast<const uint32_t *>(p + off);
 #pragma unroll
-            for (int i = 0; i < 8; i++) x.w[i] = d[i];
-        } else {  // the bytes begin in the middle of a word and end in the middle of one
-            uint32_t a = w[0];
-#pragma unroll
-            for (int i = 0; i < 7; i++) {
-                const uint32_t b = w[i + 1];
-                x.w[i] = __funnelshift_r(a, b, 16);
-                a = b;
-            }
-            x.w[7] = __funnelshift_r(a, *reinterpret_cast<const uint16_t *>(p + 32), 16);
-        }
+        for (int i = 0; i < 8; i++) x.w[i] = d[i];
+        x.more = *reinterpret_cast<const uint16_t *>(p + (off ? 0 : 32));
     } else if (!(reinterpret_cast<uintptr_t>(p) & 15)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -72,9 +64,20 @@ template <int KV> __device__ __forceinline__ void fetch_block(Block<KV> &x, cons
     }
 }
 
-// To 32 f16 values; returns whether one of an f16 block is not finite (it becomes 0 where `clean`).
-template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x, __half *to, bool clean) {
+// To 32 f16 values and the block's scale; from: what was fetched (its address, of a q8_0 block); returns whether one of an f16 block is not finite (it becomes 0 where `clean`).
+template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x, const unsigned char *from, __half *to, float *scale, bool clean) {
     bool odd = false;
+    uint32_t bytes[8];
+    if (KV == KV_WORDS) {
+        *scale = __uint_as_float(x.more);
+#pragma unroll
+        for (int i = 0; i < 8; i++) bytes[i] = x.w[i];
+    } else if (KV == KV_Q8) {
+        const bool apart = reinterpret_cast<uintptr_t>(from) & 2;  // the scale lies before the words, not in the first one
+        *scale = __half2float(__ushort_as_half((unsigned short)(apart ? x.more : x.w[0])));
+#pragma unroll
+        for (int i = 0; i < 8; i++) bytes[i] = apart ? x.w[i] : __funnelshift_r(x.w[i], i < 7 ? x.w[i < 7 ? i + 1 : 7] : x.more, 16);
+    }
     uint4 *dst = reinterpret_cast<uint4 *>(to);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -90,7 +93,7 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
                     if (o1) h[c] &= 0x0000ffffu;
                 }
             } else {
-                const uint32_t u = offset_bytes<KV>(x.w[2 * i + (c >> 1)]);
+                const uint32_t u = offset_bytes<KV>(bytes[2 * i + (c >> 1)]);
                 h[c] = bytes_to_half2(u, c & 1 ? 0x4342 : 0x4140);
             }
         }
@@ -118,17 +121,18 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     const int per_share = (seen_tiles + split.splits - 1) / split.splits, tile0 = min(share * per_share, seen_tiles), tiles = min(seen_tiles, tile0 + per_share);  // tile0 .. tiles - 1
     if (tid == 0) sm.odd = 0;
 
+    auto block_at = [&](int n, int tile) {
+        return (n < SL * NB ? a.k_cache : a.v_cache) + (int64_t)(tile * SL + n / NB % SL) * a.bytes_per_token + (kvh * NB + n % NB) * F::BYTES;
+    };
     auto fetch = [&](Block<KV> &x, int i, int tile) {
-        const int n = tid + i * C::THREADS, b = n % NB, slot = tile * SL + n / NB % SL;
-        const unsigned char *cache = n < SL * NB ? a.k_cache : a.v_cache;
-        fetch_block<KV>(x, cache + (int64_t)slot * a.bytes_per_token + (kvh * NB + b) * F::BYTES, n < 2 * SL * NB && slot < end);
+        const int n = tid + i * C::THREADS;
+        fetch_block<KV>(x, block_at(n, tile), n < 2 * SL * NB && tile * SL + n / NB % SL < end);
     };
     auto place = [&](const Block<KV> &x, int i, int tile) {
         const int n = tid + i * C::THREADS, b = n % NB, slot = n / NB % SL;
         const bool is_k = n < SL * NB;
         if (n >= 2 * SL * NB) return;
-        const bool odd = place_block<KV>(x, (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, !is_k);
-        if (KV != KV_F16) (is_k ? sm.ks : sm.vs)[tile & 1][slot][b] = x.scale;
+        const bool odd = place_block<KV>(x, block_at(n, tile), (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, &(is_k ? sm.ks : sm.vs)[tile & 1][slot][b], !is_k);
         if (KV == KV_F16 && odd) sm.odd = 1;
     };
     constexpr int HELD = NB <= 4 ? C::BLOCKS : 1;  // blocks that wait in registers while a tile is worked on; larger heads have none left for them
