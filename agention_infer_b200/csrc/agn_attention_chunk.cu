@@ -1,9 +1,10 @@
 // Attention of a prompt's rows (consecutive positions of one sequence) over the KV cache, to f32's precision: f32 rows, and f16 rows of head sizes
 // that the tensor-memory form (agn_attention_prompt.cu) does not cover.
 //
-// Bound by the matrix units: per 16 rows, 8 slots and 32 dims 4 products m16n8k16 (f16) for the scores and 8 m16n8k8 (tf32) for the output, which caps the
-// kernel near 190 TFLOP/s for heads of 128.  Precision comes from two-part operands as in the decode kernel: queries as hi + lo f16 against the cached
-// bytes (exact in f16), weights times the block scale as hi + lo tf32 against the cached bytes.  A CTA takes 16 rows per warp of one KV head - row r
+// Bound by the matrix units: per 16 rows, 16 slots and 32 dims 8 products m16n8k16 (f16) for the scores and 8 for the output, which caps the kernel near 276
+// TFLOP/s; with eight warps an SM they are busy 40 % of the time.  Precision comes from two-part operands as in the decode kernel: queries as hi + lo f16 against the cached
+// bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached
+// bytes (397 -> 322 us for 2048 rows of 28/4 heads of 128 against tf32 parts and blocks taken apart at once).  A CTA takes 16 rows per warp of one KV head - row r
 // is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory once for all warps,
 // the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 36.7 us (128 CTAs, eight tiles one after the other); 2048 tokens of 28/4 heads of 128:
 // 374 us, 80 TFLOP/s.  Blocks of four warps, two to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
@@ -25,6 +26,7 @@ template <int NB> struct ChunkTiles {
     __half q[2][C::ROWS * C::ROW];  // hi, lo
     __half k[2][SL * C::ROW], v[2][SL * C::ROW];
     float ks[2][SL][NB], vs[2][SL][NB], coef[C::ROWS];
+    uint32_t most[3][NB], least[3][NB];  // of the scales of a tile's values that are not 0, as bits of their magnitudes
     int odd;
 };
 
@@ -102,6 +104,19 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
     return odd;
 }
 
+// Weights times scales as two f16 parts, V_UP times: at most 2^15 (weights reach 2^8, scales are brought below 2).  The lower part's smallest step, 2^-24, is then 2^-30
+// of a full weight; scales that lie further apart than 2^6 take the tf32 products, whose parts have f32's range.
+constexpr float V_UP = 64.0f;
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
 }
@@ -120,6 +135,10 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     const int last_row = min(r0 + C::ROWS, rows) - 1, end = a.pos_start + last_row / G + 1, seen_tiles = (end + SL - 1) / SL;
     const int per_share = (seen_tiles + split.splits - 1) / split.splits, tile0 = min(share * per_share, seen_tiles), tiles = min(seen_tiles, tile0 + per_share);  // tile0 .. tiles - 1
     if (tid == 0) sm.odd = 0;
+    if (KV != KV_F16 && tid < 3 * NB) {
+        sm.most[tid / NB][tid % NB] = 0;
+        sm.least[tid / NB][tid % NB] = 0x7f800000u;
+    }
 
     auto block_at = [&](int n, int tile) {
         return (n < SL * NB ? a.k_cache : a.v_cache) + (int64_t)(tile * SL + n / NB % SL) * a.bytes_per_token + (kvh * NB + n % NB) * F::BYTES;
@@ -134,6 +153,13 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
         if (n >= 2 * SL * NB) return;
         const bool odd = place_block<KV>(x, block_at(n, tile), (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, &(is_k ? sm.ks : sm.vs)[tile & 1][slot][b], !is_k);
         if (KV == KV_F16 && odd) sm.odd = 1;
+        if (KV != KV_F16 && !is_k) {
+            const uint32_t size = __float_as_uint(sm.vs[tile & 1][slot][b]) & 0x7fffffffu;
+            if (size) {
+                atomicMax(&sm.most[tile % 3][b], size);
+                atomicMin(&sm.least[tile % 3][b], size);
+            }
+        }
     };
     constexpr int HELD = NB <= 4 ? C::BLOCKS : 1;  // blocks that wait in registers while a tile is worked on; larger heads have none left for them
     Block<KV> next[HELD];
@@ -187,6 +213,10 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     for (int i = 0; i < 4 * NB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
     for (int tile = tile0; tile < tiles; tile++) {
+        if (KV != KV_F16 && tid < NB) {  // of the tile before this one and of the one after the next
+            sm.most[(tile + 2) % 3][tid] = 0;
+            sm.least[(tile + 2) % 3][tid] = 0x7f800000u;
+        }
         if (tile + 1 < tiles) fetch_tile(tile + 1);
         if (tile * SL <= warp_last) {  // a warp whose rows see none of it waits for the others
             const int buf = tile & 1;
@@ -259,41 +289,70 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                     s[n][i] = ex2(__fmaf_rn(s[n][i], coef[i >> 1], -mu[i >> 1]));
                     l[i >> 1] += s[n][i];
                 }
-            // ---- O += P V; the sums of a tile in the matrix unit (whose adder cuts), the running ones by rounded additions
+            // ---- O += P V; the sums of a tile in the matrix unit (whose adder cuts), the running ones by rounded additions.  Dims 8 c + 2 t4 (+ 1) of the block in o[4 b + c].
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                float acc[4][4];
+                float acc[4][4], down = 1.0f / V_UP;
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
+                const uint32_t most = KV == KV_F16 ? 0u : sm.most[tile % 3][b], least = KV == KV_F16 ? 0u : sm.least[tile % 3][b];
+                if (KV == KV_F16 || (most < 0x7f000000u && (most >> 23) <= (least >> 23) + 6)) {
+                    float fold = V_UP;
+                    if (KV != KV_F16) {  // the largest scale to [1, 2)
+                        const uint32_t e = max(most >> 23, 7u);
+                        fold = __uint_as_float((254 + 6 - e) << 23);
+                        down = __uint_as_float((e - 6) << 23);
+                    }
 #pragma unroll
-                for (int n = 0; n < SL / 8; n++) {
-                    float hi[4], lo[4], w[4] = {s[n][0], s[n][1], s[n][2], s[n][3]};
-                    if (KV != KV_F16) {
-                        const float s0 = sm.vs[buf][8 * n + 2 * t4][b], s1 = sm.vs[buf][8 * n + 2 * t4 + 1][b];
-                        w[0] *= s0; w[1] *= s1; w[2] *= s0; w[3] *= s1;
-                        if (edge) {  // a scale that is not finite, in a slot that the row does not see
+                    for (int n = 0; n < SL / 8; n += 2) {
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (tile * SL + 8 * n + 2 * t4 + (i & 1) > lim[i >> 1]) w[i] = 0.0f;
+                        for (int u = 0; u < 2; u++) {
+                            float f0 = fold, f1 = fold;
+                            if (KV != KV_F16) {
+                                const float2 f = make_float2(sm.vs[buf][8 * (n + u) + 2 * t4][b], sm.vs[buf][8 * (n + u) + 2 * t4 + 1][b]);
+                                f0 *= f.x;
+                                f1 *= f.y;
+                            }
+                            split_half2(s[n + u][0] * f0, s[n + u][1] * f1, hi[2 * u], lo[2 * u]);
+                            split_half2(s[n + u][2] * f0, s[n + u][3] * f1, hi[2 * u + 1], lo[2 * u + 1]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 4; c += 2) {
+                            uint32_t v[4];
+                            ldsm4t(v, sm.v[buf] + (8 * n + (lane & 15)) * ROW + b * 32 + c * 8 + (lane >> 4) * 8);
+                            mma_f16(acc[c], hi, v[0], v[1]);
+                            mma_f16(acc[c + 1], hi, v[2], v[3]);
+                            mma_f16(acc[c], lo, v[0], v[1]);
+                            mma_f16(acc[c + 1], lo, v[2], v[3]);
                         }
                     }
+                } else {
+                    down = 1.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        hi[i] = __uint_as_float(__float_as_uint(w[i]) & 0xffffe000u);
-                        lo[i] = fminf(w[i] - hi[i], 1e35f);  // with an infinite scale not inf - inf
+                    for (int n = 0; n < SL / 8; n++) {
+                        const float s0 = sm.vs[buf][8 * n + 2 * t4][b], s1 = sm.vs[buf][8 * n + 2 * t4 + 1][b];
+                        float hi[4], lo[4], w[4] = {s[n][0] * s0, s[n][1] * s1, s[n][2] * s0, s[n][3] * s1};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            // a scale that is not finite, in a slot that the row does not see
+                            if (edge && tile * SL + 8 * n + 2 * t4 + (i & 1) > lim[i >> 1]) w[i] = 0.0f;
+                            hi[i] = __uint_as_float(__float_as_uint(w[i]) & 0xffffe000u);
+                            lo[i] = fminf(w[i] - hi[i], 1e35f);  // with an infinite scale not inf - inf
+                        }
+                        const __half *v = sm.v[buf] + (8 * n + 2 * t4) * ROW + b * 32 + g;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const float e0 = __half2float(v[8 * c]), e1 = __half2float(v[8 * c + ROW]);
+                            mma_tf32(acc[c], hi[0], hi[2], hi[1], hi[3], e0, e1);
+                            mma_tf32(acc[c], lo[0], lo[2], lo[1], lo[3], e0, e1);
+                        }
                     }
-                    const uint2 x0 = *reinterpret_cast<const uint2 *>(sm.v[buf] + (8 * n + 2 * t4) * ROW + b * 32 + 4 * g);
-                    const uint2 x1 = *reinterpret_cast<const uint2 *>(sm.v[buf] + (8 * n + 2 * t4 + 1) * ROW + b * 32 + 4 * g);
-                    const float2 u0 = __half22float2(*reinterpret_cast<const __half2 *>(&x0.x)), u1 = __half22float2(*reinterpret_cast<const __half2 *>(&x0.y));
-                    const float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&x1.x)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&x1.y));
-                    const float e0[4] = {u0.x, u0.y, u1.x, u1.y}, e1[4] = {v0.x, v0.y, v1.x, v1.y};
-#pragma unroll
-                    for (int c = 0; c < 4; c++) mma_tf32(acc[c], hi[0], hi[2], hi[1], hi[3], e0[c], e1[c]);
-#pragma unroll
-                    for (int c = 0; c < 4; c++) mma_tf32(acc[c], lo[0], lo[2], lo[1], lo[3], e0[c], e1[c]);
                 }
 #pragma unroll
-                for (int c = 0; c < 4; c++) add4(o[4 * b + c], acc[c]);
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[4 * b + c][i] = __fmaf_rn(acc[c][i], down, o[4 * b + c][i]);
             }
         }
         if (tile + 1 < tiles) place_tile(tile + 1);
@@ -312,18 +371,21 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
             if (t4 == 0) *reinterpret_cast<float2 *>(to + HD) = make_float2(m[i], l[i]);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                *reinterpret_cast<float4 *>(to + b * 32 + 8 * t4) = make_float4(o[4 * b][2 * i], o[4 * b + 1][2 * i], o[4 * b + 2][2 * i], o[4 * b + 3][2 * i]);
-                *reinterpret_cast<float4 *>(to + b * 32 + 8 * t4 + 4) = make_float4(o[4 * b][2 * i + 1], o[4 * b + 1][2 * i + 1], o[4 * b + 2][2 * i + 1], o[4 * b + 3][2 * i + 1]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) *reinterpret_cast<float2 *>(to + b * 32 + 8 * c + 2 * t4) = make_float2(o[4 * b + c][2 * i], o[4 * b + c][2 * i + 1]);
             }
             continue;
         }
         const float inv = m[i] == -INFINITY ? NAN : 1.0f / l[i];  // all scores -inf: 0 / 0
 #pragma unroll
-        for (int b = 0; b < NB; b++) {  // dims 8 t4 .. 8 t4 + 7 of the block
-            store_act4(d, at, b * 8 + 2 * t4, make_float4(o[4 * b][2 * i] * inv, o[4 * b + 1][2 * i] * inv, o[4 * b + 2][2 * i] * inv, o[4 * b + 3][2 * i] * inv));
-            store_act4(d, at, b * 8 + 2 * t4 + 1,
-                       make_float4(o[4 * b][2 * i + 1] * inv, o[4 * b + 1][2 * i + 1] * inv, o[4 * b + 2][2 * i + 1] * inv, o[4 * b + 3][2 * i + 1] * inv));
-        }
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float2 y = make_float2(o[4 * b + c][2 * i] * inv, o[4 * b + c][2 * i + 1] * inv);
+                const int64_t x = at + b * 32 + 8 * c + 2 * t4;
+                if (d.act16) *reinterpret_cast<__half2 *>(static_cast<__half *>(a.out) + x) = __floats2half2_rn(y.x, y.y);
+                else *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + x) = y;
+            }
     }
     if (KV == KV_F16) {  // rare: V held values that are not finite
         __syncthreads();

@@ -312,3 +312,22 @@ def test_keys_of_nan_in_the_last_share_alone(backend, form):
     k, v = k.astype(np.float64), v.astype(np.float64)
     want, mag = ref.attention(q[:, 2:], k[:, 1:], v[:, 1:], [start + t for t in range(T)], hd ** -0.5)
     close(got[:, 2:], want, mag, q[:, 2:], k[:, 1:], start + T, hd ** -0.5, act)
+
+
+@pytest.mark.parametrize("kv,low,high", [("q8_0", -4, 2), ("words", -6, 6), ("words", 36, 37), ("words", -37, -36), ("words", 0, 1), ("f16", -4, 3)])
+@pytest.mark.parametrize("hd", [64, 160])
+def test_values_of_very_different_sizes(backend, kv, low, high, hd):
+    """V's magnitude changes from slot to slot by up to twelve orders, at both ends of f32's range too; some rows see only small ones."""
+    rng = np.random.default_rng(hd + high)
+    T, start, nq, nkv = 50, 150, 6, 2
+    slots = start + T
+    c = Cache(backend, rng, kv, 1, slots, nkv, hd, [slots])
+    v = rng.standard_normal((slots, nkv * hd)) * 10.0 ** rng.uniform(low, high, (slots, 1))
+    v[start + 20] *= 10.0 if high > 30 else 1.0
+    k = rng.standard_normal((slots, nkv * hd)).astype(np.float32)
+    backend.kv_write(c.kv, backend.upload(k), backend.upload(v.astype(np.float32)), c.bufs[0], c.bufs[1], slots, nkv * hd, None, slots)
+    q = rng.standard_normal((T, nq, hd)).astype(np.float32)
+    k, v = c.values(0, slots)
+    want, mag = ref.attention(q, k, v, [start + t for t in range(T)], hd ** -0.5)
+    # a row's error is counted against its own weights' sum of |v|: what is small beside a value that the row does not see stays exact
+    close(run_chunk(backend, c, q, start, "f32"), want, mag, q, k, slots, hd ** -0.5, "f32")
