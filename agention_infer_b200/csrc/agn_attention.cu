@@ -139,9 +139,9 @@ int64_t attn_workspace(int64_t T, int n_q, int hd) {
     return T > 0 && T <= ATTN_MAX_SPLIT_ROWS ? (int64_t)2 * 2 * ATTN_MAX_SMS * n_q * (hd + 4) * 4 : 0;
 }
 
-// Few rows of one sequence are quicker as single rows (f32, 28/4 heads of 128, single rows / chunks, us: behind 8000 q8_0 slots 8 rows 38 / 49, 16 rows 55 / 51, 32 rows 92 / 66;
-// behind 1000 slots 16 rows 23 / 25, 32 rows 32 / 26).
-constexpr int CHUNK_MIN_TOKENS = 16;
+// Few rows of one sequence are quicker as single rows (f32 over q8_0, single rows / chunks, us: 28/4 heads of 128 behind 8000 slots 8 rows 35 / 37, 12 rows 42 / 39, behind
+// 1000 slots 12 rows 18 / 19; 32/8 heads of 128 behind 8000 slots 8 rows 50 / 50, 12 rows 67 / 51).
+constexpr int CHUNK_MIN_TOKENS = 12;
 bool chunk_fits(int64_t T, int n_q, int n_kv) { return T >= CHUNK_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30); }
 
 template <typename T>

@@ -2,12 +2,12 @@
 // that the tensor-memory form (agn_attention_prompt.cu) does not cover.
 //
 // Bound by the matrix units: per 16 rows, 16 slots and 32 dims 8 products m16n8k16 (f16) for the scores and 8 for the output, which caps the kernel near 276
-// TFLOP/s; with eight warps an SM they are busy 40 % of the time.  Precision comes from two-part operands as in the decode kernel: queries as hi + lo f16 against the cached
-// bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached
-// bytes (397 -> 322 us for 2048 rows of 28/4 heads of 128 against tf32 parts and blocks taken apart at once).  A CTA takes 16 rows per warp of one KV head - row r
-// is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory once for all warps,
-// the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 36.7 us (128 CTAs, eight tiles one after the other); 2048 tokens of 28/4 heads of 128:
-// 374 us, 80 TFLOP/s.  Blocks of four warps, two to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
+// TFLOP/s; what holds it is shared memory (77 % busy, the matrix units 42 %), where each warp's 16 rows read every tile again.  Precision comes from two-part operands
+// as in the decode kernel: queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached bytes.  A CTA takes
+// 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory
+// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 33 us (128 CTAs, eight tiles one after the other); 2048 tokens
+// of 28/4 heads of 128: 310 us, 97 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end).  Blocks of four warps, two
+// to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
 #include <math.h>
 
 #include "agn_attention_decode.cuh"
@@ -25,14 +25,14 @@ template <int NB> struct ChunkTiles {
     using C = ChunkShape<NB>;
     __half q[2][C::ROWS * C::ROW];  // hi, lo
     __half k[2][SL * C::ROW], v[2][SL * C::ROW];
-    float ks[2][SL][NB], vs[2][SL][NB], coef[C::ROWS];
+    __align__(16) float ks[2][NB][SL + 8], vs[2][NB][SL + 8], coef[C::ROWS];  // scales of neighbouring slots side by side
     uint32_t most[3][NB], least[3][NB];  // of the scales of a tile's values that are not 0, as bits of their magnitudes
     int odd;
 };
 
 // One block of 32 values on its way from the cache: 16 words of f16, or 8 words of bytes and a scale.  q8_0 as the words lie in memory: a block that begins at a
 // multiple of 4 is 8 words (scale and bytes) and the last two bytes, one that does not is the scale and 8 words.  Taking them apart is left to place_block, since a
-// use of a loaded word here would wait for it (2048 rows of 28/4 heads of 128: 397 us, so 374).
+// use of a loaded word here would wait for it (2048 rows of 28/4 heads of 128, at that step: 397 us, so 374).
 template <int KV> struct Block {
     uint32_t w[KV == KV_F16 ? 16 : 8];
     uint32_t more;  // q8_0: the two bytes outside the words; words: the scale
@@ -151,10 +151,10 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
         const int n = tid + i * C::THREADS, b = n % NB, slot = n / NB % SL;
         const bool is_k = n < SL * NB;
         if (n >= 2 * SL * NB) return;
-        const bool odd = place_block<KV>(x, block_at(n, tile), (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, &(is_k ? sm.ks : sm.vs)[tile & 1][slot][b], !is_k);
+        const bool odd = place_block<KV>(x, block_at(n, tile), (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, &(is_k ? sm.ks : sm.vs)[tile & 1][b][slot], !is_k);
         if (KV == KV_F16 && odd) sm.odd = 1;
         if (KV != KV_F16 && !is_k) {
-            const uint32_t size = __float_as_uint(sm.vs[tile & 1][slot][b]) & 0x7fffffffu;
+            const uint32_t size = __float_as_uint(sm.vs[tile & 1][b][slot]) & 0x7fffffffu;
             if (size) {
                 atomicMax(&sm.most[tile % 3][b], size);
                 atomicMin(&sm.least[tile % 3][b], size);
@@ -218,9 +218,11 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
             sm.least[(tile + 2) % 3][tid] = 0x7f800000u;
         }
         if (tile + 1 < tiles) fetch_tile(tile + 1);
-        if (tile * SL <= warp_last) {  // a warp whose rows see none of it waits for the others
-            const int buf = tile & 1;
-            float s[SL / 8][4];
+        const bool sees = tile * SL <= warp_last;  // a warp whose rows see none of it waits for the others
+        const int buf = tile & 1;
+        const bool edge = tile * SL + SL - 1 > warp_first;
+        float s[SL / 8][4];
+        if (sees) {
 #pragma unroll
             for (int n = 0; n < SL / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
@@ -248,15 +250,14 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                 if (KV != KV_F16) {
 #pragma unroll
                     for (int n = 0; n < SL / 8; n++) {
-                        const float s0 = sm.ks[buf][8 * n + 2 * t4][b], s1 = sm.ks[buf][8 * n + 2 * t4 + 1][b];
-                        s[n][0] = __fmaf_rn(blk[n][0], s0, s[n][0]);
-                        s[n][1] = __fmaf_rn(blk[n][1], s1, s[n][1]);
-                        s[n][2] = __fmaf_rn(blk[n][2], s0, s[n][2]);
-                        s[n][3] = __fmaf_rn(blk[n][3], s1, s[n][3]);
+                        const float2 f = *reinterpret_cast<const float2 *>(&sm.ks[buf][b][8 * n + 2 * t4]);
+                        s[n][0] = __fmaf_rn(blk[n][0], f.x, s[n][0]);
+                        s[n][1] = __fmaf_rn(blk[n][1], f.y, s[n][1]);
+                        s[n][2] = __fmaf_rn(blk[n][2], f.x, s[n][2]);
+                        s[n][3] = __fmaf_rn(blk[n][3], f.y, s[n][3]);
                     }
                 }
             }
-            const bool edge = tile * SL + SL - 1 > warp_first;
             float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < SL / 8; n++)
@@ -289,6 +290,9 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                     s[n][i] = ex2(__fmaf_rn(s[n][i], coef[i >> 1], -mu[i >> 1]));
                     l[i >> 1] += s[n][i];
                 }
+        }
+        if (tile + 1 < tiles) place_tile(tile + 1);
+        if (sees) {
             // ---- O += P V; the sums of a tile in the matrix unit (whose adder cuts), the running ones by rounded additions.  Dims 8 c + 2 t4 (+ 1) of the block in o[4 b + c].
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -310,7 +314,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                         for (int u = 0; u < 2; u++) {
                             float f0 = fold, f1 = fold;
                             if (KV != KV_F16) {
-                                const float2 f = make_float2(sm.vs[buf][8 * (n + u) + 2 * t4][b], sm.vs[buf][8 * (n + u) + 2 * t4 + 1][b]);
+                                const float2 f = *reinterpret_cast<const float2 *>(&sm.vs[buf][b][8 * (n + u) + 2 * t4]);
                                 f0 *= f.x;
                                 f1 *= f.y;
                             }
@@ -331,7 +335,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                     down = 1.0f;
 #pragma unroll
                     for (int n = 0; n < SL / 8; n++) {
-                        const float s0 = sm.vs[buf][8 * n + 2 * t4][b], s1 = sm.vs[buf][8 * n + 2 * t4 + 1][b];
+                        const float s0 = sm.vs[buf][b][8 * n + 2 * t4], s1 = sm.vs[buf][b][8 * n + 2 * t4 + 1];
                         float hi[4], lo[4], w[4] = {s[n][0] * s0, s[n][1] * s1, s[n][2] * s0, s[n][3] * s1};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
@@ -355,7 +359,6 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                     for (int i = 0; i < 4; i++) o[4 * b + c][i] = __fmaf_rn(acc[c][i], down, o[4 * b + c][i]);
             }
         }
-        if (tile + 1 < tiles) place_tile(tile + 1);
         __syncthreads();
     }
 
@@ -418,7 +421,7 @@ struct ChunkLayout {
 ChunkLayout chunk_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere = false) {
     ChunkLayout l;
     l.row_tiles = (int)((T * (n_q / n_kv) + chunk_rows(hd) - 1) / chunk_rows(hd));
-    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 0.5 + 0.045 * hd, T * n_q, hd, sms);
+    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 1.0 + 0.033 * hd, T * n_q, hd, sms);
     l.odd = attn_part_bytes(l.splits, T, n_q, hd);
     l.bytes = l.splits > 1 ? l.odd + (n_kv * 4 + 15) / 16 * 16 : 0;
     return l;
