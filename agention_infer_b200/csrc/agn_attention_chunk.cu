@@ -5,7 +5,7 @@
 // TFLOP/s; what holds it is shared memory (77 % busy, the matrix units 42 %), where each warp's 16 rows read every tile again.  Precision comes from two-part operands
 // as in the decode kernel: queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached bytes.  A CTA takes
 // 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory
-// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 33 us (128 CTAs, eight tiles one after the other); 2048 tokens
+// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 30.4 us (128 CTAs, eight tiles one after the other); 2048 tokens
 // of 28/4 heads of 128: 310 us, 97 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end).  Blocks of four warps, two
 // to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
 #include <math.h>
@@ -104,8 +104,9 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
     return odd;
 }
 
-// Weights times scales as two f16 parts, V_UP times: at most 2^15 (weights reach 2^8, scales are brought below 2).  The lower part's smallest step, 2^-24, is then 2^-30
-// of a full weight; scales that lie further apart than 2^6 take the tf32 products, whose parts have f32's range.
+// Weights times scales as two f16 parts, V_UP times: at most 2^15 (weights reach 2^8, scales are brought below 2).  The lower part is off by half its smallest step, 2^-25 or
+// 2^-31 of a full weight and scale, whatever the weight: 7 bits below what f32 rounds the sum to, but a weight under 2^-31 is lost, which shows in dims where
+// the values of all larger weights are exactly 0.  Scales that lie further apart than 2^6 take the tf32 products, whose parts have f32's range.
 constexpr float V_UP = 64.0f;
 __device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);

@@ -331,3 +331,23 @@ def test_values_of_very_different_sizes(backend, kv, low, high, hd):
     want, mag = ref.attention(q, k, v, [start + t for t in range(T)], hd ** -0.5)
     # a row's error is counted against its own weights' sum of |v|: what is small beside a value that the row does not see stays exact
     close(run_chunk(backend, c, q, start, "f32"), want, mag, q, k, slots, hd ** -0.5, "f32")
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0", "words"])
+def test_small_weights_beside_a_large_one_on_a_value_of_zero(backend, kv):
+    """One slot has nearly all the weight and a V of exactly 0.  The other slots' weights are exact to 2^-30 of it (half of the lower f16 part's smallest step, 2^-25, over
+    the 2^6 that weights are brought up by, for scales of half the largest at least): with n of them the row is off by at most n 2^-30 max |v| beside the usual bound."""
+    rng = np.random.default_rng(6)
+    T, start, nq, nkv, hd = 40, 260, 4, 2, 64
+    slots = start + T
+    c = Cache(backend, rng, kv, 1, slots, nkv, hd, [slots])
+    k, v = (rng.standard_normal((slots, nkv * hd)).astype(np.float32) for _ in range(2))
+    v[100] = 0.0
+    k[100] = 1.0
+    q = (0.2 * rng.standard_normal((T, nq, hd)) + np.linspace(0.5, 4.0, T)[:, None, None]).astype(np.float32)
+    backend.kv_write(c.kv, backend.upload(k), backend.upload(v), c.bufs[0], c.bufs[1], slots, nkv * hd, None, slots)
+    got = run_chunk(backend, c, q, start, "f32").astype(np.float64)
+    k, v = c.values(0, slots)
+    want, mag = ref.attention(q, k, v, [start + t for t in range(T)], hd ** -0.5)
+    bound = ref.attention_bound(q, k, mag, slots, hd ** -0.5) + slots * 2.0 ** -30 * np.abs(v).max()
+    assert np.all(np.abs(got - want) <= bound)
