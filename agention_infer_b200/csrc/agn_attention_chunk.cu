@@ -6,7 +6,7 @@
 // as in the decode kernel: queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached bytes.  A CTA takes
 // 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory
 // once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 30.4 us (128 CTAs, eight tiles one after the other); 2048 tokens
-// of 28/4 heads of 128: 310 us, 97 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end).  Blocks of four warps, two
+// of 28/4 heads of 128: 288 us, 104 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end, and queries loaded row by row).  Blocks of four warps, two
 // to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
 #include <math.h>
 
@@ -181,25 +181,34 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     if (tile0 < tiles) fetch_tile(tile0);
 
     // ---- Q, a warp's 16 rows: largest value to [1, 2), two f16 parts
-    for (int i = 0; i < 16; i++) {
-        const int r = r0 + warp * 16 + i;
-        const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD;
-        float x[NB], amax = 0.0f;
+    constexpr int QB = NB <= 4 ? 8 : 4;  // rows whose loads are on their way together (one after the other: 312 us for 2048 rows of 28/4 heads of 128, so 288)
+    for (int i0 = 0; i0 < 16; i0 += QB) {
+        float x[QB][NB];
 #pragma unroll
-        for (int c = 0; c < NB; c++) {
-            x[c] = r >= rows ? 0.0f : d.act16 ? __half2float(static_cast<const __half *>(a.q)[at + c * 32 + lane]) : static_cast<const float *>(a.q)[at + c * 32 + lane];
-            amax = fmaxf(amax, fabsf(x[c]));
+        for (int i = 0; i < QB; i++) {
+            const int r = r0 + warp * 16 + i0 + i;
+            const int64_t at = ((int64_t)(r / G) * a.n_q + kvh * G + r % G) * HD + lane;
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                x[i][c] = r >= rows ? 0.0f : d.act16 ? __half2float(static_cast<const __half *>(a.q)[at + c * 32]) : static_cast<const float *>(a.q)[at + c * 32];
         }
-        amax = agn_warp_max(amax);
-        const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        if (lane == 0) sm.coef[warp * 16 + i] = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), 1.17549435e-38f);
 #pragma unroll
-        for (int c = 0; c < NB; c++) {
-            const float v = x[c] * down;
-            const __half h = __float2half_rn(v);
-            sm.q[0][(warp * 16 + i) * ROW + c * 32 + lane] = h;
-            sm.q[1][(warp * 16 + i) * ROW + c * 32 + lane] = __float2half_rn(v - __half2float(h));
+        for (int i = 0; i < QB; i++) {
+            const int row = warp * 16 + i0 + i;
+            float amax = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NB; c++) amax = fmaxf(amax, fabsf(x[i][c]));
+            amax = agn_warp_max(amax);
+            const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);
+            const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+            if (lane == 0) sm.coef[row] = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), 1.17549435e-38f);
+#pragma unroll
+            for (int c = 0; c < NB; c++) {
+                const float v = x[i][c] * down;
+                const __half h = __float2half_rn(v);
+                sm.q[0][row * ROW + c * 32 + lane] = h;
+                sm.q[1][row * ROW + c * 32 + lane] = __float2half_rn(v - __half2float(h));
+            }
         }
     }
     if (tile0 < tiles) place_tile(tile0);
