@@ -5,7 +5,7 @@
 // TFLOP/s; what holds it is shared memory (77 % busy, the matrix units 42 %), where each warp's 16 rows read every tile again.  Precision comes from two-part operands
 // as in the decode kernel: queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached bytes.  A CTA takes
 // 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory
-// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 30.4 us (128 CTAs, eight tiles one after the other); 2048 tokens
+// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 27.8 us (128 CTAs, eight tiles one after the other); 2048 tokens
 // of 28/4 heads of 128: 288 us, 104 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end, and queries loaded row by row).  Blocks of four warps, two
 // to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
 #include <math.h>
