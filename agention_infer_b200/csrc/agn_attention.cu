@@ -166,6 +166,7 @@ int32_t attention_kv(agn_ctx *ctx, const T *q, T *out, int32_t kv_dtype, const v
     const int ca = kv_dtype == AGN_KV_Q8_0_WORDS ? 4 : 2;
     if (!agn_aligned(k_cache, ca) || !agn_aligned(v_cache, ca))
         return agn_fail(ctx, AGN_EINVAL, "attention_kv: caches must be %d-byte aligned", ca);
+    if (!agn_aligned(pos, 4) || !agn_aligned(seq, 4)) return agn_fail(ctx, AGN_EINVAL, "attention_kv: pos and seq must be 4-byte aligned");
     const bool prompt = !pos && sizeof(T) == 2 && agn_attention_prompt_fits(rows, n_q, n_kv, hd);
     const bool chunk = !pos && !prompt && chunk_fits(rows, n_q, n_kv);
     const int sms = ctx->sm_count < ATTN_MAX_SMS ? ctx->sm_count : ATTN_MAX_SMS;

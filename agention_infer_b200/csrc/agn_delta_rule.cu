@@ -889,6 +889,8 @@ extern "C" int32_t agn_gated_delta_rule_f32(agn_ctx *ctx, const float *q, const 
     if (!agn_aligned16(state_in) || !agn_aligned16(state_out) || !agn_aligned16(q) || !agn_aligned16(k) || !agn_aligned16(v) || !agn_aligned16(out) ||
         q_stride % 4 || k_stride % 4 || v_stride % 4)
         return agn_fail(ctx, AGN_EINVAL, "gated_delta_rule: q, k, v, out and the states must be 16-byte aligned, row strides multiples of 4");
+    if (!agn_aligned(g, 4) || !agn_aligned(beta, 4) || !agn_aligned(cu_seqlens, 4))
+        return agn_fail(ctx, AGN_EINVAL, "gated_delta_rule: g, beta and cu_seqlens must be aligned to their element type");
     if (out && (out == q || out == k || out == v)) return agn_fail(ctx, AGN_EINVAL, "gated_delta_rule: out must not alias q, k or v");
     AGN_CUDA(ctx, cudaSetDevice(ctx->device));
     DeltaArgs a;

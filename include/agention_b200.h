@@ -354,7 +354,8 @@ AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
  *   pos == NULL: the rows are the positions pos_start + t of the one sequence the caches hold — a prompt, or a
  *     piece of one, whose own keys are already in the cache (seq must be NULL, pos_start + T <= max_seq_len).
  * What the cache holds in slots that a row does not see, infinities and NaN included, does not change that row.
- * head_dim: a multiple of 32 up to 256; scale > 0 and finite; q and out 16-byte aligned and not the same buffer.
+ * head_dim: a multiple of 32 up to 256; scale > 0 and finite; q and out 16-byte aligned and not the same buffer; pos and seq
+ * 4-byte aligned.
  * workspace: at least agn_attention_kv_workspace_bytes(...) bytes of device memory, 16-byte aligned, whose contents
  * need not be kept between calls; calls that can overlap on the GPU need a workspace each.  NULL if that is 0.
  * The function takes the call's own sizes (has_pos: pos != NULL; any pos_start), needs no context and returns 0 for sizes the op refuses. */
@@ -383,7 +384,8 @@ AGN_API int32_t agn_attention_kv_f16(agn_ctx *ctx, const void *q, void *out, int
  * cu_seqlens: device int32 [n_seqs + 1], sequence s is the rows cu_seqlens[s] .. cu_seqlens[s+1] (none: its state is copied);
  * NULL: T / n_seqs rows each.  Rows behind the last sequence are left as they are.  Offsets outside [0, T] or out of order make the next
  * agn_sync return AGN_EOOB_ID; what the call writes then stays inside its buffers but is otherwise unspecified.
- * head_k 64 or 128, head_v a multiple of 32 up to 256.  workspace as in agn_attention_kv_f32. */
+ * head_k 64 or 128, head_v a multiple of 32 up to 256.  q, k, v, out and the states 16-byte aligned, g, beta and cu_seqlens 4-byte
+ * aligned.  workspace as in agn_attention_kv_f32. */
 AGN_API int64_t agn_gated_delta_rule_workspace_bytes(int64_t T, int64_t n_seqs, int32_t n_k_heads, int32_t n_v_heads,
                                                      int32_t head_k, int32_t head_v);
 AGN_API int32_t agn_gated_delta_rule_f32(agn_ctx *ctx, const float *q, const float *k, const float *v, const float *g,
