@@ -810,7 +810,10 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         freed(&sm.p_free);
         tell_state();
     }
-    if (gave_up) return;  // reported by the fetching warp, whose waits end as well
+    if (gave_up) {  // by the workers themselves: the fetching warps may have looked at sm.gave_up before one of these waits ran out
+        if (tid == 0) atomicOr(d.flags, AGN_FLAG_TIMEOUT);
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         *reinterpret_cast<float2 *>(d.state_out + soff + 8 * (n0 + n)) = make_float2(S[n][0], S[n][1]);
