@@ -97,7 +97,7 @@ template <typename Look> __device__ __forceinline__ float odd_value(const AttnAr
         }
         const unsigned char *row = a.v_cache + (int64_t)s * a.bytes_per_token;
         const float v = kv_dtype == AGN_F16 ? cache_value<KV_F16>(row, d) : kv_dtype == AGN_Q8_0 ? cache_value<KV_Q8>(row, d) : cache_value<KV_WORDS>(row, d);
-        if (half_finite(v)) continue;
+        if (fabsf(v) < INFINITY) continue;
         if (v != v) return NAN;
         if (v > 0.0f) up = true;
         else down = true;

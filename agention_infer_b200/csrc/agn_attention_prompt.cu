@@ -26,20 +26,26 @@ struct PromptArgs {
     AttnArgs a;
     __half *k, *v;   // [n_kv][tiles] images of TILE x hd
     int *odd;        // [n_kv][tiles]: the V tile has a value that is not finite
+    int *range;      // [K, V][n_kv][tiles]: RANGE_* of what the tile holds
     int kv_dtype;
     int64_t tiles, rows;  // tiles of the sequence; rows T * G of a KV head
     int spin, row_tiles;
     AttnSplit split;
 };
 
+// Whether f16 holds a tile: something of 65520 or more, which f16 turns into infinity; keys from f16's smallest normal number on; keys other than 0.  Keys that all
+// lie below it would lose their bits (a large `scale` may still make scores of them); small values are as exact as the f16 result.
+constexpr int RANGE_OVER = 1, RANGE_NORMAL = 2, RANGE_SOME = 4;
+
 // One CTA per (tile, KV head, K or V).  Values that are not finite are 0 in V's image and noted: a weight of 0 for a slot that a
 // row does not see must not meet them in the product.
-template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(PromptArgs p) {
+template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(const __grid_constant__ PromptArgs p) {
     agn_pdl_prologue();
     const AttnArgs &a = p.a;
     const int64_t tile = blockIdx.x;
     const int head = blockIdx.y, hd = a.hd, chunks = hd / 8;
     bool odd = false;
+    float most = 0.0f;
     const bool is_v = blockIdx.z;
     const int end = a.pos_start + (int)a.T;
     const unsigned char *src = is_v ? a.v_cache : a.k_cache;
@@ -70,11 +76,15 @@ template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(Pro
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = 0.0f;
         }
+        if (KV != KV_F16) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) most = fmaxf(most, fabsf(v[k]));  // NaN is ignored
+        }
         if (is_v) {
 #pragma unroll
             for (int k = 0; k < 8; k++)
                 if (!half_finite(v[k])) {
-                    odd = true;
+                    odd |= !(fabsf(v[k]) < INFINITY);
                     v[k] = 0.0f;
                 }
         }
@@ -85,6 +95,80 @@ template <int KV> __global__ void __launch_bounds__(1024) attn_unpack_kernel(Pro
     }
     odd = __syncthreads_or(odd);
     if (is_v && threadIdx.x == 0) p.odd[head * p.tiles + tile] = odd;
+    if (KV != KV_F16) {  // f16 tiles are what the cache holds
+        __shared__ float warp_most[32];
+        most = agn_warp_max(most);
+        if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            most = agn_warp_max(warp_most[threadIdx.x]);
+            int bits = most >= 65520.0f ? RANGE_OVER : 0;
+            if (!is_v) bits |= (most >= 6.103515625e-5f ? RANGE_NORMAL : 0) | (most > 0.0f ? RANGE_SOME : 0);
+            if (threadIdx.x == 0) p.range[((is_v ? a.n_kv : 0) + head) * p.tiles + tile] = bits;
+        }
+    }
+}
+
+// Rows whose tiles f16 does not hold, straight from the cache in f32: the CTA's rows r0 .. r0 + 2 TILE - 1 over its share's tiles, written as the kernel below writes
+// them (values that are not finite as 0).  A warp per row, four slots at a time; rare, and slow (2048 rows of 28/4 heads of 128 over 2048 slots: 23 ms, where the tensor
+// cores take 55 us).
+template <int HD, int KV> __device__ __noinline__ void prompt_rows_f32(const PromptArgs &p, int head, int share, int64_t r0, int tile0, int tiles) {
+    const AttnArgs &a = p.a;
+    const int lane = threadIdx.x & 31, G = a.n_q / a.n_kv;
+    constexpr int V = HD / 32;
+    const float coef = a.scale * 1.4426950408889634f;
+    for (int i = threadIdx.x >> 5; i < 2 * TILE && r0 + i < p.rows; i += PROMPT_THREADS / 32) {
+        const int64_t r = r0 + i, row = r / G * a.n_q + head * G + r % G;
+        const int end = min(a.pos_start + (int)(r / G) + 1, (tile0 + tiles) * TILE);
+        float q[V], o[V], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int c = 0; c < V; c++) {
+            q[c] = __half2float(static_cast<const __half *>(a.q)[row * HD + lane + 32 * c]);
+            o[c] = 0.0f;
+        }
+        for (int j = tile0 * TILE; j < end; j += 4) {
+            float s[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const unsigned char *key = a.k_cache + (int64_t)min(j + k, end - 1) * a.bytes_per_token;
+                float x = 0.0f;
+#pragma unroll
+                for (int c = 0; c < V; c++) x = __fmaf_rn(q[c], cache_value<KV>(key, head * HD + lane + 32 * c), x);
+                s[k] = agn_warp_sum(x) * coef;
+                if (j + k >= end) s[k] = -INFINITY;
+            }
+            const float mt = fmaxf(fmaxf(m, fmaxf(s[0], s[1])), fmaxf(s[2], s[3])), mu = mt == -INFINITY ? 0.0f : mt, down = ex2(m - mu);
+            m = mt;
+            l *= down;
+#pragma unroll
+            for (int c = 0; c < V; c++) o[c] *= down;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (j + k >= end) break;
+                const unsigned char *value = a.v_cache + (int64_t)(j + k) * a.bytes_per_token;
+                const float w = ex2(s[k] - mu);
+                l += w;
+#pragma unroll
+                for (int c = 0; c < V; c++) {
+                    const float v = cache_value<KV>(value, head * HD + lane + 32 * c);
+                    o[c] = __fmaf_rn(w, fabsf(v) < INFINITY ? v : 0.0f, o[c]);
+                }
+            }
+        }
+        if (p.split.splits > 1) {
+            float *to = p.split.part + ((int64_t)share * a.T * a.n_q + row) * (HD + 4);
+#pragma unroll
+            for (int c = 0; c < V; c++) to[lane + 32 * c] = o[c];
+            if (lane == 0) {
+                to[HD] = m;
+                to[HD + 1] = l;
+            }
+        } else {
+            const float inv = m == -INFINITY ? NAN : 1.0f / l;
+#pragma unroll
+            for (int c = 0; c < V; c++) static_cast<__half *>(a.out)[row * HD + lane + 32 * c] = __float2half_rn(o[c] * inv);
+        }
+    }
 }
 
 // ---- tensor-core instructions
@@ -155,10 +239,10 @@ template <int HD> struct PromptSmem {
     unsigned char q[2][TILE * HD * 2], kv[SLOTS][TILE * HD * 2];  // tiles in the order K0 V0 K1 V1 ..
     uint64_t q_full, full[SLOTS], free[SLOTS], s_full[2], p_full[2], o_full[2], drained;
     uint32_t tmem;
-    int gave_up;
+    int gave_up, range, odd;
 };
 
-template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prompt_kernel(PromptArgs p) {
+template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs p) {
     agn_pdl_prologue();
     extern __shared__ unsigned char raw[];
     PromptSmem<HD> &sm = *reinterpret_cast<PromptSmem<HD> *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -206,7 +290,7 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
         }
         agn_mbar_init(&sm.drained, 1);
         agn_mbar_init_fence();
-        sm.gave_up = 0;
+        sm.gave_up = sm.range = sm.odd = 0;
     }
     fence_before();
     __syncthreads();
@@ -436,11 +520,24 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
     }
     if (tid == 0 && sm.gave_up) atomicOr(a.flags, AGN_FLAG_TIMEOUT);
 
-    // Rare: V holds values that are not finite.  They were 0 in the product.
-    if (p.split.splits > 1) return;  // by agn_attention_join
-    bool any = false;
-    for (int j = tid; j < tiles; j += PROMPT_THREADS) any |= p.odd[head * p.tiles + j] != 0;
-    if (!__syncthreads_or(any)) return;
+    // Rare: f16 does not hold the keys or values of these tiles, or V holds values that are not finite (they were 0 in the product).
+    const bool may_be_out = p.kv_dtype != AGN_F16;
+    int range = 0, odd = 0;
+    for (int j = tid; j < tiles; j += PROMPT_THREADS) {
+        const int64_t at = head * p.tiles + tile0 + j;
+        odd |= p.odd[at];
+        if (may_be_out) range |= p.range[at] | p.range[a.n_kv * p.tiles + at];
+    }
+    if (range) atomicOr(&sm.range, range);
+    if (odd) sm.odd = 1;
+    __syncthreads();
+    range = sm.range;
+    if ((range & RANGE_OVER) || (range & (RANGE_NORMAL | RANGE_SOME)) == RANGE_SOME) {
+        if (p.kv_dtype == AGN_Q8_0) prompt_rows_f32<HD, KV_Q8>(p, head, share, r0, tile0, tiles);
+        else prompt_rows_f32<HD, KV_WORDS>(p, head, share, r0, tile0, tiles);
+        __syncthreads();
+    }
+    if (p.split.splits > 1 || !sm.odd) return;  // shares: by agn_attention_join
     for (int64_t x = tid; x < 2 * TILE * HD; x += PROMPT_THREADS) {
         const int64_t r = r0 + x / HD;
         const int d = (int)(x % HD), last = a.pos_start + (int)(r / G);
@@ -486,7 +583,7 @@ PromptLayout prompt_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, 
     PromptLayout l;
     l.image = image_bytes(slots, n_kv, hd);
     l.odd = 2 * l.image;
-    l.part = l.odd + (odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;
+    l.part = l.odd + (3 * odd_ints(slots, n_kv) * 4 + 15) / 16 * 16;  // odd, range of K, range of V
     l.row_tiles = (int)((T * (n_q / n_kv) + 2 * TILE - 1) / (2 * TILE));
     l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + TILE - 1) / TILE, 2.4, T * n_q, hd, sms);
     l.bytes = l.part + attn_part_bytes(l.splits, T, n_q, hd);
@@ -507,6 +604,7 @@ int32_t agn_attention_prompt_f16(agn_ctx *ctx, const AttnArgs &a, int kv_dtype, 
     p.k = reinterpret_cast<__half *>(w);
     p.v = reinterpret_cast<__half *>(w + l.image);
     p.odd = reinterpret_cast<int *>(w + l.odd);
+    p.range = p.odd + odd_ints(slots, a.n_kv);
     p.split.part = reinterpret_cast<float *>(w + l.part);
     p.split.splits = l.splits;
     p.row_tiles = l.row_tiles;
