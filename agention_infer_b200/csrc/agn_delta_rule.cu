@@ -146,15 +146,16 @@ template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kern
 // delta_prepare_kernel computes N, P, c, r_C and the normalised q and k of every chunk side by side; delta_chunk_kernel carries 32
 // columns of one head's state from chunk to chunk (the columns are independent: 128 CTAs for one sequence of 32 heads of 128).
 //
-// Bound by shared memory (71 % busy: every fragment of K and Q is read from there for 32 columns) and the matrix units (49 %: 1.05 M multiply-adds per chunk and 32
-// columns, three times over); a chunk takes 3.6 us.  4096 rows of 16/32 heads of 128: 87 us of preparation and 239 us of chunks.  f32 operands are split into two f16
-// parts each, x = hi + lo (22 bits), and hi hi + hi lo + lo hi is summed in f32 by m16n8k16 (twice the rate of tf32's three
-// products; two tf32 parts would not need the scaling below).  f16's range is met by powers of two: |k|, |q| <= 1 and the
-// entries of N and P have known bounds; states and values are scaled by a power of two taken from their largest magnitude in front of
-// every chunk.  Those bounds hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that breaks them is
-// computed row by row in f32 instead.
+// Bound by the matrix units (59 % busy on the SMs at work: 1.05 M multiply-adds per chunk and 32 columns, three times over, at tf32's rate) and by the waits between
+// dependent products; a chunk takes 6 us.  4096 rows of 16/32 heads of 128: 87 us of preparation and 390 us of chunks.  Every product is taken in two parts of 11
+// bits each, x = hi + lo, as hi hi + hi lo + lo hi, summed in f32.  K, Q, N and P, whose size is known, are f16 parts in the workspace, brought up by KQ_UP and NP_UP;
+// f16 is exact in tf32.  S, V - c K S, D and r D stay f32 in shared memory and are split into tf32 parts, which have f32's range, as they are read: columns do not share a
+// scale, so that one of another size, a large row later in the chunk or a state that has decayed takes no bits from the rest.  (f16 parts under one power of two per 32
+// columns and chunk, at m16n8k16's double rate: 239 us of chunks, but a column 2^-20 of its neighbour had ten bits left.  bf16 for the two mixed products: 367 us, twice the
+// error.  Sixteen workers of eight columns each: 430 us.)  The bounds of K, Q, N and P hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that
+// breaks them is computed row by row in f32 instead.
 constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 128;
-constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals
+constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals; taken back from the other operand
 
 // The workspace holds the operands as they stand in shared memory, rows 16 bytes off a multiple of 128 (so that the eight rows of a fragment do not collide):
 // a chunk's K, Q, N or P is one bulk copy.
@@ -189,6 +190,42 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const float *a, float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+// A 16 x 16 fragment of f16 operands (four registers as ldmatrix gives them) as the operands of two products of eight: slots t4 and t4 + 4 of the first one stand
+// for columns 2 t4 and 2 t4 + 1, those of the second one for columns 2 t4 + 8 and 2 t4 + 9.  f16 is exact in tf32.
+__device__ __forceinline__ void half_to_tf32(const uint32_t (&r)[4], float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&r[i]));
+        f[(i >> 1) * 4 + (i & 1)] = x.x;
+        f[(i >> 1) * 4 + (i & 1) + 2] = x.y;
+    }
+}
+// The other operand, 16 rows from b on (this lane's column), split into two tf32 parts on its way: hi rounded to 11 bits, lo the rest.
+struct Split16 {
+    float hi[4], lo[4];
+    __device__ __forceinline__ Split16(const float *b, int row) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = b[((i >> 1) * 8 + (i & 1)) * row];
+            hi[i] = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+            lo[i] = x - hi[i];
+        }
+    }
+};
+// big += hi hi, small += hi lo + lo hi: apart, because the matrix unit's adder cuts what is below the sum's last bit
+__device__ __forceinline__ void mma_split(float (&big)[4], float (&small)[4], const float (&ah)[8], const float (&al)[8], const Split16 &b) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        mma8(big, ah + 4 * i, b.hi[2 * i], b.hi[2 * i + 1]);
+        mma8(small, ah + 4 * i, b.lo[2 * i], b.lo[2 * i + 1]);
+        mma8(small, al + 4 * i, b.hi[2 * i], b.hi[2 * i + 1]);
+    }
 }
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(agn_smem_u32(dst)), "l"(src) : "memory");
@@ -426,11 +463,11 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
 }
 
 template <int DK> struct ChunkSmem {
-    static constexpr int KROW = kq_row(DK), NROW = NP_ROW, SROW = 40, VROW = 40;  // elements; rows whose fragments do not collide
+    static constexpr int KROW = kq_row(DK), NROW = NP_ROW, BROW = 36, VROW = 40;  // elements; rows whose fragments do not collide
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
-    __half s[2][DK * SROW], xx[2][CH * SROW], dd[2][CH * SROW], dr[2][CH * SROW];  // B operands: S, V - c K S, D, r D (hi, lo)
+    float s[DK * BROW], xx[CH * BROW], dd[CH * BROW], dr[CH * BROW];  // S / KQ_UP, (V - c K S) / NP_UP, D / NP_UP, r D / KQ_UP
     float v[2][CH * VROW], decay[2][2 * CH];
-    uint32_t most[9];
+    int bad[9];  // the state's columns of each worker, the chunk's values: not all finite
     uint64_t kq_full, v_full, n_full, p_full, kq_free, n_free, p_free;
     int gave_up;
 };
@@ -487,7 +524,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
     extern __shared__ __align__(128) unsigned char raw[];
     using SM = ChunkSmem<DK>;
     SM &sm = *reinterpret_cast<SM *>(raw);
-    constexpr int KROW = SM::KROW, NROW = SM::NROW, SROW = SM::SROW, VROW = SM::VROW;
+    constexpr int KROW = SM::KROW, NROW = SM::NROW, BROW = SM::BROW, VROW = SM::VROW;
     constexpr int MT = DK / 16, NU = MT / 2;  // the state's 16 x 8 tiles: MT x 4, NU to a warp
     const DeltaArgs &d = x.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -535,9 +572,9 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         }
         cp16(sm.decay[c & 1] + lane * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + lane * 4);
     };
-    auto tell_largest = [&](uint32_t most) {  // magnitudes as bits: NaN above infinity above the numbers
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 0) sm.most[warp] = most;
+    auto tell_finite = [&](float sum) {  // of differences x - x: 0 where every x is finite, NaN otherwise
+        const bool bad = __any_sync(0xffffffffu, !(sum == 0.0f));
+        if (lane == 0) sm.bad[warp] = bad;
     };
     // a bounded wait; once one has run out the CTA's other waits give up after their next poll
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -571,14 +608,13 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
                 load_v(c);
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 const float *v = sm.v[c & 1];
-                uint32_t most = 0;
+                float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < CH * 8 / 32; i++) {
                     const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
-                    most = max(most, max(max(__float_as_uint(y.x) & 0x7fffffffu, __float_as_uint(y.y) & 0x7fffffffu),
-                                         max(__float_as_uint(y.z) & 0x7fffffffu, __float_as_uint(y.w) & 0x7fffffffu)));
+                    sum += ((y.x - y.x) + (y.y - y.y)) + ((y.z - y.z) + (y.w - y.w));
                 }
-                tell_largest(most);
+                tell_finite(sum);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.v_full);
             } else if (lane == 0) {
@@ -601,12 +637,10 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         if (lane == 0) mbar_arrive(bar);
     };
     auto tell_state = [&] {
-        uint32_t most = 0;
+        float sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NU; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(S[n][i]) & 0x7fffffffu);
-        tell_largest(most);
+        for (int n = 0; n < NU; n++) sum += ((S[n][0] - S[n][0]) + (S[n][1] - S[n][1])) + ((S[n][2] - S[n][2]) + (S[n][3] - S[n][3]));
+        tell_finite(sum);
     };
     tell_state();
     for (int64_t c = 0; c < chunks; c++) {
@@ -614,12 +648,12 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         const int rows = (int)(e - first < CH ? e - first : CH);
         const uint32_t turn = c & 1;
         if ((gave_up = workers_sync_or(!(wait(&sm.kq_full, turn) && wait(&sm.v_full, turn))))) break;
-        uint32_t most = 0;
+        int bad = 0;
 #pragma unroll
-        for (int w = 0; w < 9; w++) most = max(most, sm.most[w]);
+        for (int w = 0; w < 9; w++) bad |= sm.bad[w];
         const int odd_next = c + 1 < chunks ? x.odd[(slot0 + c + 1) * d.n_v + hv] : 0;
         const float *v = sm.v[c & 1];
-        if (odd || most >= 0x7f800000u) {
+        if (odd || bad) {
             // nobody's copies into these buffers may be on their way any more
             if ((gave_up = workers_sync_or(!(wait(&sm.n_full, turn) && wait(&sm.p_full, turn))))) break;
             float *Sf = reinterpret_cast<float *>(sm.q), *tmp = reinterpret_cast<float *>(sm.n);  // q, N are not needed
@@ -637,64 +671,56 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
             freed(&sm.kq_free);
             freed(&sm.n_free);
             freed(&sm.p_free);
-            workers_sync();  // the maxima have been read
+            workers_sync();  // sm.bad has been read
             tell_state();
             odd = odd_next;
             continue;
         }
         odd = odd_next;
-        // up = 2^(5 - exponent): the largest becomes 2^5 .. 2^6, V - c K S at most 2^10, D at most 2^15
-        const int ex = max((int)(most >> 23), 24);
-        const float up = __uint_as_float((uint32_t)(259 - ex) << 23), down = __uint_as_float((uint32_t)(ex - 5) << 23);
 #pragma unroll
         for (int n = 0; n < NU; n++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint32_t h2, l2;
-                split2(S[n][2 * i] * up, S[n][2 * i + 1] * up, h2, l2);
-                const int at = (16 * mt + g + 8 * i) * SROW + 8 * (n0 + n) + 2 * t4;
-                *reinterpret_cast<uint32_t *>(&sm.s[0][at]) = h2;
-                *reinterpret_cast<uint32_t *>(&sm.s[1][at]) = l2;
-            }
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<float2 *>(&sm.s[(16 * mt + g + 8 * i) * BROW + 8 * (n0 + n) + 2 * t4]) = make_float2(S[n][2 * i] * (1.0f / KQ_UP), S[n][2 * i + 1] * (1.0f / KQ_UP));
         workers_sync();
 
         // ---- K S and Q S: 16 rows and 16 columns per warp
-        const int wm = warp & 3, wn = (warp >> 2) * 16;
+        const int wm = warp & 3, wn = (warp >> 2) * 16, bat = 2 * t4 * BROW + g;  // this lane's first element of a B fragment
         const __half *kh = sm.k[c & 1][0], *kl = sm.k[c & 1][1];
-        float ks[2][4] = {}, qs[2][4] = {};
+        float ks[2][4] = {}, qs[2][4] = {}, ks_low[2][4] = {}, qs_low[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < DK / 16; kk++) {
-            uint32_t a0[4], a1[4], q0[4], q1[4], bh[4], bl[4];
+            uint32_t r0[4], r1[4];
+            float kfh[8], kfl[8], qfh[8], qfl[8];
             const int arow = (wm * 16 + (lane & 15)) * KROW + kk * 16 + (lane >> 4) * 8;
-            const int brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
-            ldsm4(a0, kh + arow);
-            ldsm4(a1, kl + arow);
-            ldsm4(q0, sm.q[0] + arow);
-            ldsm4(q1, sm.q[1] + arow);
-            ldsm4t(bh, sm.s[0] + brow);
-            ldsm4t(bl, sm.s[1] + brow);
+            ldsm4(r0, kh + arow);
+            ldsm4(r1, kl + arow);
+            half_to_tf32(r0, kfh);
+            half_to_tf32(r1, kfl);
+            ldsm4(r0, sm.q[0] + arow);
+            ldsm4(r1, sm.q[1] + arow);
+            half_to_tf32(r0, qfh);
+            half_to_tf32(r1, qfl);
 #pragma unroll
-            for (int n = 0; n < 2; n++) { mma16(ks[n], a0, bh[2 * n], bh[2 * n + 1]); mma16(qs[n], q0, bh[2 * n], bh[2 * n + 1]); }
-#pragma unroll
-            for (int n = 0; n < 2; n++) { mma16(ks[n], a0, bl[2 * n], bl[2 * n + 1]); mma16(qs[n], q0, bl[2 * n], bl[2 * n + 1]); }
-#pragma unroll
-            for (int n = 0; n < 2; n++) { mma16(ks[n], a1, bh[2 * n], bh[2 * n + 1]); mma16(qs[n], q1, bh[2 * n], bh[2 * n + 1]); }
+            for (int n = 0; n < 2; n++) {
+                const Split16 f(sm.s + kk * 16 * BROW + wn + 8 * n + bat, BROW);
+                mma_split(ks[n], ks_low[n], kfh, kfl, f);
+                mma_split(qs[n], qs_low[n], qfh, qfl, f);
+            }
         }
         const int r0 = wm * 16 + g;
         const float *dec = sm.decay[c & 1];
-        const float cg[2] = {dec[r0] * (1.0f / KQ_UP), dec[r0 + 8] * (1.0f / KQ_UP)};
+        const float cg[2] = {dec[r0], dec[r0 + 8]};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int col = wn + 8 * n + 2 * t4;
                 const float2 vv = *reinterpret_cast<const float2 *>(v + (r0 + 8 * i) * VROW + col);
-                uint32_t h2, l2;
-                split2(__fmaf_rn(-cg[i], ks[n][2 * i], vv.x * up), __fmaf_rn(-cg[i], ks[n][2 * i + 1], vv.y * up), h2, l2);
-                *reinterpret_cast<uint32_t *>(&sm.xx[0][(r0 + 8 * i) * SROW + col]) = h2;
-                *reinterpret_cast<uint32_t *>(&sm.xx[1][(r0 + 8 * i) * SROW + col]) = l2;
-                qs[n][2 * i] *= cg[i];
-                qs[n][2 * i + 1] *= cg[i];
+                const float x0 = __fmaf_rn(-cg[i], ks[n][2 * i] + ks_low[n][2 * i], vv.x), x1 = __fmaf_rn(-cg[i], ks[n][2 * i + 1] + ks_low[n][2 * i + 1], vv.y);
+                *reinterpret_cast<float2 *>(&sm.xx[(r0 + 8 * i) * BROW + col]) = make_float2(x0 * (1.0f / NP_UP), x1 * (1.0f / NP_UP));
+                qs[n][2 * i] = cg[i] * (qs[n][2 * i] + qs_low[n][2 * i]);
+                qs[n][2 * i + 1] = cg[i] * (qs[n][2 * i + 1] + qs_low[n][2 * i + 1]);
             }
         freed(&sm.kq_free);  // q has been read; the other buffers of k and v were last chunk's
         if ((gave_up = workers_sync_or(!wait(&sm.n_full, turn)))) break;
@@ -702,111 +728,87 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         // ---- D = N X.  (N is a lower triangle, but leaving its empty blocks out would only make the warps uneven: the slowest one does them all.)
         float dd[2][4] = {}, po[2][4] = {};
         {
-            float t1[2][4] = {}, t2[2][4] = {};  // the three products apart: short chains
+            float low[2][4] = {};
 #pragma unroll
             for (int kk = 0; kk < CH / 16; kk++) {
                 if (kk > wm) break;
-                uint32_t a0[4], a1[4], bh[4], bl[4];
-                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
-                ldsm4(a0, sm.n[0] + arow);
-                ldsm4(a1, sm.n[1] + arow);
-                ldsm4t(bh, sm.xx[0] + brow);
-                ldsm4t(bl, sm.xx[1] + brow);
+                uint32_t r0[4], r1[4];
+                float fh[8], fl[8];
+                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8;
+                ldsm4(r0, sm.n[0] + arow);
+                ldsm4(r1, sm.n[1] + arow);
+                half_to_tf32(r0, fh);
+                half_to_tf32(r1, fl);
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    mma16(dd[n], a0, bh[2 * n], bh[2 * n + 1]);
-                    mma16(t1[n], a0, bl[2 * n], bl[2 * n + 1]);
-                    mma16(t2[n], a1, bh[2 * n], bh[2 * n + 1]);
-                }
+                for (int n = 0; n < 2; n++) mma_split(dd[n], low[n], fh, fl, Split16(sm.xx + kk * 16 * BROW + wn + 8 * n + bat, BROW));
             }
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) dd[n][i] += t1[n][i] + t2[n][i];
+                for (int i = 0; i < 4; i++) dd[n][i] += low[n][i];
         }
-        const float rc[2] = {dec[CH + r0], dec[CH + r0 + 8]};
+        const float rc[2] = {dec[CH + r0] * (1.0f / KQ_UP), dec[CH + r0 + 8] * (1.0f / KQ_UP)};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int at = (r0 + 8 * i) * SROW + wn + 8 * n + 2 * t4;
-                const float u = dd[n][2 * i] * (1.0f / NP_UP), w = dd[n][2 * i + 1] * (1.0f / NP_UP);
-                uint32_t h2, l2;
-                split2(u, w, h2, l2);
-                *reinterpret_cast<uint32_t *>(&sm.dd[0][at]) = h2;
-                *reinterpret_cast<uint32_t *>(&sm.dd[1][at]) = l2;
-                split2(u * rc[i], w * rc[i], h2, l2);
-                *reinterpret_cast<uint32_t *>(&sm.dr[0][at]) = h2;
-                *reinterpret_cast<uint32_t *>(&sm.dr[1][at]) = l2;
+                const int at = (r0 + 8 * i) * BROW + wn + 8 * n + 2 * t4;
+                *reinterpret_cast<float2 *>(&sm.dd[at]) = make_float2(dd[n][2 * i] * (1.0f / NP_UP), dd[n][2 * i + 1] * (1.0f / NP_UP));
+                *reinterpret_cast<float2 *>(&sm.dr[at]) = make_float2(dd[n][2 * i] * rc[i], dd[n][2 * i + 1] * rc[i]);
             }
         freed(&sm.n_free);
         if ((gave_up = workers_sync_or(!wait(&sm.p_full, turn)))) break;
 
         // ---- S' = c_C S + K^T (r D)
-        float up_s[NU][4];
+        {
+            float sum[NU][4] = {}, low[NU][4] = {};
 #pragma unroll
-        for (int n = 0; n < NU; n++) up_s[n][0] = up_s[n][1] = up_s[n][2] = up_s[n][3] = 0.0f;
+            for (int kk = 0; kk < CH / 16; kk++) {
+                uint32_t r0[4], r1[4];
+                float fh[8], fl[8];
+                const int arow = (kk * 16 + (lane & 7) + (lane >> 4) * 8) * KROW + mt * 16 + ((lane >> 3) & 1) * 8;
+                ldsm4t(r0, kh + arow);
+                ldsm4t(r1, kl + arow);
+                half_to_tf32(r0, fh);
+                half_to_tf32(r1, fl);
 #pragma unroll
-        for (int kk = 0; kk < CH / 16; kk++) {
-            uint32_t a0[4], a1[4];
-            const int arow = (kk * 16 + (lane & 7) + (lane >> 4) * 8) * KROW + mt * 16 + ((lane >> 3) & 1) * 8;
-            ldsm4t(a0, kh + arow);
-            ldsm4t(a1, kl + arow);
-#pragma unroll
-            for (int n = 0; n < NU; n += 2) {
-                uint32_t bh[4], bl[4];
-                const int brow = (kk * 16 + (lane & 15)) * SROW + 8 * (n0 + n) + (lane >> 4) * 8;
-                ldsm4t(bh, sm.dr[0] + brow);
-                ldsm4t(bl, sm.dr[1] + brow);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    mma16(up_s[n + h], a0, bh[2 * h], bh[2 * h + 1]);
-                    mma16(up_s[n + h], a0, bl[2 * h], bl[2 * h + 1]);
-                    mma16(up_s[n + h], a1, bh[2 * h], bh[2 * h + 1]);
-                }
+                for (int n = 0; n < NU; n++) mma_split(sum[n], low[n], fh, fl, Split16(sm.dr + kk * 16 * BROW + 8 * (n0 + n) + bat, BROW));
             }
+            const float cc = dec[CH - 1];
+#pragma unroll
+            for (int n = 0; n < NU; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) S[n][i] = __fmaf_rn(cc, S[n][i], sum[n][i] + low[n][i]);
         }
-        const float cc = dec[CH - 1], f = down * (1.0f / KQ_UP);
-#pragma unroll
-        for (int n = 0; n < NU; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) S[n][i] = __fmaf_rn(up_s[n][i], f, cc * S[n][i]);
 
         // ---- O = c Q S + P D
         {
-            float t1[2][4] = {}, t2[2][4] = {};  // the three products apart: short chains
+            float low[2][4] = {};
 #pragma unroll
             for (int kk = 0; kk < CH / 16; kk++) {
                 if (kk > wm) break;
-                uint32_t a0[4], a1[4], bh[4], bl[4];
-                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8, brow = (kk * 16 + (lane & 15)) * SROW + wn + (lane >> 4) * 8;
-                ldsm4(a0, sm.p[0] + arow);
-                ldsm4(a1, sm.p[1] + arow);
-                ldsm4t(bh, sm.dd[0] + brow);
-                ldsm4t(bl, sm.dd[1] + brow);
+                uint32_t r0[4], r1[4];
+                float fh[8], fl[8];
+                const int arow = (wm * 16 + (lane & 15)) * NROW + kk * 16 + (lane >> 4) * 8;
+                ldsm4(r0, sm.p[0] + arow);
+                ldsm4(r1, sm.p[1] + arow);
+                half_to_tf32(r0, fh);
+                half_to_tf32(r1, fl);
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    mma16(po[n], a0, bh[2 * n], bh[2 * n + 1]);
-                    mma16(t1[n], a0, bl[2 * n], bl[2 * n + 1]);
-                    mma16(t2[n], a1, bh[2 * n], bh[2 * n + 1]);
-                }
+                for (int n = 0; n < 2; n++) mma_split(po[n], low[n], fh, fl, Split16(sm.dd + kk * 16 * BROW + wn + 8 * n + bat, BROW));
             }
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) po[n][i] += t1[n][i] + t2[n][i];
+                for (int i = 0; i < 4; i++) po[n][i] += low[n][i];
         }
-        const float fo = d.scale * down;
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                if (r0 + 8 * i < rows) {
-                    float2 y;
-                    y.x = __fmaf_rn(po[n][2 * i], 1.0f / NP_UP, qs[n][2 * i]) * fo;
-                    y.y = __fmaf_rn(po[n][2 * i + 1], 1.0f / NP_UP, qs[n][2 * i + 1]) * fo;
-                    *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) = y;
-                }
+                if (r0 + 8 * i < rows)
+                    *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) =
+                        make_float2((qs[n][2 * i] + po[n][2 * i]) * d.scale, (qs[n][2 * i + 1] + po[n][2 * i + 1]) * d.scale);
         freed(&sm.p_free);
         tell_state();
     }
