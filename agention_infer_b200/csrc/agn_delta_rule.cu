@@ -148,14 +148,25 @@ template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kern
 //
 // Bound by the matrix units (59 % busy on the SMs at work: 1.05 M multiply-adds per chunk and 32 columns, three times over, at tf32's rate) and by the waits between
 // dependent products; a chunk takes 6 us.  4096 rows of 16/32 heads of 128: 87 us of preparation and 390 us of chunks.  Every product is taken in two parts of 11
-// bits each, x = hi + lo, as hi hi + hi lo + lo hi, summed in f32.  K, Q, N and P, whose size is known, are f16 parts in the workspace, brought up by KQ_UP and NP_UP;
+// bits each, x = hi + lo, as hi hi + hi lo + lo hi, summed in f32.  K, Q, N and P are f16 parts in the workspace, every row brought to UP by a power of two of its own
+// (its largest entry; a row of one product is a row of the result, which takes the factor back), so that a small key, query or write strength keeps its bits;
 // f16 is exact in tf32.  S, V - c K S, D and r D stay f32 in shared memory and are split into tf32 parts, which have f32's range, as they are read: columns do not share a
 // scale, so that one of another size, a large row later in the chunk or a state that has decayed takes no bits from the rest.  (f16 parts under one power of two per 32
 // columns and chunk, at m16n8k16's double rate: 239 us of chunks, but a column 2^-20 of its neighbour had ten bits left.  bf16 for the two mixed products: 367 us, twice the
-// error.  Sixteen workers of eight columns each: 430 us.)  The bounds of K, Q, N and P hold for 0 <= beta <= 2, g <= 0, |k|, |q| <= 1 and finite numbers: a chunk that
-// breaks them is computed row by row in f32 instead.
+// error.  Sixteen workers of eight columns each: 430 us.)  Errors do not grow from row to row where 0 <= beta <= 2, g <= 0, |k| <= 1 and numbers are finite: a
+// chunk that is not so is computed row by row in f32 instead.
 constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 128;
-constexpr float KQ_UP = 64.0f, NP_UP = 256.0f;  // what keeps the lower parts out of f16's subnormals; taken back from the other operand
+constexpr float UP = 1024.0f, DOWN = 1.0f / UP;  // rows' largest entries lie in [UP, 2 UP); what is kept of the others is 2^-35 of that or better
+
+// A row whose largest entry is m times `up` has it in [UP, 2 UP); times `down`, it is what it was.
+__device__ __forceinline__ void row_scale(float m, float &up, float &down) {
+    const int e = min(max((int)(__float_as_uint(m) >> 23), 11), 254);  // from 2^-116 on
+    up = __uint_as_float((uint32_t)(264 - e) << 23);
+    down = __uint_as_float((uint32_t)(e - 10) << 23);
+}
+// Per chunk and value head, for its rows' results: RF_X: c_i times K's factor (of K S), RF_QS: c_i times Q's, RF_D: N's, RF_R: r_Ci times K's (of r D, in front of K^T),
+// RF_PD: P's; then c_C.  Factors of products with an operand that has been brought down (by DOWN) include UP.
+constexpr int RF_X = 0, RF_QS = 64, RF_D = 128, RF_R = 192, RF_PD = 256, RF_C = 320, ROW_FACTORS = 324;
 
 // The workspace holds the operands as they stand in shared memory, rows 16 bytes off a multiple of 128 (so that the eight rows of a fragment do not collide):
 // a chunk's K, Q, N or P is one bulk copy.
@@ -164,10 +175,10 @@ constexpr int NP_ROW = CH + 8;
 
 struct ChunkArgs {
     DeltaArgs d;
-    __half *kq;    // [slots][n_k][k hi, k lo, q hi, q lo][64][kq_row], times KQ_UP
-    __half *np;    // [slots][n_v][N hi, N lo, P hi, P lo][64][NP_ROW], times NP_UP
-    float *decay;  // [slots][n_v][128]: c_i, then r_Cj
-    int *odd;      // [slots][n_v]: the chunk breaks the bounds
+    __half *kq;      // [slots][n_k][k hi, k lo, q hi, q lo][64][kq_row]
+    __half *np;      // [slots][n_v][N hi, N lo, P hi, P lo][64][NP_ROW]
+    float *factors;  // [slots][n_v][ROW_FACTORS]
+    int *odd;        // [slots][n_v]: the chunk breaks the bounds
     int spin;
 };
 
@@ -241,6 +252,7 @@ template <int DK> struct PrepSmem {
             float kk[CH][TROW], qk[CH][TROW], A[CH][TROW], N[CH][TROW];
         } t;
     };
+    float down[2][CH];  // factors of the rows of k, of q
     float a[CH], beta[CH], whole[8], tail[CH];  // products of a over eight rows, over the rows behind a column up to the end of its eight
     int odd_kq, odd;
 };
@@ -325,15 +337,22 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
 #pragma unroll
             for (int j = 0; j < V; j++) ss = __fmaf_rn(v[n][w][j], v[n][w][j], ss);
             ss = agn_warp_sum(ss);
-            const float f = d.eps >= 0.0f ? rsqrtf(ss + d.eps) : 1.0f;
-            // the normalised row's norm is at most 1 unless a sum of squares overflowed or was not a number
-            if (lane == 0 && !(d.eps >= 0.0f ? ss < INFINITY && (ss + d.eps > 0.0f || i >= rows) : ss < 1.01f)) sm.odd_kq = 1;
+            const float f = i >= rows ? 0.0f : d.eps >= 0.0f ? rsqrtf(ss + d.eps) : 1.0f;
+            // the normalised row's norm is at most 1 unless a sum of squares overflowed or was not a number; a query may have any
+            if (lane == 0 && !(d.eps >= 0.0f ? ss < INFINITY && (ss + d.eps > 0.0f || i >= rows) : ss < (w == 0 ? 1.01f : INFINITY))) sm.odd_kq = 1;
+            float most = 0.0f, up, down;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                v[n][w][j] *= f;
+                most = fmaxf(most, fabsf(v[n][w][j]));
+            }
+            row_scale(agn_warp_max(most), up, down);
+            if (lane == 0) sm.down[w][i] = down;
             __half *g = x.kq + (((slot * d.n_k + hk) * 4 + 2 * w) * CH + i) * ROW;
-            const float u = i < rows ? f * KQ_UP : 0.0f;
 #pragma unroll
             for (int j = 0; j < V / 2; j++) {
                 uint32_t h2, l2;
-                split2(v[n][w][2 * j] * u, v[n][w][2 * j + 1] * u, h2, l2);
+                split2(v[n][w][2 * j] * up, v[n][w][2 * j + 1] * up, h2, l2);
                 const int at = 2 * (lane + 32 * j);
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w][i * ROW + at]) = h2;
                 *reinterpret_cast<uint32_t *>(&sm.op[2 * w + 1][i * ROW + at]) = l2;
@@ -373,13 +392,15 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
     __syncthreads();  // the operands are done with: the tables take their place
     {
         float(*to)[TROW] = which ? sm.t.qk : sm.t.kk;
-        constexpr float DOWN = 1.0f / (KQ_UP * KQ_UP);
+        const float f0 = sm.down[which][wm * 16 + g], f1 = sm.down[which][wm * 16 + g + 8];
 #pragma unroll
         for (int n = 0; n < 8; n++) {
-            to[wm * 16 + g][n * 8 + 2 * t4] = acc[n][0] * DOWN;
-            to[wm * 16 + g][n * 8 + 2 * t4 + 1] = acc[n][1] * DOWN;
-            to[wm * 16 + g + 8][n * 8 + 2 * t4] = acc[n][2] * DOWN;
-            to[wm * 16 + g + 8][n * 8 + 2 * t4 + 1] = acc[n][3] * DOWN;
+            const int col = n * 8 + 2 * t4;
+            const float c0 = sm.down[0][col], c1 = sm.down[0][col + 1];
+            to[wm * 16 + g][col] = acc[n][0] * f0 * c0;
+            to[wm * 16 + g][col + 1] = acc[n][1] * f0 * c1;
+            to[wm * 16 + g + 8][col] = acc[n][2] * f1 * c0;
+            to[wm * 16 + g + 8][col + 1] = acc[n][3] * f1 * c1;
         }
     }
 
@@ -404,7 +425,7 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
         }
         __syncthreads();
         __half *np = x.np + (slot * d.n_v + hv) * 4 * CH * NP_ROW;
-        float *decay = x.decay + (slot * d.n_v + hv) * 2 * CH;
+        float *factors = x.factors + (slot * d.n_v + hv) * ROW_FACTORS;
         {
             // r_ij down the eight rows, beginning with the product up to the row above them
             float r[2] = {1.0f, 1.0f}, between = 1.0f, c = 1.0f;
@@ -423,12 +444,21 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
                 if (i > col + 1) r[1] *= ai;
                 *reinterpret_cast<float2 *>(&sm.t.A[i][col]) = make_float2(i > col ? be * r[0] * kk.x : 0.0f, i > col + 1 ? be * r[1] * kk.y : 0.0f);
                 *reinterpret_cast<float2 *>(&sm.t.N[i][col]) = make_float2(0.0f, 0.0f);
+                const float p0 = i >= col ? r[0] * qk.x : 0.0f, p1 = i >= col + 1 ? r[1] * qk.y : 0.0f;
+                float up, down;
+                row_scale(agn_warp_max(fmaxf(fabsf(p0), fabsf(p1))), up, down);  // a warp has whole rows
                 uint32_t h2, l2;
-                split2(i >= col ? r[0] * qk.x * NP_UP : 0.0f, i >= col + 1 ? r[1] * qk.y * NP_UP : 0.0f, h2, l2);
+                split2(p0 * up, p1 * up, h2, l2);
                 *reinterpret_cast<uint32_t *>(np + (2 * CH + i) * NP_ROW + col) = h2;
                 *reinterpret_cast<uint32_t *>(np + (3 * CH + i) * NP_ROW + col) = l2;
-                if (col == 0) decay[i] = c *= ai;
-                if (i == CH - 1) *reinterpret_cast<float2 *>(decay + CH + col) = make_float2(r[0], r[1]);
+                c *= ai;
+                if (col == 0) {
+                    factors[RF_X + i] = c * sm.down[0][i] * UP;
+                    factors[RF_QS + i] = c * sm.down[1][i] * UP;
+                    factors[RF_PD + i] = down * UP;
+                    if (i == CH - 1) factors[RF_C] = c;
+                }
+                if (i == CH - 1) *reinterpret_cast<float2 *>(factors + RF_R + col) = make_float2(r[0] * sm.down[0][col], r[1] * sm.down[0][col + 1]);
             }
         }
         __syncthreads();
@@ -453,9 +483,13 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
         for (int i = tid; i < CH * CH / 2; i += CHUNK_THREADS) {
             const int row = i >> 5, col = 2 * (i & 31);
             uint32_t h2, l2;
-            split2(sm.t.N[row][col] * sm.beta[col] * NP_UP, sm.t.N[row][col + 1] * sm.beta[col + 1] * NP_UP, h2, l2);
+            const float n0 = sm.t.N[row][col] * sm.beta[col], n1 = sm.t.N[row][col + 1] * sm.beta[col + 1];
+            float up, down;
+            row_scale(agn_warp_max(fmaxf(fabsf(n0), fabsf(n1))), up, down);  // a row per warp
+            split2(n0 * up, n1 * up, h2, l2);
             *reinterpret_cast<uint32_t *>(np + row * NP_ROW + col) = h2;
             *reinterpret_cast<uint32_t *>(np + (CH + row) * NP_ROW + col) = l2;
+            if (col == 0) factors[RF_D + row] = down * UP;
         }
         if (tid == 0) x.odd[slot * d.n_v + hv] = sm.odd | sm.odd_kq;
         __syncthreads();
@@ -465,8 +499,8 @@ template <int DK> __global__ void __launch_bounds__(CHUNK_THREADS, 3) delta_prep
 template <int DK> struct ChunkSmem {
     static constexpr int KROW = kq_row(DK), NROW = NP_ROW, BROW = 36, VROW = 40;  // elements; rows whose fragments do not collide
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
-    float s[DK * BROW], xx[CH * BROW], dd[CH * BROW], dr[CH * BROW];  // S / KQ_UP, (V - c K S) / NP_UP, D / NP_UP, r D / KQ_UP
-    float v[2][CH * VROW], decay[2][2 * CH];
+    float s[DK * BROW], xx[CH * BROW], dd[CH * BROW], dr[CH * BROW];  // S and V - c K S and D, times DOWN; r D times K's factors
+    float v[2][CH * VROW], factors[2][ROW_FACTORS];
     int bad[9];  // the state's columns of each worker, the chunk's values: not all finite
     uint64_t kq_full, v_full, n_full, p_full, kq_free, n_free, p_free;
     int gave_up;
@@ -570,7 +604,8 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
             if (first + row < e) cp16(dst + row * VROW + at, src + row * d.v_stride + at);
             else *reinterpret_cast<float4 *>(dst + row * VROW + at) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        cp16(sm.decay[c & 1] + lane * 4, x.decay + ((slot0 + c) * d.n_v + hv) * 2 * CH + lane * 4);
+        const float *f = x.factors + ((slot0 + c) * d.n_v + hv) * ROW_FACTORS;
+        for (int i = 4 * lane; i < ROW_FACTORS; i += 128) cp16(sm.factors[c & 1] + i, f + i);
     };
     auto tell_finite = [&](float sum) {  // of differences x - x: 0 where every x is finite, NaN otherwise
         const bool bad = __any_sync(0xffffffffu, !(sum == 0.0f));
@@ -681,7 +716,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         for (int n = 0; n < NU; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                *reinterpret_cast<float2 *>(&sm.s[(16 * mt + g + 8 * i) * BROW + 8 * (n0 + n) + 2 * t4]) = make_float2(S[n][2 * i] * (1.0f / KQ_UP), S[n][2 * i + 1] * (1.0f / KQ_UP));
+                *reinterpret_cast<float2 *>(&sm.s[(16 * mt + g + 8 * i) * BROW + 8 * (n0 + n) + 2 * t4]) = make_float2(S[n][2 * i] * DOWN, S[n][2 * i + 1] * DOWN);
         workers_sync();
 
         // ---- K S and Q S: 16 rows and 16 columns per warp
@@ -709,18 +744,18 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
             }
         }
         const int r0 = wm * 16 + g;
-        const float *dec = sm.decay[c & 1];
-        const float cg[2] = {dec[r0], dec[r0 + 8]};
+        const float *rf = sm.factors[c & 1] + r0;
+        const float of_x[2] = {rf[RF_X], rf[RF_X + 8]}, of_qs[2] = {rf[RF_QS], rf[RF_QS + 8]};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int col = wn + 8 * n + 2 * t4;
                 const float2 vv = *reinterpret_cast<const float2 *>(v + (r0 + 8 * i) * VROW + col);
-                const float x0 = __fmaf_rn(-cg[i], ks[n][2 * i] + ks_low[n][2 * i], vv.x), x1 = __fmaf_rn(-cg[i], ks[n][2 * i + 1] + ks_low[n][2 * i + 1], vv.y);
-                *reinterpret_cast<float2 *>(&sm.xx[(r0 + 8 * i) * BROW + col]) = make_float2(x0 * (1.0f / NP_UP), x1 * (1.0f / NP_UP));
-                qs[n][2 * i] = cg[i] * (qs[n][2 * i] + qs_low[n][2 * i]);
-                qs[n][2 * i + 1] = cg[i] * (qs[n][2 * i + 1] + qs_low[n][2 * i + 1]);
+                const float x0 = __fmaf_rn(-of_x[i], ks[n][2 * i] + ks_low[n][2 * i], vv.x), x1 = __fmaf_rn(-of_x[i], ks[n][2 * i + 1] + ks_low[n][2 * i + 1], vv.y);
+                *reinterpret_cast<float2 *>(&sm.xx[(r0 + 8 * i) * BROW + col]) = make_float2(x0 * DOWN, x1 * DOWN);
+                qs[n][2 * i] = of_qs[i] * (qs[n][2 * i] + qs_low[n][2 * i]);
+                qs[n][2 * i + 1] = of_qs[i] * (qs[n][2 * i + 1] + qs_low[n][2 * i + 1]);
             }
         freed(&sm.kq_free);  // q has been read; the other buffers of k and v were last chunk's
         if ((gave_up = workers_sync_or(!wait(&sm.n_full, turn)))) break;
@@ -747,14 +782,15 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
 #pragma unroll
                 for (int i = 0; i < 4; i++) dd[n][i] += low[n][i];
         }
-        const float rc[2] = {dec[CH + r0] * (1.0f / KQ_UP), dec[CH + r0 + 8] * (1.0f / KQ_UP)};
+        const float of_d[2] = {rf[RF_D], rf[RF_D + 8]}, of_r[2] = {rf[RF_R], rf[RF_R + 8]};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const int at = (r0 + 8 * i) * BROW + wn + 8 * n + 2 * t4;
-                *reinterpret_cast<float2 *>(&sm.dd[at]) = make_float2(dd[n][2 * i] * (1.0f / NP_UP), dd[n][2 * i + 1] * (1.0f / NP_UP));
-                *reinterpret_cast<float2 *>(&sm.dr[at]) = make_float2(dd[n][2 * i] * rc[i], dd[n][2 * i + 1] * rc[i]);
+                const float d0 = dd[n][2 * i] * of_d[i], d1 = dd[n][2 * i + 1] * of_d[i];
+                *reinterpret_cast<float2 *>(&sm.dd[at]) = make_float2(d0 * DOWN, d1 * DOWN);
+                *reinterpret_cast<float2 *>(&sm.dr[at]) = make_float2(d0 * of_r[i], d1 * of_r[i]);
             }
         freed(&sm.n_free);
         if ((gave_up = workers_sync_or(!wait(&sm.p_full, turn)))) break;
@@ -774,7 +810,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
 #pragma unroll
                 for (int n = 0; n < NU; n++) mma_split(sum[n], low[n], fh, fl, Split16(sm.dr + kk * 16 * BROW + 8 * (n0 + n) + bat, BROW));
             }
-            const float cc = dec[CH - 1];
+            const float cc = sm.factors[c & 1][RF_C];
 #pragma unroll
             for (int n = 0; n < NU; n++)
 #pragma unroll
@@ -802,13 +838,14 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
 #pragma unroll
                 for (int i = 0; i < 4; i++) po[n][i] += low[n][i];
         }
+        const float of_pd[2] = {rf[RF_PD], rf[RF_PD + 8]};
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++)
                 if (r0 + 8 * i < rows)
                     *reinterpret_cast<float2 *>(d.out + ((first + r0 + 8 * i) * d.n_v + hv) * d.dv + c0 + wn + 8 * n + 2 * t4) =
-                        make_float2((qs[n][2 * i] + po[n][2 * i]) * d.scale, (qs[n][2 * i + 1] + po[n][2 * i + 1]) * d.scale);
+                        make_float2(__fmaf_rn(po[n][2 * i], of_pd[i], qs[n][2 * i]) * d.scale, __fmaf_rn(po[n][2 * i + 1], of_pd[i], qs[n][2 * i + 1]) * d.scale);
         freed(&sm.p_free);
         tell_state();
     }
@@ -829,15 +866,15 @@ constexpr int CHUNK_MIN_ROWS = 32;
 bool delta_chunked(int64_t T, int64_t n_seqs) { return T >= CHUNK_MIN_ROWS * n_seqs; }
 
 struct ChunkLayout {
-    int64_t slots, kq, np, decay, odd, bytes;  // byte offsets
+    int64_t slots, kq, np, factors, odd, bytes;  // byte offsets
 };
 ChunkLayout chunk_layout(int64_t T, int64_t n_seqs, int n_k, int n_v, int dk) {
     ChunkLayout l;
     l.slots = T / CH + n_seqs;
     l.kq = 0;
     l.np = l.kq + l.slots * n_k * 4 * CH * kq_row(dk) * 2;
-    l.decay = l.np + l.slots * n_v * 4 * CH * NP_ROW * 2;
-    l.odd = l.decay + l.slots * n_v * 2 * CH * 4;
+    l.factors = l.np + l.slots * n_v * 4 * CH * NP_ROW * 2;
+    l.odd = l.factors + l.slots * n_v * ROW_FACTORS * 4;
     l.bytes = (l.odd + l.slots * n_v * 4 + 15) / 16 * 16;
     return l;
 }
@@ -849,7 +886,7 @@ template <int DK> int32_t launch_chunked(agn_ctx *ctx, const DeltaArgs &d, void 
     x.d = d;
     x.kq = reinterpret_cast<__half *>(w + l.kq);
     x.np = reinterpret_cast<__half *>(w + l.np);
-    x.decay = reinterpret_cast<float *>(w + l.decay);
+    x.factors = reinterpret_cast<float *>(w + l.factors);
     x.odd = reinterpret_cast<int *>(w + l.odd);
     x.spin = ctx->mbar_spin_limit;
     if (agn_ring_ctas_per_sm(ctx, delta_prepare_kernel<DK>, CHUNK_THREADS, sizeof(PrepSmem<DK>)) < 1 ||

@@ -85,3 +85,64 @@ def test_rows_of_the_state_of_different_sizes(backend, T):
     want, wS = expected(x, [T], 0.125, -1.0)
     hold(out, want, 5 * sizes[np.argmax(x["q"][:, 0], axis=1), None, None], "out")
     hold(S[0, 0], wS[0, 0], 5 * sizes[:, None], "state")
+
+
+def running(x, scale, eps):
+    """(out, state, |S| of each head after every row [T, nv]) in float64, one sequence."""
+    q, k, v, S = (x[n].astype(np.float64) for n in ("q", "k", "v", "S"))
+    if eps >= 0:
+        q, k = (a / np.sqrt((a * a).sum(-1, keepdims=True) + eps) for a in (q, k))
+    rep, S = v.shape[1] // k.shape[1], S[0]
+    q, k = (np.repeat(a, rep, axis=1) for a in (q * scale, k))
+    out, size = np.zeros(v.shape), np.zeros(v.shape[:2])
+    for t in range(len(v)):
+        S = S * np.exp(x["g"][t].astype(np.float64))[:, None, None]
+        d = x["beta"][t].astype(np.float64)[:, None] * (v[t] - np.einsum("hkv,hk->hv", S, k[t]))
+        S = S + k[t][:, :, None] * d[:, None, :]
+        out[t] = np.einsum("hkv,hk->hv", S, q[t])
+        size[t] = np.abs(S).max(axis=(1, 2))
+    return out, S, size, np.linalg.norm(q, axis=2)
+
+
+@pytest.mark.parametrize("T", [10, 64, 100])
+@pytest.mark.parametrize("what", ["queries", "keys", "both"])
+@pytest.mark.parametrize("eps", [-1.0, 1e-6, 1.0])
+@pytest.mark.parametrize("size", [1e-2, 1e-4, 1e-6, 1e-9])
+def test_small_queries_and_keys_keep_their_bits(backend, size, eps, what, T):
+    """Taken as they are, or far below the epsilon of their norm: an output row is as large as its query, a state that begins at 0 as its keys."""
+    x = inputs(np.random.default_rng(T), [T], 2, 4, 128, 64)
+    for n in "qk":
+        x[n] /= np.sqrt((x[n] ** 2).sum(-1, keepdims=True))
+    if what != "keys":
+        x["q"][::2] *= np.float32(size)
+    if what != "queries":
+        x["k"] *= np.float32(size)
+        x["S"][:] = 0
+    out, S = launch(backend, x, [T], 2, 4, 128, 64, l2norm_eps=eps)
+    want, wS, of_S, of_q = running(x, 128 ** -0.5, eps)
+    hold(out, want, (of_S * of_q)[..., None], "out")
+    hold(S[0], wS, of_S[-1][:, None, None], "state")
+
+
+@pytest.mark.parametrize("T", [10, 64, 100])
+@pytest.mark.parametrize("low", [1e-3, 1e-6, 1e-9])
+def test_weak_writes_keep_their_bits(backend, low, T):
+    """Write strengths of all sizes from `low` to 1, growing, on a state of 0: the first rows' results are as small as they are."""
+    x = inputs(np.random.default_rng(T), [T], 1, 2, 64, 64)
+    x["S"][:] = 0
+    x["beta"][:] = np.exp(np.linspace(np.log(low), 0, T))[:, None]
+    out, S = launch(backend, x, [T], 1, 2, 64, 64)
+    want, wS, of_S, of_q = running(x, 0.125, 1e-6)
+    hold(out, want, (of_S * of_q)[..., None], "out")
+    hold(S[0], wS, of_S[-1][:, None, None], "state")
+
+
+@pytest.mark.parametrize("T", [10, 100])
+def test_long_queries_taken_as_they_are(backend, T):
+    x = inputs(np.random.default_rng(T), [T], 1, 2, 64, 64)
+    x["k"] /= np.sqrt((x["k"] ** 2).sum(-1, keepdims=True))
+    x["q"] *= (10.0 ** np.random.default_rng(1).uniform(-6, 6, T)[:, None, None]).astype(np.float32)
+    out, S = launch(backend, x, [T], 1, 2, 64, 64, l2norm_eps=-1.0)
+    want, wS, of_S, of_q = running(x, 0.125, -1.0)
+    hold(out, want, (of_S * of_q)[..., None], "out")
+    hold(S[0], wS, of_S[-1][:, None, None], "state")
