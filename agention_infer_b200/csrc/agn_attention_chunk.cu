@@ -1,13 +1,13 @@
 // Attention of a prompt's rows (consecutive positions of one sequence) over the KV cache, to f32's precision: f32 rows, and f16 rows of head sizes
 // that the tensor-memory form (agn_attention_prompt.cu) does not cover.
 //
-// Bound by the matrix units: per 16 rows, 16 slots and 32 dims 8 products m16n8k16 (f16) for the scores and 8 for the output, which caps the kernel near 276
-// TFLOP/s; what holds it is shared memory (77 % busy, the matrix units 42 %), where each warp's 16 rows read every tile again.  Precision comes from two-part operands
-// as in the decode kernel: queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as hi + lo f16 against the cached bytes.  A CTA takes
-// 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the cache's blocks to f16 rows in shared memory
-// once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 27.8 us (128 CTAs, eight tiles one after the other); 2048 tokens
-// of 28/4 heads of 128: 288 us, 104 TFLOP/s (397 with tf32 parts, blocks taken apart as they were fetched and placed at a tile's end, and queries loaded row by row).  Blocks of four warps, two
-// to an SM, convert every tile twice as often: 256 rows behind 8000 slots 440 -> 847 us.
+// Bound by the matrix units: per 16 rows, 16 slots and 32 dims 8 products m16n8k16 (f16) for the scores and 12 (bf16) for the output, which caps the kernel near 220
+// TFLOP/s; what holds it is shared memory, where each warp's 16 rows read every tile again, and the splitting of the weights.  Precision comes from operands in parts:
+// queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as three bf16 parts against the cached bytes (exact in bf16), and against an
+// f16 cache as two tf32 parts.  A CTA takes 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the
+// cache's blocks to 16-bit rows in shared memory once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 34 us (128 CTAs, eight
+// tiles one after the other); 2048 tokens of 28/4 heads of 128: 351 us, 86 TFLOP/s (f16 cache 325 us).  Blocks of four warps, two to an SM, convert every tile twice as
+// often: 256 rows behind 8000 slots 440 -> 847 us (with the weights as two tf32 parts throughout).
 #include <math.h>
 
 #include "agn_attention_decode.cuh"
@@ -26,13 +26,12 @@ template <int NB> struct ChunkTiles {
     __half q[2][C::ROWS * C::ROW];  // hi, lo
     __half k[2][SL * C::ROW], v[2][SL * C::ROW];
     __align__(16) float ks[2][NB][SL + 8], vs[2][NB][SL + 8], coef[C::ROWS];  // scales of neighbouring slots side by side
-    uint32_t most[3][NB], least[3][NB];  // of the scales of a tile's values that are not 0, as bits of their magnitudes
     int odd;
 };
 
 // One block of 32 values on its way from the cache: 16 words of f16, or 8 words of bytes and a scale.  q8_0 as the words lie in memory: a block that begins at a
 // multiple of 4 is 8 words (scale and bytes) and the last two bytes, one that does not is the scale and 8 words.  Taking them apart is left to place_block, since a
-// use of a loaded word here would wait for it (2048 rows of 28/4 heads of 128, at that step: 397 us, so 374).
+// use of a loaded word here would wait for it (2048 rows of 28/4 heads of 128, with the weights as tf32 parts: 397 us, so 374).
 template <int KV> struct Block {
     uint32_t w[KV == KV_F16 ? 16 : 8];
     uint32_t more;  // q8_0: the two bytes outside the words; words: the scale
@@ -66,8 +65,16 @@ template <int KV> __device__ __forceinline__ void fetch_block(Block<KV> &x, cons
     }
 }
 
-// To 32 f16 values and the block's scale; from: what was fetched (its address, of a q8_0 block); returns whether one of an f16 block is not finite (it becomes 0 where `clean`).
-template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x, const unsigned char *from, __half *to, float *scale, bool clean) {
+// Two of four bytes (as byte + 128) as exact bf16: 128 + the lower seven bits, less 128 or 256 by the upper one (0x4380 is 256, 0x4300 128).
+__device__ __forceinline__ uint32_t bytes_to_bf162(uint32_t u, uint32_t sel) {
+    const uint32_t a = __byte_perm(u & 0x7f7f7f7fu, 0x43434343u, sel), b = __byte_perm(~u & 0x80808080u, 0x43434343u, sel);
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// To 32 values of 16 bits and the block's scale: f16, but bf16 for the bytes of V (is_v), whose weights are bf16 parts.  from: what was fetched (its address, of a q8_0
+// block).  Returns whether one of V's f16 values is not finite (it becomes 0).
+template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x, const unsigned char *from, __half *to, float *scale, bool is_v) {
     bool odd = false;
     uint32_t bytes[8];
     if (KV == KV_WORDS) {
@@ -88,7 +95,7 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
         for (int c = 0; c < 4; c++) {
             if (KV == KV_F16) {
                 h[c] = x.w[4 * i + c];
-                if (clean) {
+                if (is_v) {
                     const bool o0 = (h[c] & 0x7c00u) == 0x7c00u, o1 = (h[c] & 0x7c000000u) == 0x7c000000u;
                     odd |= o0 || o1;
                     if (o0) h[c] &= 0xffff0000u;
@@ -96,7 +103,7 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
                 }
             } else {
                 const uint32_t u = offset_bytes<KV>(bytes[2 * i + (c >> 1)]);
-                h[c] = bytes_to_half2(u, c & 1 ? 0x4342 : 0x4140);
+                h[c] = is_v ? bytes_to_bf162(u, c & 1 ? 0x4342 : 0x4140) : bytes_to_half2(u, c & 1 ? 0x4342 : 0x4140);
             }
         }
         dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -104,16 +111,23 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
     return odd;
 }
 
-// Weights times scales as two f16 parts, V_UP times: at most 2^15 (weights reach 2^8, scales are brought below 2).  The lower part is off by half its smallest step, 2^-25 or
-// 2^-31 of a full weight and scale, whatever the weight: 7 bits below what f32 rounds the sum to, but a weight under 2^-31 is lost, which shows in dims where
-// the values of all larger weights are exactly 0.  Scales that lie further apart than 2^6 take the tf32 products, whose parts have f32's range.
-constexpr float V_UP = 64.0f;
-__device__ __forceinline__ void split_half2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+// Weights have f32's range: a weight however small may meet a value that outweighs it.  Times the scale of a block of bytes they are three bf16 parts (8 bits each; the
+// bytes are exact in bf16), against an f16 cache two tf32 parts (11 bits each; f16 is exact in tf32).  (Two f16 parts under the tile's largest scale, 289 us for 2048 rows
+// of 28/4 heads of 128, lost weights under 2^-25 to 2^-31 of the row's largest.)
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    const auto pair = [](float a, float b) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    };
+    hi = pair(x, y);
+    x = fminf(x - __uint_as_float(hi << 16), 1e35f);  // with an infinite scale not inf - inf
+    y = fminf(y - __uint_as_float(hi & 0xffff0000u), 1e35f);
+    mid = pair(x, y);
+    lo = pair(x - __uint_as_float(mid << 16), y - __uint_as_float(mid & 0xffff0000u));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3},{%4,%5,%6,%7},{%8,%9},{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(agn_smem_u32(p)) : "memory");
@@ -136,10 +150,6 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     const int last_row = min(r0 + C::ROWS, rows) - 1, end = a.pos_start + last_row / G + 1, seen_tiles = (end + SL - 1) / SL;
     const int per_share = (seen_tiles + split.splits - 1) / split.splits, tile0 = min(share * per_share, seen_tiles), tiles = min(seen_tiles, tile0 + per_share);  // tile0 .. tiles - 1
     if (tid == 0) sm.odd = 0;
-    if (KV != KV_F16 && tid < 3 * NB) {
-        sm.most[tid / NB][tid % NB] = 0;
-        sm.least[tid / NB][tid % NB] = 0x7f800000u;
-    }
 
     auto block_at = [&](int n, int tile) {
         return (n < SL * NB ? a.k_cache : a.v_cache) + (int64_t)(tile * SL + n / NB % SL) * a.bytes_per_token + (kvh * NB + n % NB) * F::BYTES;
@@ -154,13 +164,6 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
         if (n >= 2 * SL * NB) return;
         const bool odd = place_block<KV>(x, block_at(n, tile), (is_k ? sm.k : sm.v)[tile & 1] + slot * ROW + b * 32, &(is_k ? sm.ks : sm.vs)[tile & 1][b][slot], !is_k);
         if (KV == KV_F16 && odd) sm.odd = 1;
-        if (KV != KV_F16 && !is_k) {
-            const uint32_t size = __float_as_uint(sm.vs[tile & 1][b][slot]) & 0x7fffffffu;
-            if (size) {
-                atomicMax(&sm.most[tile % 3][b], size);
-                atomicMin(&sm.least[tile % 3][b], size);
-            }
-        }
     };
     constexpr int HELD = NB <= 4 ? C::BLOCKS : 1;  // blocks that wait in registers while a tile is worked on; larger heads have none left for them
     Block<KV> next[HELD];
@@ -181,7 +184,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     if (tile0 < tiles) fetch_tile(tile0);
 
     // ---- Q, a warp's 16 rows: largest value to [1, 2), two f16 parts
-    constexpr int QB = NB <= 4 ? 8 : 4;  // rows whose loads are on their way together (one after the other: 312 us for 2048 rows of 28/4 heads of 128, so 288)
+    constexpr int QB = NB <= 4 ? 8 : 4;  // rows whose loads are on their way together (one after the other: 24 us more for 2048 rows of 28/4 heads of 128)
     for (int i0 = 0; i0 < 16; i0 += QB) {
         float x[QB][NB];
 #pragma unroll
@@ -223,10 +226,6 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     for (int i = 0; i < 4 * NB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
     for (int tile = tile0; tile < tiles; tile++) {
-        if (KV != KV_F16 && tid < NB) {  // of the tile before this one and of the one after the next
-            sm.most[(tile + 2) % 3][tid] = 0;
-            sm.least[(tile + 2) % 3][tid] = 0x7f800000u;
-        }
         if (tile + 1 < tiles) fetch_tile(tile + 1);
         const bool sees = tile * SL <= warp_last;  // a warp whose rows see none of it waits for the others
         const int buf = tile & 1;
@@ -306,67 +305,61 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
             // ---- O += P V; the sums of a tile in the matrix unit (whose adder cuts), the running ones by rounded additions.  Dims 8 c + 2 t4 (+ 1) of the block in o[4 b + c].
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                float acc[4][4], down = 1.0f / V_UP;
+                float acc[4][4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.0f;
-                const uint32_t most = KV == KV_F16 ? 0u : sm.most[tile % 3][b], least = KV == KV_F16 ? 0u : sm.least[tile % 3][b];
-                if (KV == KV_F16 || (most < 0x7f000000u && (most >> 23) <= (least >> 23) + 6)) {
-                    float fold = V_UP;
-                    if (KV != KV_F16) {  // the largest scale to [1, 2)
-                        const uint32_t e = max(most >> 23, 7u);
-                        fold = __uint_as_float((254 + 6 - e) << 23);
-                        down = __uint_as_float((e - 6) << 23);
-                    }
 #pragma unroll
-                    for (int n = 0; n < SL / 8; n += 2) {
-                        uint32_t hi[4], lo[4];
+                for (int n = 0; n < SL / 8; n += 2) {
+                    if (KV == KV_F16) {
+                        float hi[2][4], lo[2][4];
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                hi[u][i] = __uint_as_float((__float_as_uint(s[n + u][i]) + 0x1000u) & 0xffffe000u);
+                                lo[u][i] = s[n + u][i] - hi[u][i];
+                            }
+#pragma unroll
+                        for (int c = 0; c < 4; c += 2) {
+                            uint32_t v[4];  // two groups of eight dims, of eight slots each
+                            ldsm4t(v, sm.v[buf] + (8 * n + (lane & 15)) * ROW + b * 32 + c * 8 + (lane >> 4) * 8);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+                                const int u = k & 1, to = c + (k >> 1);
+                                mma_tf32(acc[to], hi[u][0], hi[u][2], hi[u][1], hi[u][3], f.x, f.y);
+                                mma_tf32(acc[to], lo[u][0], lo[u][2], lo[u][1], lo[u][3], f.x, f.y);
+                            }
+                        }
+                    } else {
+                        uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            float f0 = fold, f1 = fold;
-                            if (KV != KV_F16) {
-                                const float2 f = *reinterpret_cast<const float2 *>(&sm.vs[buf][b][8 * (n + u) + 2 * t4]);
-                                f0 *= f.x;
-                                f1 *= f.y;
+                            const float2 f = *reinterpret_cast<const float2 *>(&sm.vs[buf][b][8 * (n + u) + 2 * t4]);
+                            float w[4] = {s[n + u][0] * f.x, s[n + u][1] * f.y, s[n + u][2] * f.x, s[n + u][3] * f.y};
+                            if (edge) {  // a scale that is not finite, in a slot that the row does not see
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    if (tile * SL + 8 * (n + u) + 2 * t4 + (i & 1) > lim[i >> 1]) w[i] = 0.0f;
                             }
-                            split_half2(s[n + u][0] * f0, s[n + u][1] * f1, hi[2 * u], lo[2 * u]);
-                            split_half2(s[n + u][2] * f0, s[n + u][3] * f1, hi[2 * u + 1], lo[2 * u + 1]);
+                            split_bf16(w[0], w[1], hi[2 * u], mid[2 * u], lo[2 * u]);
+                            split_bf16(w[2], w[3], hi[2 * u + 1], mid[2 * u + 1], lo[2 * u + 1]);
                         }
 #pragma unroll
                         for (int c = 0; c < 4; c += 2) {
                             uint32_t v[4];
                             ldsm4t(v, sm.v[buf] + (8 * n + (lane & 15)) * ROW + b * 32 + c * 8 + (lane >> 4) * 8);
-                            mma_f16(acc[c], hi, v[0], v[1]);
-                            mma_f16(acc[c + 1], hi, v[2], v[3]);
-                            mma_f16(acc[c], lo, v[0], v[1]);
-                            mma_f16(acc[c + 1], lo, v[2], v[3]);
-                        }
-                    }
-                } else {
-                    down = 1.0f;
-#pragma unroll
-                    for (int n = 0; n < SL / 8; n++) {
-                        const float s0 = sm.vs[buf][b][8 * n + 2 * t4], s1 = sm.vs[buf][b][8 * n + 2 * t4 + 1];
-                        float hi[4], lo[4], w[4] = {s[n][0] * s0, s[n][1] * s1, s[n][2] * s0, s[n][3] * s1};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            // a scale that is not finite, in a slot that the row does not see
-                            if (edge && tile * SL + 8 * n + 2 * t4 + (i & 1) > lim[i >> 1]) w[i] = 0.0f;
-                            hi[i] = __uint_as_float(__float_as_uint(w[i]) & 0xffffe000u);
-                            lo[i] = fminf(w[i] - hi[i], 1e35f);  // with an infinite scale not inf - inf
-                        }
-                        const __half *v = sm.v[buf] + (8 * n + 2 * t4) * ROW + b * 32 + g;
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const float e0 = __half2float(v[8 * c]), e1 = __half2float(v[8 * c + ROW]);
-                            mma_tf32(acc[c], hi[0], hi[2], hi[1], hi[3], e0, e1);
-                            mma_tf32(acc[c], lo[0], lo[2], lo[1], lo[3], e0, e1);
+                            mma_bf16(acc[c], hi, v[0], v[1]);
+                            mma_bf16(acc[c + 1], hi, v[2], v[3]);
+                            mma_bf16(acc[c], mid, v[0], v[1]);
+                            mma_bf16(acc[c + 1], mid, v[2], v[3]);
+                            mma_bf16(acc[c], lo, v[0], v[1]);
+                            mma_bf16(acc[c + 1], lo, v[2], v[3]);
                         }
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[4 * b + c][i] = __fmaf_rn(acc[c][i], down, o[4 * b + c][i]);
+                for (int c = 0; c < 4; c++) add4(o[4 * b + c], acc[c]);
             }
         }
         __syncthreads();
