@@ -20,9 +20,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_split_join_kernel(const 
     for (int x = lane; x < split.splits; x += 32) M = fmaxf(M, weight[warp][x] = part[x * stride + hd]);
     M = agn_warp_max(M);
     for (int x = lane; x < split.splits; x += 32) {
-        const float c = ex2(weight[warp][x] - (M == -INFINITY ? 0.0f : M));
-        weight[warp][x] = c;
-        L = __fmaf_rn(c, part[x * stride + hd + 1], L);  // NaN where all of a share's scores are: its maximum is still -inf
+        const float m = weight[warp][x], l = part[x * stride + hd + 1], c = ex2(m - (M == -INFINITY ? 0.0f : M));
+        weight[warp][x] = m == -INFINITY && l == 0.0f ? -1.0f : c;  // -1: nothing in it, not even sums
+        L = __fmaf_rn(c, l, L);  // NaN where all of a share's scores are: its maximum is still -inf
     }
     L = agn_warp_sum(L);
     __syncwarp();
@@ -39,7 +39,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) attn_split_join_kernel(const 
 #pragma unroll 4
         for (int x = 0; x < split.splits; x++) {
             const float c = weight[warp][x];
-            const float4 v = c != 0.0f ? *reinterpret_cast<const float4 *>(part + x * stride + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // an empty share left only its maximum
+            if (c < 0.0f) continue;
+            const float4 v = *reinterpret_cast<const float4 *>(part + x * stride + i);  // sums that are not finite count whatever their weight is
             o.x = __fmaf_rn(c, v.x, o.x); o.y = __fmaf_rn(c, v.y, o.y); o.z = __fmaf_rn(c, v.z, o.z); o.w = __fmaf_rn(c, v.w, o.w);
         }
         o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
