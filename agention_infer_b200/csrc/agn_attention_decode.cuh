@@ -104,8 +104,14 @@ __device__ __forceinline__ float byte_to_float(uint32_t u, int i) {
 // it: with an infinite value lo must not be 0 (0 * inf), with an infinite p it must not be inf - inf, for the sum of
 // the two products to be what the one product would be.
 template <int KV> __device__ __forceinline__ void split_tf32(float p, float &hi, float &lo, uint32_t half = 0) {
-    hi = __uint_as_float((__float_as_uint(p) + half) & 0xffffe000u);  // half: half a step of hi, for a hi that is rounded and used alone
+    hi = __uint_as_float((__float_as_uint(p) + half) & 0xffffe000u);  // half: half a step of hi, for a weight that is rounded and used alone (a row with a NaN among its weights has it in their sum)
     lo = KV == KV_F16 ? fmaxf(p - hi, 1.17549435e-38f) : fminf(p - hi, 1e35f);
+}
+// rounded to tf32, for a weight times scale that is used alone: NaN stays NaN (half a step added to its bits would make it -0)
+__device__ __forceinline__ float round_tf32(float p) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(p));
+    return __uint_as_float(r);
 }
 // four / eight bytes at an address that is a multiple of 4, or (odd) 2 behind one
 __device__ __forceinline__ uint32_t load4_at(const unsigned char *p, bool odd) {
@@ -416,7 +422,9 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                         const uint32_t w = offset_bytes<KV>(load4_at(blk + F::DATA + g * 4, odd));
 #pragma unroll
                         for (int c = 0; c < 4; c++) f[i][c] = byte_to_float(w, c);
-                        split_tf32<KV>(sc[u][i] * block_scale<KV>(blk), ph[u][i], pl[u][i], half);
+                        const float weight = sc[u][i] * block_scale<KV>(blk);
+                        split_tf32<KV>(weight, ph[u][i], pl[u][i]);
+                        if (!lo) ph[u][i] = round_tf32(weight);
                     }
                 }
                 mma_tf32(acc0, f[0][0], f[0][1], f[1][0], f[1][1], ph[u][0], ph[u][1]);
