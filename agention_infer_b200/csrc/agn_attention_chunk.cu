@@ -112,7 +112,7 @@ template <int KV> __device__ __forceinline__ bool place_block(const Block<KV> &x
 }
 
 // Weights have f32's range: a weight however small may meet a value that outweighs it.  Times the scale of a block of bytes they are three bf16 parts (8 bits each; the
-// bytes are exact in bf16), against an f16 cache two tf32 parts (11 bits each; f16 is exact in tf32).  (Two f16 parts under the tile's largest scale, 289 us for 2048 rows
+// bytes are exact in bf16), against an f16 cache two tf32 parts (11 bits each; f16 is exact in tf32).  (Two f16 parts under the tile's largest scale, 287 us for 2048 rows
 // of 28/4 heads of 128, lost weights under 2^-25 to 2^-31 of the row's largest.)
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
     const auto pair = [](float a, float b) {
@@ -183,7 +183,7 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
     __syncthreads();
     if (tile0 < tiles) fetch_tile(tile0);
 
-    // ---- Q, a warp's 16 rows: largest value to [1, 2), two f16 parts
+    // ---- Q, a warp's 16 rows: largest value to [2^14, 2^15), two f16 parts
     constexpr int QB = NB <= 4 ? 8 : 4;  // rows whose loads are on their way together (one after the other: 24 us more for 2048 rows of 28/4 heads of 128)
     for (int i0 = 0; i0 < 16; i0 += QB) {
         float x[QB][NB];
@@ -202,12 +202,12 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
 #pragma unroll
             for (int c = 0; c < NB; c++) amax = fmaxf(amax, fabsf(x[i][c]));
             amax = agn_warp_max(amax);
-            const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);
-            const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-            if (lane == 0) sm.coef[row] = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), 1.17549435e-38f);
+            float up;
+            const float coef = query_scale(amax, a.scale, up);
+            if (lane == 0) sm.coef[row] = coef;
 #pragma unroll
             for (int c = 0; c < NB; c++) {
-                const float v = x[i][c] * down;
+                const float v = x[i][c] * up;
                 const __half h = __float2half_rn(v);
                 sm.q[0][row * ROW + c * 32 + lane] = h;
                 sm.q[1][row * ROW + c * 32 + lane] = __float2half_rn(v - __half2float(h));

@@ -9,7 +9,7 @@
 //
 // Per 8 slots and head, on the matrix units so that the instructions per cached byte stay below what the stream allows:
 //   S = Q K^T as m16n8k16 f16: rows 0-7 hold the upper halves of the (up to 8) query heads, rows 8-15 the lower halves (q = hi + lo, each 11 bits,
-//     after a power of two has brought the row's largest value to [1, 2)), the columns are slots; the cached bytes are exact in f16, so a score
+//     after a power of two has brought the row's largest value to [2^14, 2^15)), the columns are slots; the cached bytes are exact in f16, so a score
 //     keeps 22 bits; block scales are applied to the f32 products of 32 dims.
 //   O^T += V^T P^T as m16n8k8 tf32, twice: p * scale split into two tf32 parts (22 bits, any range), V's bytes exact in tf32; f16 rows take the
 //     upper part alone (their result has 11 bits).  The accumulators of S are P^T's operand layout as they are (columns 2t, 2t + 1 stand for
@@ -87,6 +87,13 @@ __device__ __forceinline__ void add4(float (&o)[4], const float (&x)[4]) {
 template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, bool in) {  // zeros where it is not `in`
     if (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(in ? N : 0) : "memory");
+}
+// The power of two that brings a query row's largest value to [2^14, 2^15), where the two f16 parts keep 22 bits of all values down to 2^-17 of it and lose what is
+// below 2^-39 of it; returns what its scores then have to be multiplied by for the softmax in base 2 (not 0: -inf times that is -inf).
+__device__ __forceinline__ float query_scale(float amax, float scale, float &up) {
+    const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 253);  // 2^(e-127) <= amax < 2^(e-126)
+    up = __uint_as_float((uint32_t)(268 - e) << 23);                        // 2^(141-e)
+    return fmaxf(scale * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 14) << 23), 1.17549435e-38f);
 }
 // four signed (q8_0) or offset-binary (words) bytes, all as byte + 128
 template <int KV> __device__ __forceinline__ uint32_t offset_bytes(uint32_t w) { return KV == KV_Q8 ? w ^ 0x80808080u : w; }
@@ -458,12 +465,11 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
             }
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const int e = min(max((int)(__float_as_uint(amax) >> 23), 1), 253);  // 2^(e-127) <= amax < 2^(e-126)
-            const float down = __uint_as_float((uint32_t)(254 - e) << 23);         // 2^(127-e)
-            coef = fmaxf(a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), 1.17549435e-38f);  // not 0: -inf * coef is -inf
+            float up;
+            coef = query_scale(amax, a.scale, up);
 #pragma unroll
             for (int b = 0; b < 2 * NB; b++) {
-                const float v[4] = {x[b].x * down, x[b].y * down, x[b].z * down, x[b].w * down};
+                const float v[4] = {x[b].x * up, x[b].y * up, x[b].z * up, x[b].w * up};
                 const __half2 h01 = __floats2half2_rn(v[0], v[1]), h23 = __floats2half2_rn(v[2], v[3]);
                 const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
                 const __half2 l01 = __floats2half2_rn(v[0] - f01.x, v[1] - f01.y), l23 = __floats2half2_rn(v[2] - f23.x, v[3] - f23.y);
