@@ -6,7 +6,7 @@
 // queries as hi + lo f16 against the cached bytes (exact in f16), weights times the block scale as three bf16 parts against the cached bytes (exact in bf16), and against an
 // f16 cache as two tf32 parts.  A CTA takes 16 rows per warp of one KV head - row r is (token r / G, head r % G) - and 64 slots at a time, which it brings from the
 // cache's blocks to 16-bit rows in shared memory once for all warps, the next 64 while these are worked on.  512 tokens of 32/8 heads of 64, q8_0: 34 us (128 CTAs, eight
-// tiles one after the other); 2048 tokens of 28/4 heads of 128: 351 us, 86 TFLOP/s (f16 cache 325 us).  Blocks of four warps, two to an SM, convert every tile twice as
+// tiles one after the other); 2048 tokens of 28/4 heads of 128: 351 us, 86 TFLOP/s (f16 cache 324 us).  Blocks of four warps, two to an SM, convert every tile twice as
 // often: 256 rows behind 8000 slots 440 -> 847 us (with the weights as two tf32 parts throughout).
 #include <math.h>
 
@@ -239,7 +239,6 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                 float blk[SL / 8][4];
 #pragma unroll
                 for (int n = 0; n < SL / 8; n++) blk[n][0] = blk[n][1] = blk[n][2] = blk[n][3] = 0.0f;
-                float(*acc)[4] = KV == KV_F16 ? s : blk;
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     uint32_t hi[4], lo[4];
@@ -250,13 +249,16 @@ template <int KV, int NB> __global__ void __launch_bounds__(ChunkShape<NB>::THRE
                     for (int n = 0; n < SL / 8; n += 2) {
                         uint32_t kf[4];  // two groups of eight slots
                         ldsm4(kf, sm.k[buf] + (n * 8 + (lane & 7) + (lane >> 4) * 8) * ROW + b * 32 + k * 16 + ((lane >> 3) & 1) * 8);
-                        mma_f16(acc[n], hi, kf[0], kf[1]);
-                        mma_f16(acc[n + 1], hi, kf[2], kf[3]);
-                        mma_f16(acc[n], lo, kf[0], kf[1]);
-                        mma_f16(acc[n + 1], lo, kf[2], kf[3]);
+                        mma_f16(blk[n], hi, kf[0], kf[1]);
+                        mma_f16(blk[n + 1], hi, kf[2], kf[3]);
+                        mma_f16(blk[n], lo, kf[0], kf[1]);
+                        mma_f16(blk[n + 1], lo, kf[2], kf[3]);
                     }
                 }
-                if (KV != KV_F16) {
+                if (KV == KV_F16) {  // blocks of dims are added up by rounded additions, too: over all dims the matrix unit's cuts would add up to 6e-6 of a result
+#pragma unroll
+                    for (int n = 0; n < SL / 8; n++) add4(s[n], blk[n]);
+                } else {
 #pragma unroll
                     for (int n = 0; n < SL / 8; n++) {
                         const float2 f = *reinterpret_cast<const float2 *>(&sm.ks[buf][b][8 * n + 2 * t4]);

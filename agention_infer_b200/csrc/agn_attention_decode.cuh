@@ -357,6 +357,11 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                     const uint4 w = *reinterpret_cast<const uint4 *>(krow + b * 64 + t4 * 16);
                     mma_f16(acc, q[2 * b], w.x, w.y);
                     mma_f16(acc, q[2 * b + 1], w.z, w.w);
+                    if (lo) {  // f32 rows: blocks of dims are added up by rounded additions, too (the matrix unit's cuts over all dims reach 6e-6 of a result)
+                        sc[u][0] += acc[0] + acc[2];
+                        sc[u][1] += acc[1] + acc[3];
+                        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                    }
                 } else {
                     float blk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     uint32_t x0, x1;
@@ -369,7 +374,7 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                     sc[u][1] = __fmaf_rn(blk[1] + blk[3], block_scale<KV>(k1 + b * F::BYTES), sc[u][1]);
                 }
             }
-            if (KV == KV_F16) { sc[u][0] = acc[0] + acc[2]; sc[u][1] = acc[1] + acc[3]; }
+            if (KV == KV_F16 && !lo) { sc[u][0] = acc[0] + acc[2]; sc[u][1] = acc[1] + acc[3]; }
         }
         float mt = -INFINITY;
 #pragma unroll
