@@ -350,7 +350,8 @@ AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
  * sequences of [max_seq_len, agn_kv_bytes_per_token(kv_dtype, n_kv_heads * head_dim)] bytes, one after the other;
  * kv_dtype AGN_F16, AGN_Q8_0 or AGN_KV_Q8_0_WORDS.  Two forms:
  *   pos != NULL: row t is the token of position p = pos[t] (device int32) of sequence s = seq[t] (device int32; NULL:
- *     sequence 0) — the decode step of many conversations.  p = -1 sees nothing: its row is 0.  A position outside
+ *     sequence 0) — the decode step of many conversations, whose keys and values one agn_kv_write_f32 writes with positions
+ *     s * max_seq_len + p and n_seqs * max_seq_len (below 2^31) for its max_seq_len.  p = -1 sees nothing: its row is 0.  A position outside
  *     [-1, max_seq_len) or a sequence outside [0, n_seqs) gives a row of zeros and makes the next agn_sync return AGN_EOOB_ID.
  *   pos == NULL: the rows are the positions pos_start + t of the one sequence the caches hold — a prompt, or a
  *     piece of one, whose own keys are already in the cache (seq must be NULL, pos_start + T <= max_seq_len).
