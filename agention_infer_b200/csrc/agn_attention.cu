@@ -139,8 +139,8 @@ int64_t attn_workspace(int64_t T, int n_q, int hd) {
     return T > 0 && T <= ATTN_MAX_SPLIT_ROWS ? (int64_t)2 * 2 * ATTN_MAX_SMS * n_q * (hd + 4) * 4 : 0;
 }
 
-// Few rows of one sequence are quicker as single rows (f32 over q8_0, single rows / chunks, us: 28/4 heads of 128 behind 8000 slots 8 rows 35 / 37, 12 rows 42 / 39, behind
-// 1000 slots 12 rows 18 / 19; 32/8 heads of 128 behind 8000 slots 8 rows 50 / 50, 12 rows 67 / 51).
+// Few rows of one sequence are quicker as single rows (f32 over q8_0, single rows / chunks, us: 28/4 heads of 128 behind 8000 slots 8 rows 35 / 39, 12 rows 43 / 41, behind
+// 1000 slots 12 rows 19 / 18; 32/8 heads of 128 behind 8000 slots 8 rows 53 / 56, 12 rows 70 / 57).
 constexpr int CHUNK_MIN_TOKENS = 12;
 bool chunk_fits(int64_t T, int n_q, int n_kv) { return T >= CHUNK_MIN_TOKENS && T * (n_q / n_kv) < (1LL << 30); }
 

@@ -860,9 +860,9 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
     }
 }
 
-// The chunked form pays from about this many rows a sequence on, on average.  16/32 heads of 128, recurrent / chunked, us: one sequence of 24 rows 20 / 23, of 32
-// 27 / 22, of 128 103 / 40; 32 sequences of 24 rows 173 / 224, of 32 226 / 226, of 128 869 / 376.
-constexpr int CHUNK_MIN_ROWS = 32;
+// The chunked form pays from about this many rows a sequence on, on average.  16/32 heads of 128, recurrent / chunked, us: one sequence of 32 rows 27 / 28, of 40
+// 34 / 28, of 128 102 / 46; 32 sequences of 32 rows 227 / 298, of 40 280 / 299, of 48 335 / 304, of 128 870 / 519.
+constexpr int CHUNK_MIN_ROWS = 40;
 bool delta_chunked(int64_t T, int64_t n_seqs) { return T >= CHUNK_MIN_ROWS * n_seqs; }
 
 struct ChunkLayout {
