@@ -11,9 +11,9 @@
 //   S = Q K^T as m16n8k16 f16: rows 0-7 hold the upper halves of the (up to 8) query heads, rows 8-15 the lower halves (q = hi + lo, each 11 bits,
 //     after a power of two has brought the row's largest value to [2^14, 2^15)), the columns are slots; the cached bytes are exact in f16, so a score
 //     keeps 22 bits; block scales are applied to the f32 products of 32 dims.
-//   O^T += V^T P^T as m16n8k8 tf32, twice: p * scale split into two tf32 parts (22 bits, any range), V's bytes exact in tf32; f16 rows take the
-//     upper part alone (their result has 11 bits).  The accumulators of S are P^T's operand layout as they are (columns 2t, 2t + 1 stand for
-//     slots t, t + 4).
+//   O^T += V^T P^T as m16n8k8 tf32, twice: p * scale split into two tf32 parts (22 bits, any range), V's bytes exact in tf32.
+//     The accumulators of S are P^T's operand layout as they are (columns 2t, 2t + 1 stand for slots t, t + 4).  f16 rows take both parts too: the upper one alone
+//     saves 5 % over words and nothing over an f16 cache, and is off by 2.8e-4 instead of the 2.1e-4 that rounding the result costs.
 // The running maximum is a reference that is moved only when a row has outgrown it by 2^8, so that the accumulators are rarely rescaled.
 #pragma once
 #include <math.h>
@@ -110,15 +110,9 @@ __device__ __forceinline__ float byte_to_float(uint32_t u, int i) {
 // p = hi + lo, hi with tf32's 11 bits (cut) and lo what is left of it.  The values it is multiplied by may not be finite, or the scale in
 // it: with an infinite value lo must not be 0 (0 * inf), with an infinite p it must not be inf - inf, for the sum of
 // the two products to be what the one product would be.
-template <int KV> __device__ __forceinline__ void split_tf32(float p, float &hi, float &lo, uint32_t half = 0) {
-    hi = __uint_as_float((__float_as_uint(p) + half) & 0xffffe000u);  // half: half a step of hi, for a weight that is rounded and used alone (a row with a NaN among its weights has it in their sum)
+template <int KV> __device__ __forceinline__ void split_tf32(float p, float &hi, float &lo) {
+    hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
     lo = KV == KV_F16 ? fmaxf(p - hi, 1.17549435e-38f) : fminf(p - hi, 1e35f);
-}
-// rounded to tf32, for a weight times scale that is used alone: NaN stays NaN (half a step added to its bits would make it -0)
-__device__ __forceinline__ float round_tf32(float p) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(p));
-    return __uint_as_float(r);
 }
 // four / eight bytes at an address that is a multiple of 4, or (odd) 2 behind one
 __device__ __forceinline__ uint32_t load4_at(const unsigned char *p, bool odd) {
@@ -338,8 +332,6 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
     int seg_start = cur.j, stage_at = 0, fill_at = (d.stages - 1) * stage_bytes;  // bytes of the stage that is read, of the one that is filled
     const int lane_k = unit * NB * F::BYTES + (group * PER + (g >> 1) + (g & 1) * 4) * RS;  // the slot whose key this lane reads
     const int lane_s = unit * NB * F::BYTES + (group * PER + t4) * RS;                      // the first slot whose score and value it holds
-    const bool lo = !d.act16;
-    const uint32_t half = lo ? 0u : 0x1000u;
 
     // Slots cur.j + group * PER + 8 u + t4 (+ 4); EDGE: some of them are behind the row's end.
     auto slots = [&](auto edge) {
@@ -357,11 +349,10 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                     const uint4 w = *reinterpret_cast<const uint4 *>(krow + b * 64 + t4 * 16);
                     mma_f16(acc, q[2 * b], w.x, w.y);
                     mma_f16(acc, q[2 * b + 1], w.z, w.w);
-                    if (lo) {  // f32 rows: blocks of dims are added up by rounded additions, too (the matrix unit's cuts over all dims reach 6e-6 of a result)
-                        sc[u][0] += acc[0] + acc[2];
-                        sc[u][1] += acc[1] + acc[3];
-                        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-                    }
+                    // blocks of dims are added up by rounded additions, too (the matrix unit's cuts over all dims reach 6e-6 of a result)
+                    sc[u][0] += acc[0] + acc[2];
+                    sc[u][1] += acc[1] + acc[3];
+                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
                 } else {
                     float blk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     uint32_t x0, x1;
@@ -374,7 +365,6 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                     sc[u][1] = __fmaf_rn(blk[1] + blk[3], block_scale<KV>(k1 + b * F::BYTES), sc[u][1]);
                 }
             }
-            if (KV == KV_F16 && !lo) { sc[u][0] = acc[0] + acc[2]; sc[u][1] = acc[1] + acc[3]; }
         }
         float mt = -INFINITY;
 #pragma unroll
@@ -411,8 +401,8 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
         if (KV == KV_F16) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                split_tf32<KV>(sc[u][0], ph[u][0], pl[u][0], half);
-                split_tf32<KV>(sc[u][1], ph[u][1], pl[u][1], half);
+                split_tf32<KV>(sc[u][0], ph[u][0], pl[u][0]);
+                split_tf32<KV>(sc[u][1], ph[u][1], pl[u][1]);
             }
         }
 #pragma unroll
@@ -434,17 +424,13 @@ template <int KV, int NB, int HC> __global__ void __launch_bounds__(ATTN_THREADS
                         const uint32_t w = offset_bytes<KV>(load4_at(blk + F::DATA + g * 4, odd));
 #pragma unroll
                         for (int c = 0; c < 4; c++) f[i][c] = byte_to_float(w, c);
-                        const float weight = sc[u][i] * block_scale<KV>(blk);
-                        split_tf32<KV>(weight, ph[u][i], pl[u][i]);
-                        if (!lo) ph[u][i] = round_tf32(weight);
+                        split_tf32<KV>(sc[u][i] * block_scale<KV>(blk), ph[u][i], pl[u][i]);
                     }
                 }
                 mma_tf32(acc0, f[0][0], f[0][1], f[1][0], f[1][1], ph[u][0], ph[u][1]);
                 mma_tf32(acc1, f[0][2], f[0][3], f[1][2], f[1][3], ph[u][0], ph[u][1]);
-                if (lo) {
-                    mma_tf32(acc0, f[0][0], f[0][1], f[1][0], f[1][1], pl[u][0], pl[u][1]);
-                    mma_tf32(acc1, f[0][2], f[0][3], f[1][2], f[1][3], pl[u][0], pl[u][1]);
-                }
+                mma_tf32(acc0, f[0][0], f[0][1], f[1][0], f[1][1], pl[u][0], pl[u][1]);
+                mma_tf32(acc1, f[0][2], f[0][3], f[1][2], f[1][3], pl[u][0], pl[u][1]);
             }
             add4(o[2 * b], acc0);
             add4(o[2 * b + 1], acc1);

@@ -124,3 +124,20 @@ def test_same_rows_whatever_the_call_beside_them(backend, act):
     for got in (prompt(be, kv, act, q, bufs, 0, T, nkv), single(be, kv, act, q, bufs, np.arange(T), np.zeros(T), 1, T, nkv),
                 np.concatenate([prompt(be, kv, act, q[:61], bufs, 0, T, nkv), prompt(be, kv, act, q[61:], bufs, 61, T, nkv)])):
         norms.hold(got, want, of, q, k[0], T, hd ** -0.5, act)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0", "words"])
+@pytest.mark.parametrize("nq,nkv,hd,T,n,form", [(28, 4, 128, 3, 2000, "rows"), (8, 8, 64, 5, 900, "rows"), (16, 2, 256, 2, 700, "rows"), (6, 3, 96, 1, 5000, "rows"),
+                                                (16, 2, 256, 60, 500, "prompt"), (6, 3, 96, 100, 100, "prompt"), (4, 2, 160, 20, 3000, "prompt")])
+def test_f16_rows_are_rounded_once(backend, kv, nq, nkv, hd, T, n, form):
+    """Single rows, and prompts of head sizes without a form of their own for f16: beside half a step of f16 of each result (2^-11 of it, or of f16's smallest normal
+    number), a row is off by what an f32 row may be."""
+    rng = np.random.default_rng(n)
+    bufs, (k, v) = write(backend, kv, rng.standard_normal((1, n, nkv, hd)), rng.standard_normal((1, n, nkv, hd)), n)
+    q = (1.5 * rng.standard_normal((T, nq, hd))).astype(np.float16)
+    pos = np.arange(n - T, n)
+    got = single(backend, kv, "f16", q, bufs, pos, np.zeros(T), 1, n, nkv) if form == "rows" else prompt(backend, kv, "f16", q, bufs, n - T, n, nkv)
+    want, of = norms.attention(q, k[0], v[0], pos, hd ** -0.5)
+    off = got.astype(np.float64) - want
+    beyond = np.sign(off) * np.maximum(np.abs(off) - 2.0 ** -11 * np.maximum(np.abs(want), 2.0 ** -14), 0)
+    norms.hold(want + beyond, want, of, q, k[0], n, hd ** -0.5, "f32")
