@@ -426,7 +426,7 @@ struct ChunkLayout {
 ChunkLayout chunk_layout(int64_t slots, int64_t T, int n_q, int n_kv, int hd, int sms, bool anywhere = false) {
     ChunkLayout l;
     l.row_tiles = (int)((T * (n_q / n_kv) + chunk_rows(hd) - 1) / chunk_rows(hd));
-    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 1.0 + 0.033 * hd, T * n_q, hd, sms);
+    l.splits = (anywhere ? attn_splits_most : attn_splits)((int64_t)l.row_tiles * n_kv, (slots + SL - 1) / SL, 1.0 + 0.041 * hd, T * n_q, hd, sms);
     l.odd = attn_part_bytes(l.splits, T, n_q, hd);
     l.bytes = l.splits > 1 ? l.odd + (n_kv * 4 + 15) / 16 * 16 : 0;
     return l;

@@ -1,8 +1,8 @@
 // Attention of single rows (any position of any sequence) over the KV cache: the decode step.  One .cu per cache layout instantiates the kernel.
 //
 // A slot's 2 * bytes_per_token bytes are read once for all query heads, which bounds it by HBM in principle; what holds it is the issue of instructions (57 % of the
-// slots of 16 warps an SM, 374 instructions per 8 slots and head): 64 rows of up to 32768 slots, 28/4 heads of 128, q8_0 in words, 1.24 GB in 329-340 us, 3.7 TB/s;
-// 8 rows of 5000 to 8192 f16 slots, 32/8 heads of 128, 59-60 us, 3.9 TB/s.  What a CTA works on is a run of tiles of TT slots: all
+// slots of 16 warps an SM, 368 instructions per 8 slots and head): 64 rows of up to 32768 slots, 28/4 heads of 128, q8_0 in words, 1.24 GB in 323-328 us, 3.8 TB/s;
+// 8 rows of 5000 to 8192 f16 slots, 32/8 heads of 128, 59.7 us, 3.8 TB/s.  What a CTA works on is a run of tiles of TT slots: all
 // rows' tiles are numbered one after the other and shared out evenly (a batch of very different lengths, or one long row, fills the GPU alike);
 // a row that falls into several CTAs is joined by attn_join_kernel.  Tiles arrive by cp.async in a ring of stages, all KV heads of a slot
 // together, and each warp takes one KV head (and a share of the tile's slots where there are fewer than 8).

@@ -38,7 +38,7 @@ __device__ __forceinline__ void delta_rows(const DeltaArgs &a, int64_t s, int64_
 // sequences on).  A CTA holds 32 columns of one head's state in registers: they evolve independently of the other columns, so a
 // single sequence of 32 heads of 128 already gives 128 CTAs.  Thread (row group rg = 0..15, column quad c4): rows rg + 16 i.
 // k^T S and q^T S are taken from the same old state in one pass (o = a q^T S + (q.k) d), so a token costs one exchange
-// between the four warps.  64 sequences of one row, 16/32 heads of 128: 47-49 us, 5.8 TB/s.
+// between the four warps.  64 sequences of one row, 16/32 heads of 128: 49 us, 5.5 TB/s.
 constexpr int TB = 8;  // tokens whose q, k, v are staged at a time
 template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kernel(const __grid_constant__ DeltaArgs a) {
     agn_pdl_prologue();
@@ -147,7 +147,7 @@ template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kern
 // columns of one head's state from chunk to chunk (the columns are independent: 128 CTAs for one sequence of 32 heads of 128).
 //
 // Bound by the matrix units (59 % busy on the SMs at work: 1.05 M multiply-adds per chunk and 32 columns, three times over, at tf32's rate) and by the waits between
-// dependent products; a chunk takes 6 us.  4096 rows of 16/32 heads of 128: 87 us of preparation and 390 us of chunks.  Every product is taken in two parts of 11
+// dependent products; a chunk takes 6 us.  4096 rows of 16/32 heads of 128: 92 us of preparation and 388 us of chunks.  Every product is taken in two parts of 11
 // bits each, x = hi + lo, as hi hi + hi lo + lo hi, summed in f32.  K, Q, N and P are f16 parts in the workspace, every row brought to UP by a power of two of its own
 // (its largest entry; a row of one product is a row of the result, which takes the factor back), so that a small key, query or write strength keeps its bits;
 // f16 is exact in tf32.  S, V - c K S, D and r D stay f32 in shared memory and are split into tf32 parts, which have f32's range, as they are read: columns do not share a

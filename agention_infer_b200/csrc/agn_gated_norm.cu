@@ -81,7 +81,7 @@ void launch_rows(agn_ctx *ctx, bool vec, const float *x, const float *gate, cons
 
 template <typename OT, int VPT>
 void launch_vpt(agn_ctx *ctx, bool vec, const float *x, const float *gate, const float *w, OT *out, int64_t rows, int n, float eps) {
-    // Two short rows per warp once they fill the GPU that way: 131072 rows of 128 in 30.8 us (6.53 TB/s); one row 36.0 us, four 31.4.  Fewer rows are
+    // Two short rows per warp once they fill the GPU that way: 131072 rows of 128 in 31 us (6.4 TB/s); one row 36 us, four 31.4.  Fewer rows are
     // over sooner the more warps they are.
     constexpr int R = VPT == 1 ? 2 : 1;
     if (R > 1 && rows >= (int64_t)4 * R * 8 * ctx->sm_count) launch_rows<OT, VPT, R>(ctx, vec, x, gate, w, out, rows, n, eps);
