@@ -91,7 +91,7 @@ template <int N> __device__ __forceinline__ void cp_async(uint32_t dst, const vo
 // The power of two that brings a query row's largest value to [2^14, 2^15), where the two f16 parts keep 22 bits of all values down to 2^-17 of it and lose what is
 // below 2^-39 of it; returns what its scores then have to be multiplied by for the softmax in base 2 (not 0: -inf times that is -inf).
 __device__ __forceinline__ float query_scale(float amax, float scale, float &up) {
-    const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 253);  // 2^(e-127) <= amax < 2^(e-126)
+    const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254);  // 2^(e-127) <= amax < 2^(e-126)
     up = __uint_as_float((uint32_t)(268 - e) << 23);                        // 2^(141-e)
     return fmaxf(scale * 1.4426950408889634f * __uint_as_float((uint32_t)(e - 14) << 23), 1.17549435e-38f);
 }

@@ -33,3 +33,25 @@ def test_small_queries_beside_large_ones(backend, form, hd, nq, nkv, T, start, s
     G = nq // nkv
     most = scale * max((np.abs(q[:, h].astype(np.float64)) @ np.abs(ck[:, h // G]).T).max() for h in range(nq))
     assert np.all(np.linalg.norm(got - want, axis=2) <= (18 * most + 16) * 2.0 ** -22 * size)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0", "words"])
+@pytest.mark.parametrize("size,scale", [(3.4025e38, 2e-38), (3.4e38, 2e-38), (1e30, 1e-30), (1e-30, 1e30), (1e-36, 1e36)])
+@pytest.mark.parametrize("form", ["prompt", "single rows"])
+def test_queries_at_the_ends_of_f32s_range(backend, form, size, scale, kv):
+    be, hd, nq, nkv, T, n = backend, 64, 4, 2, 20, 90
+    rng = np.random.default_rng(5)
+    scale = float(np.float32(scale))
+    q = (np.where(rng.random((T, nq, hd)) < 0.5, -1, 1) * size * (np.arange(hd) == 3) + 0.1 * size * rng.uniform(-1, 1, (T, nq, hd)) * (np.arange(hd) != 3)).astype(np.float32)
+    k, v = (rng.standard_normal((n, nkv * hd)).astype(np.float32) for _ in range(2))
+    bpt = be.kv_bytes_per_token(KV[kv], nkv * hd)
+    bufs = [be.upload(np.zeros(n * bpt, np.uint8)) for _ in range(2)]
+    be.kv_write(KV[kv], be.upload(k), be.upload(v), bufs[0], bufs[1], n, nkv * hd, None, n)
+    kw = dict(pos_start=n - T) if form == "prompt" else dict(pos=be.upload(np.arange(n - T, n, dtype=np.int32)))
+    got = be.read(be.launch_attention_kv(be.upload(q), bufs[0], bufs[1], KV[kv], T, nq, nkv, hd, n, scale=scale, **kw), np.float32, q.shape)
+    be.sync()
+    ck, cv = (ref.cache_values(KV[kv], be.read(b, np.uint8, (n, bpt)), nkv * hd).reshape(n, nkv, hd) for b in bufs)
+    want, of = norms.attention(q, ck, cv, [n - T + t for t in range(T)], scale)
+    # as above; and the scale's own last bit, where it is close to f32's smallest numbers
+    most = scale * max((np.abs(q[:, h].astype(np.float64)) @ np.abs(ck[:, h // 2]).T).max() for h in range(nq))
+    assert np.all(np.linalg.norm(got - want, axis=2) <= (18 * most + 16) * 2.0 ** -22 * of)
