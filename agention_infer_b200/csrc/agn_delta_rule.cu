@@ -153,8 +153,8 @@ template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kern
 // f16 is exact in tf32.  S, V - c K S, D and r D stay f32 in shared memory and are split into tf32 parts, which have f32's range, as they are read: columns do not share a
 // scale, so that one of another size, a large row later in the chunk or a state that has decayed takes no bits from the rest.  (f16 parts under one power of two per 32
 // columns and chunk, at m16n8k16's double rate: 239 us of chunks, but a column 2^-20 of its neighbour had ten bits left.  bf16 for the two mixed products: 367 us, twice the
-// error.  Sixteen workers of eight columns each: 430 us.)  Errors do not grow from row to row where 0 <= beta <= 2, g <= 0, |k| <= 1 and numbers are finite: a
-// chunk that is not so is computed row by row in f32 instead.
+// error.  Sixteen workers of eight columns each: 430 us.)  Errors do not grow from row to row where 0 <= beta <= 2, g <= 0, |k| <= 1, and products do not
+// overflow where states and values are below 2^112: a chunk that is not so is computed row by row in f32 instead.
 constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 128;
 constexpr float UP = 1024.0f, DOWN = 1.0f / UP;  // rows' largest entries lie in [UP, 2 UP); what is kept of the others is 2^-35 of that or better
 
@@ -501,7 +501,7 @@ template <int DK> struct ChunkSmem {
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
     float s[DK * BROW], xx[CH * BROW], dd[CH * BROW], dr[CH * BROW];  // S and V - c K S and D, times DOWN; r D times K's factors
     float v[2][CH * VROW], factors[2][ROW_FACTORS];
-    int bad[9];  // the state's columns of each worker, the chunk's values: not all finite
+    int bad[9];  // the state's columns of each worker, the chunk's values: some are not finite, or too large
     uint64_t kq_full, v_full, n_full, p_full, kq_free, n_free, p_free;
     int gave_up;
 };
@@ -607,7 +607,12 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         const float *f = x.factors + ((slot0 + c) * d.n_v + hv) * ROW_FACTORS;
         for (int i = 4 * lane; i < ROW_FACTORS; i += 128) cp16(sm.factors[c & 1] + i, f + i);
     };
-    auto tell_finite = [&](float sum) {  // of differences x - x: 0 where every x is finite, NaN otherwise
+    // 0 where x is below 2^112, NaN otherwise: where it is not finite, or so large that a product with rows that have been brought up could overflow
+    auto beyond = [](float x) {
+        const float y = x * 65536.0f;
+        return y - y;
+    };
+    auto tell_beyond = [&](float sum) {
         const bool bad = __any_sync(0xffffffffu, !(sum == 0.0f));
         if (lane == 0) sm.bad[warp] = bad;
     };
@@ -647,9 +652,9 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
 #pragma unroll
                 for (int i = 0; i < CH * 8 / 32; i++) {
                     const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
-                    sum += ((y.x - y.x) + (y.y - y.y)) + ((y.z - y.z) + (y.w - y.w));
+                    sum += (beyond(y.x) + beyond(y.y)) + (beyond(y.z) + beyond(y.w));
                 }
-                tell_finite(sum);
+                tell_beyond(sum);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.v_full);
             } else if (lane == 0) {
@@ -674,8 +679,8 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
     auto tell_state = [&] {
         float sum = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NU; n++) sum += ((S[n][0] - S[n][0]) + (S[n][1] - S[n][1])) + ((S[n][2] - S[n][2]) + (S[n][3] - S[n][3]));
-        tell_finite(sum);
+        for (int n = 0; n < NU; n++) sum += (beyond(S[n][0]) + beyond(S[n][1])) + (beyond(S[n][2]) + beyond(S[n][3]));
+        tell_beyond(sum);
     };
     tell_state();
     for (int64_t c = 0; c < chunks; c++) {

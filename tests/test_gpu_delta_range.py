@@ -146,3 +146,24 @@ def test_long_queries_taken_as_they_are(backend, T):
     want, wS, of_S, of_q = running(x, 0.125, -1.0)
     hold(out, want, (of_S * of_q)[..., None], "out")
     hold(S[0], wS, of_S[-1][:, None, None], "state")
+
+
+@pytest.mark.parametrize("T", [10, 150])
+@pytest.mark.parametrize("size", [1e34, 1e36, 2e37])
+@pytest.mark.parametrize("what", ["all", "the state", "a state along the keys", "a late value"])
+def test_near_the_end_of_f32s_range(backend, what, size, T):
+    """What stays finite token by token stays finite, and exact, whatever the form."""
+    x = inputs(np.random.default_rng(T), [T], 1, 2, 128, 64)
+    if what == "all":
+        x["v"] *= np.float32(size)
+    if what == "a state along the keys":  # sums of 128 terms of one sign
+        x["k"][:], x["S"][:] = 1, 0.3 * size
+    elif what != "a late value":
+        x["S"] *= np.float32(size)
+    else:
+        x["v"][T - 3, 1, 5] = size
+    out, S = launch(backend, x, [T], 1, 2, 128, 64)
+    want, wS = expected(x, [T], 128 ** -0.5, 1e-6)
+    of = columns(x, want, wS)
+    hold(out, want, of[None], "out")
+    hold(S[0], wS[0], of[:, None], "state")
