@@ -153,8 +153,8 @@ template <int DK> __global__ void __launch_bounds__(128, 6) delta_recurrent_kern
 // f16 is exact in tf32.  S, V - c K S, D and r D stay f32 in shared memory and are split into tf32 parts, which have f32's range, as they are read: columns do not share a
 // scale, so that one of another size, a large row later in the chunk or a state that has decayed takes no bits from the rest.  (f16 parts under one power of two per 32
 // columns and chunk, at m16n8k16's double rate: 239 us of chunks, but a column 2^-20 of its neighbour had ten bits left.  bf16 for the two mixed products: 367 us, twice the
-// error.  Sixteen workers of eight columns each: 430 us.)  Errors do not grow from row to row where 0 <= beta <= 2, g <= 0, |k| <= 1, and products do not
-// overflow where states and values are below 2^112: a chunk that is not so is computed row by row in f32 instead.
+// error.  Sixteen workers of eight columns each: 430 us.)  Errors do not grow from row to row where 0 <= beta <= 2, g <= 0 and |k| <= 1; products neither
+// overflow nor lose their lower parts where the largest state or value lies between 2^-90 and 2^112.  A chunk that is not so is computed row by row in f32 instead.
 constexpr int CH = 64, CHUNK_THREADS = 256, CARRY_THREADS = CHUNK_THREADS + 128;
 constexpr float UP = 1024.0f, DOWN = 1.0f / UP;  // rows' largest entries lie in [UP, 2 UP); what is kept of the others is 2^-35 of that or better
 
@@ -501,7 +501,7 @@ template <int DK> struct ChunkSmem {
     __half k[2][2][CH * KROW], q[2][CH * KROW], n[2][CH * NROW], p[2][CH * NROW];
     float s[DK * BROW], xx[CH * BROW], dd[CH * BROW], dr[CH * BROW];  // S and V - c K S and D, times DOWN; r D times K's factors
     float v[2][CH * VROW], factors[2][ROW_FACTORS];
-    int bad[9];  // the state's columns of each worker, the chunk's values: some are not finite, or too large
+    uint32_t most[9];  // the largest magnitude in the state's columns of each worker, in the chunk's values
     uint64_t kq_full, v_full, n_full, p_full, kq_free, n_free, p_free;
     int gave_up;
 };
@@ -607,15 +607,11 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         const float *f = x.factors + ((slot0 + c) * d.n_v + hv) * ROW_FACTORS;
         for (int i = 4 * lane; i < ROW_FACTORS; i += 128) cp16(sm.factors[c & 1] + i, f + i);
     };
-    // 0 where x is below 2^112, NaN otherwise: where it is not finite, or so large that a product with rows that have been brought up could overflow
-    auto beyond = [](float x) {
-        const float y = x * 65536.0f;
-        return y - y;
+    auto tell_largest = [&](uint32_t most) {  // magnitudes as bits: NaN above infinity above the numbers
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) sm.most[warp] = most;
     };
-    auto tell_beyond = [&](float sum) {
-        const bool bad = __any_sync(0xffffffffu, !(sum == 0.0f));
-        if (lane == 0) sm.bad[warp] = bad;
-    };
+    auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
     // a bounded wait; once one has run out the CTA's other waits give up after their next poll
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         for (int left = x.spin; left > 0; left -= 1024) {
@@ -648,13 +644,13 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
                 load_v(c);
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 const float *v = sm.v[c & 1];
-                float sum = 0.0f;
+                uint32_t most = 0;
 #pragma unroll
                 for (int i = 0; i < CH * 8 / 32; i++) {
                     const float4 y = *reinterpret_cast<const float4 *>(v + ((lane >> 3) + 4 * i) * VROW + (lane & 7) * 4);
-                    sum += (beyond(y.x) + beyond(y.y)) + (beyond(y.z) + beyond(y.w));
+                    most = max(most, max(max(bits(y.x), bits(y.y)), max(bits(y.z), bits(y.w))));
                 }
-                tell_beyond(sum);
+                tell_largest(most);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.v_full);
             } else if (lane == 0) {
@@ -677,10 +673,10 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         if (lane == 0) mbar_arrive(bar);
     };
     auto tell_state = [&] {
-        float sum = 0.0f;
+        uint32_t most = 0;
 #pragma unroll
-        for (int n = 0; n < NU; n++) sum += (beyond(S[n][0]) + beyond(S[n][1])) + (beyond(S[n][2]) + beyond(S[n][3]));
-        tell_beyond(sum);
+        for (int n = 0; n < NU; n++) most = max(most, max(max(bits(S[n][0]), bits(S[n][1])), max(bits(S[n][2]), bits(S[n][3]))));
+        tell_largest(most);
     };
     tell_state();
     for (int64_t c = 0; c < chunks; c++) {
@@ -688,9 +684,10 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
         const int rows = (int)(e - first < CH ? e - first : CH);
         const uint32_t turn = c & 1;
         if ((gave_up = workers_sync_or(!(wait(&sm.kq_full, turn) && wait(&sm.v_full, turn))))) break;
-        int bad = 0;
+        uint32_t most = 0;
 #pragma unroll
-        for (int w = 0; w < 9; w++) bad |= sm.bad[w];
+        for (int w = 0; w < 9; w++) most = max(most, sm.most[w]);
+        const bool bad = most >= 0x77800000u || (most > 0 && most < 0x12800000u);  // 2^112 and more, not finite; all below 2^-90
         const int odd_next = c + 1 < chunks ? x.odd[(slot0 + c + 1) * d.n_v + hv] : 0;
         const float *v = sm.v[c & 1];
         if (odd || bad) {
@@ -711,7 +708,7 @@ template <int DK> __global__ void __launch_bounds__(CARRY_THREADS) delta_chunk_k
             freed(&sm.kq_free);
             freed(&sm.n_free);
             freed(&sm.p_free);
-            workers_sync();  // sm.bad has been read
+            workers_sync();  // sm.most has been read
             tell_state();
             odd = odd_next;
             continue;

@@ -167,3 +167,16 @@ def test_near_the_end_of_f32s_range(backend, what, size, T):
     of = columns(x, want, wS)
     hold(out, want, of[None], "out")
     hold(S[0], wS[0], of[:, None], "state")
+
+
+@pytest.mark.parametrize("T", [10, 64, 150])
+@pytest.mark.parametrize("size", [1e-28, 1e-31, 1e-33, 1e-35])
+def test_near_the_smallest_numbers_of_f32(backend, size, T):
+    x = inputs(np.random.default_rng(T), [T], 1, 2, 64, 64)
+    x["v"] *= np.float32(size)
+    x["S"] *= np.float32(size)
+    out, S = launch(backend, x, [T], 1, 2, 64, 64)
+    want, wS = expected(x, [T], 0.125, 1e-6)
+    of = columns(x, want, wS)
+    hold(out, want, of[None], "out")
+    hold(S[0], wS[0], of[:, None], "state")
