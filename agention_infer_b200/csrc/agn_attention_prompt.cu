@@ -13,7 +13,7 @@
 //   serves the whole group - as two tiles of 128, so that the tensor cores work on one tile while the softmax of the other
 //   runs.  Warps 0-3 and 4-7: softmax of the two tiles, a row per thread; warp 8 fetches tiles; warp 9 issues the products.
 //   TMEM: S0, S1, O0, O1 (128 columns each); the weights overwrite their scores as f16 and are the A operand of the second
-//   product from there.  The output is rescaled only when a row's maximum has grown by more than 2^8 (weights stay below f16's
+//   product from there.  The output is rescaled only when a row's maximum has grown by more than 2^8 (weights stay in f16's
 //   range; sums and accumulators are f32).
 #include <math.h>
 
@@ -21,6 +21,9 @@
 
 namespace {
 
+// The reference is W_UP powers of two below a row's maximum, so that weights reach 2^W_UP and, with the 2^8 that a row may outgrow it by, stay below 2^15: f16 then keeps
+// its 11 bits down to 2^-21 of a row's largest weight (light slots may have the larger values) and something down to 2^-32.
+constexpr float W_UP = 7.0f;
 constexpr int TILE = 128, PROMPT_THREADS = 320, SLOTS = 5, DRAIN_POLLS = AGN_MBAR_SPIN_LIMIT_DEFAULT;  // the last waits are not cut short by the option
 
 struct PromptArgs {
@@ -405,10 +408,10 @@ template <int HD> __global__ void __launch_bounds__(PROMPT_THREADS, 1) attn_prom
             // Where a row's maximum has grown by more than 2^8 (its first piece, and rarely after that), everything taken against the old one is scaled: the sums, the
             // output of earlier tiles, the weights of this tile's first `done` pieces.
             auto grown = [&](float mt, int done) {
-                const bool grow = mt > m + 8.0f;
+                const bool grow = mt > m + (8.0f + W_UP);
                 if (!__any_sync(0xffffffffu, grow)) return;
-                const float f = grow ? ex2(m - mt) : 1.0f;
-                if (grow) m = mt;
+                const float f = grow ? ex2(m - (mt - W_UP)) : 1.0f;
+                if (grow) m = mt - W_UP;
                 l *= f;
                 sum.x *= f;
                 sum.y *= f;

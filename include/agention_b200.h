@@ -346,7 +346,7 @@ AGN_API int64_t agn_kv_bytes_per_token(int32_t kv_dtype, int64_t head_dim_kv);
  *   out[t,h] = sum_j softmax_j(scale * q[t,h] . K[s,j,h/G]) V[s,j,h/G],  j = 0 .. p,  G = n_q_heads / n_kv_heads
  * q, out: [T, n_q_heads, head_dim], f32 or f16.  Sums and softmax are f32 in both; operands are taken in
  * parts of 22 bits or more together, so that f32 rows keep f32's precision and f16 rows are rounded once.  Prompts of f16 rows (8 or more, head sizes 64 and 128)
- * round weights, keys and values to f16 as well; those that see keys or values which f16 does not hold - 65520 and more, or keys all below 2^-14 - are
+ * round weights (2^7 times them: 11 bits down to 2^-21 of a row's largest, 0 below 2^-32), keys and values to f16 as well; those that see keys or values which f16 does not hold - 65520 and more, or keys all below 2^-14 - are
  * computed in f32, slowly.  Caches: n_seqs
  * sequences of [max_seq_len, agn_kv_bytes_per_token(kv_dtype, n_kv_heads * head_dim)] bytes, one after the other;
  * kv_dtype AGN_F16, AGN_Q8_0 or AGN_KV_Q8_0_WORDS.  Two forms:

@@ -59,3 +59,25 @@ def test_light_slots_of_large_values_throughout(backend, hd, T, start, bits, kv,
     weight[:100] = 1
     v[:100] = rng.uniform(1, 2, (100, 2, hd)) * small
     run(backend, kv, "prompt", hd, T, weight, v, bits)
+
+
+@pytest.mark.parametrize("hd,T,start", [(128, 40, 150), (64, 300, 0), (128, 16, 3000), (64, 70, 130)])
+@pytest.mark.parametrize("bits", [10, 14, 17, 20])
+def test_light_slots_of_f16_prompts(backend, hd, T, start, bits):
+    """f16 rows over an f16 cache: a weight of 2^-bits with values that outweigh those of the slot of weight 1 by as much."""
+    be, nq, nkv, n = backend, 4, 2, start + T
+    rng, scale = np.random.default_rng(bits), hd ** -0.5
+    weight, v = np.full(n, 2.0 ** -30), rng.uniform(-2, 2, (n, nkv, hd)) * 1e-3
+    weight[2], weight[n // 2] = 1, 2.0 ** -bits
+    v[n // 2] *= 2.0 ** bits
+    one = np.where(rng.random(hd) < 0.5, -1.0, 1.0)
+    k = ((np.log(weight) / (scale * hd))[:, None, None] * one + 1e-3 * rng.standard_normal((n, nkv, hd))).astype(np.float16)
+    v = np.ascontiguousarray(v, np.float16)
+    q = (one + 0.01 * rng.standard_normal((T, nq, hd))).astype(np.float16)
+    bufs = [be.upload(x.reshape(n, -1)) for x in (k, v)]
+    got = be.read(be.launch_attention_kv(be.upload(q), bufs[0], bufs[1], AGN_F16, T, nq, nkv, hd, n, pos_start=start, act_dtype=AGN_F16), np.float16, q.shape)
+    k, v = k.astype(np.float64), v.astype(np.float64)
+    want, size = norms.attention(q, k, v, [start + t for t in range(T)], scale)
+    # queries, keys and values are f16 as they are: a weight is rounded once (2^-11) and the result once (2^-11, or 2^-25 for its subnormals); scores as for f32 rows
+    most = scale * np.abs(q).astype(np.float64).max() * np.abs(k).sum(axis=2).max()
+    assert np.all(np.linalg.norm(got - want, axis=2) <= (2.0 ** -10 + 10 * most * 2.0 ** -22) * size + 2.0 ** -25 * hd ** 0.5)
