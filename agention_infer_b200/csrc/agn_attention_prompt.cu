@@ -2,7 +2,7 @@
 //
 // Bound by the tensor cores (4 * head_dim flop per row, head and slot) and, equally, by the exponentials (16 a clock and SM
 // against 128 x 128 products of 128 in 1024 clocks); what holds it is the way from scores to weights to the next scores.  4096 tokens of 28/4 heads of 128, q8_0:
-// 154-158 us with the unpacking (8), 760-780 TFLOP/s; 1001 tokens behind 7001 slots, 32/8 heads of 128: 172 us.  Keys, values and weights are rounded to f16, for
+// 154-159 us with the unpacking (8), 760-780 TFLOP/s; 1001 tokens behind 7001 slots, 32/8 heads of 128: 172 us.  Keys, values and weights are rounded to f16, for
 // one product each instead of two and three: rows are off by 4.7e-4 to 5.4e-4 of their norm, where rounding the result alone costs 2.1e-4.  Two kernels:
 //
 //   attn_unpack_kernel writes the sequence's K and V as f16 tiles of 128 slots of one head, each the very bytes that the matrix
